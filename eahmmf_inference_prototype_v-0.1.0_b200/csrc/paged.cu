@@ -1,0 +1,790 @@
+// paged.cu -- the paged key/value cache on sm_100a: rotary positions with the append of new keys and values,
+// attention of new tokens over the pages, and copies of whole pages.
+//
+// A pool holds pages [n_kv][page][hd]; a page of one kv head is one contiguous run, so 16 positions of a head
+// (PAGE_MIN) are contiguous too and a warp that takes 16 of them needs one page id.
+//
+//   k_rope_append   one block per row of the q|k|v projection
+//   k_paged_attn    rows of a few tokens against a span of positions, the whole call split evenly over the GPU
+//   k_paged_merge   joins the row tiles that the split cut
+//   k_pages_copy    page copies of a list of pairs, every layer, both pools
+#include <algorithm>
+#include <mutex>
+
+#include "kernels.cuh"
+#include "paged.cuh"
+
+namespace eb {
+namespace {
+
+// ------------------------------------------------------------------------------------------------
+// rotary positions + append
+// ------------------------------------------------------------------------------------------------
+// Row r of sequence s is at position p = kv - q + (r - q0). Each q and k head x: x <- x / sqrt(mean x^2 + eps) * w
+// when weights are given; then for pair i < n_rot / 2 with angle p * inv_freq[i] (the product and its sine and cosine
+// in 64 bits: at p = 1e5 a 32-bit product is off by 4e-3 rad):
+//   (a, b) <- (a cos - b sin, a sin + b cos),  (a, b) = (x[i], x[i + n_rot/2]) or (x[2i], x[2i + 1]).
+// Bytes: 4 hd (n_head + 2 n_kv) in, 4 hd n_head + 2 hd n_kv es out per row; nothing is read twice.
+constexpr int AP_NT = 256;
+constexpr int AP_PF = 4;  // head vectors a thread loads before it needs the row's sequence
+
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(__half* p, const float (&v)[4]) {  // one rounding to the pool's 11 bits
+    const __half2 a = __floats2half2_rn(v[0], v[1]), b = __floats2half2_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(AP_NT) k_rope_append(PagedArgs a, EahmmfRope rope, const float* __restrict__ qkv,
+                                                       int ld, const float* __restrict__ qn,
+                                                       const float* __restrict__ kn, float eps, float* __restrict__ q,
+                                                       int ldq) {
+    constexpr int LPH = HD / 4, HPP = AP_NT / LPH;  // lanes per head, heads per pass of the block
+    __shared__ float2 cs[HD / 2];
+    __shared__ __align__(16) float xs[HPP][HD];
+    const int row = blockIdx.x, tid = threadIdx.x, l = tid % LPH, hp = tid / LPH;
+    const uint32_t lanes = LPH == 32 ? 0xffffffffu : 0xffffu << (tid & 16);  // the lanes of this head (two heads a warp at 64)
+    const int n_q = a.n_head, n_all = a.n_head + 2 * a.n_kv, half = rope.n_rot / 2;
+    pdl_wait();
+    pdl_trigger();
+    const float* src = qkv + (size_t)row * ld + 4 * l;
+    float4 pf[AP_PF];
+#pragma unroll
+    for (int j = 0; j < AP_PF; j++)
+        if (hp + j * HPP < n_all) pf[j] = *reinterpret_cast<const float4*>(src + (size_t)(hp + j * HPP) * HD);
+    const float fr = tid < half ? rope.d_inv_freq[tid] : 0.f;
+    // the row's sequence: how many sequences end at or before the row
+    int seq = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += AP_NT)
+        seq += __syncthreads_count(s0 + tid < a.n_seq && a.cu_q[s0 + tid + 1] <= row);
+    if (seq >= a.n_seq) return;  // a row behind the last sequence
+    const Seq sq = paged_seq(a, seq, tid == 0);
+    if (row < sq.q0 || row >= sq.q0 + sq.q) {
+        if (tid == 0) paged_flag(a.status);
+        return;
+    }
+    const int pos = sq.kv - sq.q + (row - sq.q0);
+    if (pos < 0) {  // no such position: nothing to append, an empty q row
+        const float z[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int h = hp; h < n_q; h += HPP) store4(q + (size_t)row * ldq + (size_t)h * HD + 4 * l, z);
+        return;
+    }
+    const int id = a.table[(size_t)seq * a.table_ld + pos / a.page];
+    if (tid < half) {
+        double sn, co;
+        sincos((double)pos * (double)fr, &sn, &co);
+        cs[tid] = make_float2((float)co * rope.mscale, (float)sn * rope.mscale);
+    }
+    const bool page_ok = (unsigned)id < (unsigned)a.n_pages;
+    if (!page_ok && tid == 0) paged_flag(a.status);
+    const size_t at = (size_t)(page_ok ? id : 0) * a.page_stride + (size_t)(pos % a.page) * HD + 4 * l;
+    __syncthreads();
+    // this lane's elements 4l .. 4l + 3 of every head: y = x * co + partner * sn (sn carries the pair's sign)
+    float co[4], sn[4];
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        const int e = 4 * l + c;
+        const bool first = rope.style == EAHMMF_ROPE_HALF ? e < half : (e & 1) == 0;
+        const int i = rope.style == EAHMMF_ROPE_HALF ? (first ? e : e - half) : e >> 1;
+        const float2 r = e < rope.n_rot ? cs[i] : make_float2(1.f, 0.f);
+        co[c] = r.x;
+        sn[c] = first ? -r.y : r.y;
+    }
+    auto head = [&](int h, const float4& x4) {
+        float v[4] = {x4.x, x4.y, x4.z, x4.w};
+        if (h >= n_q + a.n_kv) {  // a v head, as it is
+            if (page_ok) store4(static_cast<T*>(a.v) + at + (size_t)(h - n_q - a.n_kv) * a.page * HD, v);
+            return;
+        }
+        const float* w = h < n_q ? qn : kn;
+        if (w) {
+            float ss = fmaf(v[0], v[0], fmaf(v[1], v[1], fmaf(v[2], v[2], v[3] * v[3])));
+#pragma unroll
+            for (int o = LPH / 2; o; o >>= 1) ss += __shfl_xor_sync(lanes, ss, o);
+            const float sc = 1.0f / sqrtf(ss / (float)HD + eps);
+            const float4 g = __ldg(reinterpret_cast<const float4*>(w) + l);
+            v[0] = v[0] * sc * g.x;
+            v[1] = v[1] * sc * g.y;
+            v[2] = v[2] * sc * g.z;
+            v[3] = v[3] * sc * g.w;
+        }
+        float y[4];
+        if (rope.style == EAHMMF_ROPE_HALF) {
+            store4(&xs[hp][4 * l], v);
+            __syncwarp(lanes);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int e = 4 * l + c;
+                y[c] = e < rope.n_rot ? xs[hp][e < half ? e + half : e - half] : 0.f;
+            }
+            __syncwarp(lanes);
+        } else {
+            y[0] = v[1];
+            y[1] = v[0];
+            y[2] = v[3];
+            y[3] = v[2];
+        }
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+            if (4 * l + c < rope.n_rot) v[c] = fmaf(v[c], co[c], y[c] * sn[c]);
+        if (h < n_q)
+            store4(q + (size_t)row * ldq + (size_t)h * HD + 4 * l, v);
+        else if (page_ok)
+            store4(static_cast<T*>(a.k) + at + (size_t)(h - n_q) * a.page * HD, v);
+    };
+    const int passes = (n_all + HPP - 1) / HPP;
+#pragma unroll
+    for (int j = 0; j < AP_PF; j++) {
+        const int h = hp + j * HPP;
+        if (j < passes && h < n_all) head(h, pf[j]);
+    }
+    for (int j = AP_PF; j < passes; j++) {
+        const int h = hp + j * HPP;
+        if (h < n_all) head(h, *reinterpret_cast<const float4*>(src + (size_t)h * HD));
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// page copies
+// ------------------------------------------------------------------------------------------------
+// The pairs travel as a kernel argument: the list is in host memory, checked there, and the call neither
+// copies nor keeps anything. Bytes: each page read once and written once, in every layer, both pools.
+constexpr int CP_NT = 256, CP_VEC = 4;  // 16-byte vectors a thread has in flight
+constexpr int CP_PAIRS = 480;           // 3840 bytes of the 4 KB that every kernel's arguments may take
+struct CopyList {
+    int2 p[CP_PAIRS];
+};
+__global__ void __launch_bounds__(CP_NT) k_pages_copy(uint4* __restrict__ k, uint4* __restrict__ v, size_t layer_stride,
+                                                      size_t page_stride, int vecs, const CopyList list) {
+    const int2 pr = list.p[blockIdx.z];
+    pdl_wait();
+    pdl_trigger();
+    uint4* pool = (blockIdx.y & 1) ? v : k;
+    const size_t lo = (size_t)(blockIdx.y >> 1) * layer_stride;
+    const uint4* s = pool + lo + (size_t)pr.x * page_stride;
+    uint4* d = pool + lo + (size_t)pr.y * page_stride;
+    const int i0 = blockIdx.x * CP_NT * CP_VEC + threadIdx.x;
+    uint4 r[CP_VEC];
+#pragma unroll
+    for (int j = 0; j < CP_VEC; j++)
+        if (i0 + j * CP_NT < vecs) r[j] = s[i0 + j * CP_NT];
+#pragma unroll
+    for (int j = 0; j < CP_VEC; j++)
+        if (i0 + j * CP_NT < vecs) d[i0 + j * CP_NT] = r[j];
+}
+
+// ------------------------------------------------------------------------------------------------
+// attention of a few rows per sequence
+// ------------------------------------------------------------------------------------------------
+// o = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q.k_j - m), over the positions j that the row sees: j <= p, and with
+// a window j > p - window or j < n_sink. One pass with the running maximum m; parts of a row's positions are
+// joined by their (m, sum, o).
+//
+// A step reads 2 hd es bytes per position and kv head and does 4 hd flops per q head with them: it is bound by
+// the reads, so every operand goes from memory straight into the registers of the matrix instructions, in the
+// order in which it lies (the sums run over hd and over positions, whose order is free, and so is the order of
+// the output's columns): no shared memory, no barrier, 16-byte loads.
+//
+// Numerics. Activations are 32-bit and the pools hold 11 or 24 bits. q and p are split in two parts of 11 bits
+// (hi + lo: 22 bits, 2^-23 relative), which the matrix instructions multiply exactly and add in 32 bits:
+//   16-bit pools   m16n8k16: (q_hi + q_lo) k and (p_hi + p_lo) v. Rows of q are first scaled by a power of two to
+//                  [2^8, 2^9), p by 2^15, so that the low parts stay above the smallest half
+//   32-bit pools   m16n8k8 on 11-bit parts of a 32-bit range: hi hi + lo hi + hi lo (lo lo is 2^-22 of it)
+// Up to 8 rows (STACK) the two parts of a row lie in rows g and g + 8 of one instruction: no extra work, and the
+// thread that holds row g holds row g + 8 too. 16 rows take an instruction for each part.
+constexpr int PA_NW = 4, PA_NT = 32 * PA_NW;
+constexpr float P_SHIFT = 15.f;
+
+template <typename T>
+constexpr int pos_step() {
+    return sizeof(T) == 2 ? 16 : 8;  // positions a warp takes at once
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t h2(__half a, __half b) {
+    const __half2 v = __halves2half2(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+// (x, y) as 11-bit parts in two packed registers
+__device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half hx = __float2half_rn(x), hy = __float2half_rn(y);
+    hi = h2(hx, hy);
+    lo = h2(__float2half_rn(x - __half2float(hx)), __float2half_rn(y - __half2float(hy)));
+}
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    const float r = x - __uint_as_float(hi);
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(r));
+}
+
+// Units of positions that some row of a sequence sees: sink units [0, us), then units [uw, ue).
+struct Units {
+    int us, uw, ue;
+    __device__ __forceinline__ int n() const { return max(1, us + ue - uw); }  // 1: rows that see nothing are written too
+    __device__ __forceinline__ int unit(int i) const { return i < us ? i : uw + (i - us); }
+};
+__device__ __forceinline__ Units units_of(const Seq& sq, int window, int n_sink, int unit) {
+    Units u;
+    u.ue = (sq.kv + unit - 1) / unit;
+    const int low = window > 0 ? max(0, max(0, sq.kv - sq.q) - window + 1) : 0;
+    u.uw = min(low / unit, u.ue);
+    u.us = window > 0 ? min((min(n_sink, sq.kv) + unit - 1) / unit, u.uw) : 0;
+    return u;
+}
+
+template <typename T, int HD, bool STACK>
+struct AttnSmem {
+    static constexpr int RT = STACK ? 8 : 16;
+    static constexpr int KS = sizeof(T) == 2 ? HD / 16 : HD / 8;  // k steps of a score
+    uint4 qf[STACK ? 1 : KS * 32 * 2];                            // 16 rows: q in fragment order, hi then lo
+    float o[PA_NW][RT][HD + 4];
+    float m[PA_NW][RT], l[PA_NW][RT];
+    float cs[RT];  // score scale of each row
+};
+
+// A partial record: o [16][hd], m [16], sum [16].
+__host__ __device__ constexpr int part_floats(int hd) { return 16 * hd + 32; }
+
+template <typename T, int HD, bool STACK>
+__global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
+    constexpr bool H16 = sizeof(T) == 2;
+    constexpr int STEP = pos_step<T>(), UNIT = STEP * PA_NW, RT = STACK ? 8 : 16, NR = STACK ? 1 : 2;
+    constexpr int KS = AttnSmem<T, HD, STACK>::KS;  // k steps of q k
+    constexpr int NT = HD / 8;                      // column tiles of p v
+    constexpr int KC = HD * (int)sizeof(T) / 64;    // 16-byte chunks of a K row a thread loads (4 threads a row)
+    constexpr int VC = HD * (int)sizeof(T) / 128;   // of a V row (8 threads a row)
+    constexpr int JT = STEP / 8;                    // score tiles of a step
+    constexpr int PT = 2 * JT;                      // positions whose V rows a thread loads
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    AttnSmem<T, HD, STACK>& S = *reinterpret_cast<AttnSmem<T, HD, STACK>*>(smem_raw);
+    __shared__ long long s_scan[PA_NW], s_start;
+    __shared__ int s_seq;
+    const PagedArgs& a = A.c;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    pdl_wait();
+    pdl_trigger();
+
+    // ---- this block's share of the call: work items in (sequence, kv head, row tile, unit) order
+    auto weight = [&](int s, bool flag) -> long long {
+        const Seq sq = paged_seq(a, s, flag);
+        if (sq.q == 0) return 0;
+        return (long long)units_of(sq, A.window, A.n_sink, UNIT).n() * a.n_kv * ((sq.q * a.grp + RT - 1) / RT);
+    };
+    long long total = 0, mine = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += PA_NT) {
+        mine = s0 + tid < a.n_seq ? weight(s0 + tid, blockIdx.x == 0) : 0;
+        long long v = mine;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == 0) s_scan[warp] = v;
+        __syncthreads();
+        total += s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+        __syncthreads();
+    }
+    const long long share = max((total + gridDim.x - 1) / gridDim.x, (long long)(A.min_units));
+    const long long begin = share * blockIdx.x, end = min(total, begin + share);
+    if (tid == 0) A.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (begin >= total) return;
+    long long run = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += PA_NT) {  // the sequence that holds `begin`
+        if (a.n_seq > PA_NT) mine = s0 + tid < a.n_seq ? weight(s0 + tid, false) : 0;
+        long long v = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long n = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += n;
+        }
+        if (lane == 31) s_scan[warp] = v;
+        __syncthreads();
+        for (int w = 0; w < warp; w++) v += s_scan[w];
+        v += run;
+        if (mine > 0 && v - mine <= begin && begin < v) {
+            s_seq = s0 + tid;
+            s_start = v - mine;
+        }
+        run += s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+        __syncthreads();
+        if (run > begin) break;
+    }
+    int seq = s_seq;
+    long long seq_at = s_start;
+    const T* kp = static_cast<const T*>(a.k);
+    const T* vp = static_cast<const T*>(a.v);
+
+    for (long long at = begin; at < end && seq < a.n_seq;) {
+        const Seq sq = paged_seq(a, seq, false);
+        const Units un = units_of(sq, A.window, A.n_sink, UNIT);
+        const int nu = un.n(), nrt = (sq.q * a.grp + RT - 1) / RT;
+        const long long here = (long long)nu * nrt * a.n_kv;
+        if (sq.q == 0 || at >= seq_at + here) {
+            if (sq.q) seq_at += here;
+            seq++;
+            continue;
+        }
+        const long long idx = at - seq_at;
+        const int item = (int)(idx / nu), u0 = (int)(idx - (long long)item * nu);
+        const int kvh = item / nrt, rt = item - kvh * nrt;
+        const int n_it = (int)min((long long)(nu - u0), end - at);
+        // ---- the row tile: rows r0 .. of (token, q head of the group)
+        const int r0 = rt * RT, n_rows = min(RT, sq.q * a.grp - r0), p_first = sq.kv - sq.q;
+        auto q_row = [&](int r) {
+            const int rr = r0 + r, tok = rr / a.grp;
+            return A.q + (size_t)(sq.q0 + tok) * A.ldq + (size_t)(kvh * a.grp + (rr - tok * a.grp)) * HD;
+        };
+        int lim[NR], low[NR];  // the positions that this thread's rows see
+        float cs[NR];
+        uint32_t qa[STACK ? KS : 1][4];
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            const int r = g + 8 * i;
+            lim[i] = r < n_rows ? p_first + (r0 + r) / a.grp : -1;
+            low[i] = A.window > 0 ? lim[i] - A.window + 1 : 0;
+            const bool ok = r < n_rows;
+            const float* qr = ok ? q_row(r) : nullptr;
+            float x[KS * (H16 ? 4 : 2)];  // the thread's elements of the row, in k-step order
+            constexpr int PER = H16 ? 4 : 2;
+#pragma unroll
+            for (int c = 0; c < (int)(sizeof(x) / 16); c++) {
+                const int e = H16 ? 8 * (t + 4 * (c >> 1)) + 4 * (c & 1) : 4 * (t + 4 * c);
+                const float4 f = ok ? *reinterpret_cast<const float4*>(qr + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+                x[4 * c] = f.x;
+                x[4 * c + 1] = f.y;
+                x[4 * c + 2] = f.z;
+                x[4 * c + 3] = f.w;
+            }
+            float sc = 1.f;
+            if (H16) {
+                float mx = 0.f;
+#pragma unroll
+                for (int c = 0; c < KS * PER; c++) mx = fmaxf(mx, fabsf(x[c]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const int ex = (int)((__float_as_uint(mx) >> 23) & 255) - 127;  // mx in [2^ex, 2^(ex+1))
+                if (ex < 128 && mx > 0.f) sc = pow2f(min(max(8 - ex, -100), 100));
+            }
+            cs[i] = A.scale * 1.4426950408889634f / sc;
+            if (STACK) {
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    if (H16) {
+                        split_f16(x[4 * k] * sc, x[4 * k + 1] * sc, qa[k][0], qa[k][1]);
+                        split_f16(x[4 * k + 2] * sc, x[4 * k + 3] * sc, qa[k][2], qa[k][3]);
+                    } else {
+                        split_tf32(x[2 * k], qa[k][0], qa[k][1]);
+                        split_tf32(x[2 * k + 1], qa[k][2], qa[k][3]);
+                    }
+                }
+            } else {
+                uint32_t* hi = reinterpret_cast<uint32_t*>(S.qf);
+#pragma unroll
+                for (int k = 0; k < KS; k++)
+                    if (k % PA_NW == warp) {
+                        uint32_t h0, l0, h1, l1;
+                        if (H16) {
+                            split_f16(x[4 * k] * sc, x[4 * k + 1] * sc, h0, l0);
+                            split_f16(x[4 * k + 2] * sc, x[4 * k + 3] * sc, h1, l1);
+                        } else {
+                            split_tf32(x[2 * k], h0, l0);
+                            split_tf32(x[2 * k + 1], h1, l1);
+                        }
+                        uint32_t* f = hi + ((size_t)k * 32 + lane) * 8;
+                        f[i] = h0;
+                        f[2 + i] = h1;
+                        f[4 + i] = l0;
+                        f[6 + i] = l1;
+                    }
+            }
+        }
+        if (!STACK) __syncthreads();
+        const int lim_max = p_first + (r0 + n_rows - 1) / a.grp, first_pos = p_first + r0 / a.grp;
+        const int low_min = A.window > 0 ? first_pos - A.window + 1 : 0;
+        auto any = [&](int j) { return j <= lim_max && (j >= low_min || j < A.n_sink); };
+
+        // ---- K and V of a step: page ids of 32 steps at a time, one per lane
+        int ids = -1;
+        auto fetch_ids = [&](int it) {
+            const int i = it + lane;
+            ids = -1;
+            if (i < n_it) {
+                const int p = un.unit(u0 + i) * UNIT + warp * STEP;
+                if (p < sq.kv && (any(p) || any(p + STEP - 1) || (p < low_min && p + STEP > low_min))) {
+                    ids = a.table[(size_t)seq * a.table_ld + p / a.page];
+                    if ((unsigned)ids >= (unsigned)a.n_pages) {
+                        paged_flag(a.status);
+                        ids = -1;
+                    }
+                }
+            }
+        };
+        uint4 kr[JT][KC], vr[PT][VC];
+        auto base_of = [&](int it, int& p) -> long long {  // element offset of the step's first position, or -1
+            if ((it & 31) == 0) fetch_ids(it);
+            const int id = __shfl_sync(0xffffffffu, ids, it & 31);
+            p = un.unit(u0 + it) * UNIT + warp * STEP;
+            if (it >= n_it || id < 0) return -1;
+            return (long long)((size_t)id * a.page_stride + ((size_t)kvh * a.page + p % a.page) * HD);
+        };
+        auto load_k = [&](long long base, int p) {
+#pragma unroll
+            for (int j = 0; j < JT; j++) {
+                const int r = 8 * j + g;
+                const bool ok = base >= 0 && any(p + r);
+                const uint4* src = reinterpret_cast<const uint4*>(kp + base + (size_t)r * HD) + t;
+#pragma unroll
+                for (int c = 0; c < KC; c++) kr[j][c] = ok ? __ldg(src + 4 * c) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto load_v = [&](long long base, int p) {  // rows of positions no row sees stay zero: 0 * NaN is NaN
+#pragma unroll
+            for (int j = 0; j < PT; j++) {
+                const int r = 8 * (j >> 1) + 2 * t + (j & 1);
+                const bool ok = base >= 0 && any(p + r);
+                const uint4* src = reinterpret_cast<const uint4*>(vp + base + (size_t)r * HD) + g;
+#pragma unroll
+                for (int c = 0; c < VC; c++) vr[j][c] = ok ? __ldg(src + 8 * c) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        float o[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        float m[NR], l[NR];
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
+        }
+        int p;
+        long long base = base_of(0, p);
+        load_k(base, p);
+        load_v(base, p);
+        for (int it = 0; it < n_it; it++) {
+            float sacc[JT][4];
+#pragma unroll
+            for (int j = 0; j < JT; j++) sacc[j][0] = sacc[j][1] = sacc[j][2] = sacc[j][3] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                uint32_t ah[4], al[4];
+                if (STACK) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) ah[i] = qa[k][i];
+                } else {
+                    const uint4 h = S.qf[(k * 32 + lane) * 2], lo4 = S.qf[(k * 32 + lane) * 2 + 1];
+                    ah[0] = h.x, ah[1] = h.y, ah[2] = h.z, ah[3] = h.w;
+                    al[0] = lo4.x, al[1] = lo4.y, al[2] = lo4.z, al[3] = lo4.w;
+                }
+#pragma unroll
+                for (int j = 0; j < JT; j++) {
+                    const uint4& w = kr[j][k >> 1];
+                    const uint32_t b0 = (k & 1) ? w.z : w.x, b1 = (k & 1) ? w.w : w.y;
+                    if (H16) {
+                        mma_f16(sacc[j], ah, b0, b1);
+                        if (!STACK) mma_f16(sacc[j], al, b0, b1);
+                    } else {
+                        uint32_t h0, l0, h1, l1;
+                        split_tf32(__uint_as_float(b0), h0, l0);
+                        split_tf32(__uint_as_float(b1), h1, l1);
+                        mma_tf32(sacc[j], ah, h0, h1);
+                        mma_tf32(sacc[j], ah, l0, l1);
+                        if (!STACK) mma_tf32(sacc[j], al, h0, h1);
+                    }
+                }
+            }
+            const int p_cur = p;
+            const bool live = base >= 0;
+            base = base_of(it + 1, p);
+            load_k(base, p);  // the next K rows travel during the softmax and p v
+            // ---- scores of this thread's rows: positions p + 8 j + 2 t + c
+            float sv[NR][PT];
+            float mx[NR];
+#pragma unroll
+            for (int i = 0; i < NR; i++) {
+                mx[i] = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < PT; j++) {
+                    const int pos = p_cur + 8 * (j >> 1) + 2 * t + (j & 1);
+                    const float raw = STACK ? sacc[j >> 1][j & 1] + sacc[j >> 1][(j & 1) + 2] : sacc[j >> 1][(j & 1) + 2 * i];
+                    const bool see = live && pos <= lim[i] && (pos >= low[i] || pos < A.n_sink);
+                    sv[i][j] = see ? raw * cs[i] : -INFINITY;
+                    mx[i] = fmaxf(mx[i], sv[i][j]);
+                }
+                mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+                mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+                mx[i] = fmaxf(mx[i], m[i]);
+            }
+            bool grew = mx[0] > m[0];
+            if (NR == 2) grew = grew || mx[NR - 1] > m[NR - 1];
+            if (__any_sync(0xffffffffu, grew)) {
+                float al[NR];
+#pragma unroll
+                for (int i = 0; i < NR; i++) {
+                    al[i] = mx[i] == -INFINITY ? 1.f : exp2f(m[i] - mx[i]);
+                    l[i] *= al[i];
+                    m[i] = mx[i];
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    o[n][0] *= al[0];
+                    o[n][1] *= al[0];
+                    o[n][2] *= al[NR - 1];
+                    o[n][3] *= al[NR - 1];
+                }
+            }
+            uint32_t ph[4], pl[4];
+#pragma unroll
+            for (int i = 0; i < NR; i++) {
+                const float mo = m[i] == -INFINITY ? 0.f : m[i] - P_SHIFT;
+#pragma unroll
+                for (int j = 0; j < PT; j++) {
+                    sv[i][j] = exp2f(sv[i][j] - mo);
+                    l[i] += sv[i][j];
+                }
+                if (H16) {
+#pragma unroll
+                    for (int j = 0; j < JT; j++)
+                        split_f16(sv[i][2 * j], sv[i][2 * j + 1], ph[2 * j + i], STACK ? ph[2 * j + 1] : pl[2 * j + i]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < PT; j++) split_tf32(sv[i][j], ph[2 * j + i], STACK ? ph[2 * j + 1] : pl[2 * j + i]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < VC; c++)
+#pragma unroll
+                for (int e = 0; e < 16 / (int)sizeof(T); e++) {
+                    const int n = c * (16 / (int)sizeof(T)) + e;
+                    if (H16) {
+                        const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
+                        auto word = [&](const uint4& w) { return (e >> 1) == 0 ? w.x : (e >> 1) == 1 ? w.y : (e >> 1) == 2 ? w.z : w.w; };
+                        const uint32_t b0 = __byte_perm(word(vr[0][c]), word(vr[1][c]), sel);
+                        const uint32_t b1 = __byte_perm(word(vr[PT - 2][c]), word(vr[PT - 1][c]), sel);
+                        mma_f16(o[n], ph, b0, b1);
+                        if (!STACK) mma_f16(o[n], pl, b0, b1);
+                    } else {
+                        auto word = [&](const uint4& w) { return e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w; };
+                        uint32_t h0, l0, h1, l1;
+                        split_tf32(__uint_as_float(word(vr[0][c])), h0, l0);
+                        split_tf32(__uint_as_float(word(vr[1][c])), h1, l1);
+                        mma_tf32(o[n], ph, h0, h1);
+                        mma_tf32(o[n], ph, l0, l1);
+                        if (!STACK) mma_tf32(o[n], pl, h0, h1);
+                    }
+                }
+            load_v(base, p);
+        }
+        // ---- the four warps' parts joined, then the output or this block's partial record
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            if (t == 0) {
+                S.m[warp][g + 8 * i] = m[i];
+                S.l[warp][g + 8 * i] = l[i];
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            constexpr int E = 16 / (int)sizeof(T);
+            const int col = E * (2 * t + 8 * (n / E)) + n % E;
+            if (STACK) {
+                S.o[warp][g][col] = o[n][0] + o[n][2];
+                S.o[warp][g][col + E] = o[n][1] + o[n][3];
+            } else {
+                S.o[warp][g][col] = o[n][0];
+                S.o[warp][g][col + E] = o[n][1];
+                S.o[warp][g + 8][col] = o[n][2];
+                S.o[warp][g + 8][col + E] = o[n][3];
+            }
+        }
+        __syncthreads();
+        const bool whole = u0 == 0 && n_it == nu;
+        float* rec = A.part + ((size_t)blockIdx.x * 2 + (u0 == 0 ? 1 : 0)) * part_floats(HD);
+        for (int i = tid; i < n_rows * (HD / 4); i += PA_NT) {
+            const int r = i / (HD / 4), c4 = i - r * (HD / 4);
+            float M = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < PA_NW; w++) M = fmaxf(M, S.m[w][r]);
+            float L = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < PA_NW; w++) {
+                const float e = S.m[w][r] == -INFINITY ? 0.f : exp2f(S.m[w][r] - M);
+                if (S.m[w][r] == -INFINITY && !(S.l[w][r] != S.l[w][r])) continue;
+                const float4 f = *reinterpret_cast<const float4*>(&S.o[w][r][4 * c4]);
+                L = fmaf(S.l[w][r], e, L);
+                acc.x = fmaf(f.x, e, acc.x);
+                acc.y = fmaf(f.y, e, acc.y);
+                acc.z = fmaf(f.z, e, acc.z);
+                acc.w = fmaf(f.w, e, acc.w);
+            }
+            if (whole) {
+                const float inv = L == 0.f ? 0.f : 1.f / L;
+                const int rr = r0 + r, tok = rr / a.grp;
+                *reinterpret_cast<float4*>(A.out + (size_t)(sq.q0 + tok) * A.ldo +
+                                           (size_t)(kvh * a.grp + (rr - tok * a.grp)) * HD + 4 * c4) =
+                    make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+            } else {
+                reinterpret_cast<float4*>(rec)[r * (HD / 4) + c4] = acc;
+                if (c4 == 0) {
+                    rec[16 * HD + r] = M;
+                    rec[16 * HD + 16 + r] = L;
+                }
+            }
+        }
+        if (!whole && u0 == 0 && tid == 0) {  // the blocks after this one hold the rest of the tile
+            const long long tile_end = at + nu;
+            A.meta[blockIdx.x] = make_int4((int)((tile_end - 1) / share) - blockIdx.x, seq, kvh, rt);
+        }
+        __syncthreads();
+        at += n_it;
+    }
+}
+
+// Joins the records of the row tiles that the split cut: block (b, r) takes row r of the tile that block b of
+// k_paged_attn began and left to the blocks after it (meta: how many, sequence, kv head, row tile).
+constexpr int PM_NT = 256;
+template <int HD>
+__global__ void __launch_bounds__(PM_NT) k_paged_merge(PagedAttnArgs A, int rt_rows) {
+    constexpr int LN = HD / 4, G = PM_NT / LN;  // lanes of a row, records taken at once
+    __shared__ __align__(16) float so[G][HD];
+    __shared__ float sm[G], sl[G];
+    const int b = blockIdx.x, r = blockIdx.y, lane = threadIdx.x % LN, grp = threadIdx.x / LN;
+    pdl_wait();
+    pdl_trigger();
+    const int4 me = A.meta[b];
+    if (me.x == 0) return;
+    const Seq sq = paged_seq(A.c, me.y, false);
+    const int rr = me.w * rt_rows + r;
+    if (rr >= sq.q * A.c.grp) return;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int j = grp; j <= me.x; j += G) {
+        const float* rec = A.part + ((size_t)(b + j) * 2 + (j == 0 ? 1 : 0)) * part_floats(HD);
+        const float mj = rec[16 * HD + r], lj = rec[16 * HD + 16 + r];
+        const float4 f = reinterpret_cast<const float4*>(rec)[r * LN + lane];
+        const float mn = fmaxf(m, mj);
+        if (mn == -INFINITY) {  // nothing seen so far (a NaN sum stays one)
+            l += lj;
+            continue;
+        }
+        const float ea = exp2f(m - mn), eb_ = exp2f(mj - mn);
+        m = mn;
+        l = fmaf(l, ea, lj * eb_);
+        o.x = fmaf(o.x, ea, f.x * eb_);
+        o.y = fmaf(o.y, ea, f.y * eb_);
+        o.z = fmaf(o.z, ea, f.z * eb_);
+        o.w = fmaf(o.w, ea, f.w * eb_);
+    }
+    reinterpret_cast<float4*>(so[grp])[lane] = o;
+    if (lane == 0) {
+        sm[grp] = m;
+        sl[grp] = l;
+    }
+    __syncthreads();
+    if (grp) return;
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int j = 0; j < G; j++) M = fmaxf(M, sm[j]);
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < G; j++) {
+        const float e = sm[j] == -INFINITY ? 0.f : exp2f(sm[j] - M);
+        const float4 f = reinterpret_cast<const float4*>(so[j])[lane];
+        L = fmaf(sl[j], e, L);
+        o.x = fmaf(f.x, e, o.x);
+        o.y = fmaf(f.y, e, o.y);
+        o.z = fmaf(f.z, e, o.z);
+        o.w = fmaf(f.w, e, o.w);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int tok = rr / A.c.grp;
+    *reinterpret_cast<float4*>(A.out + (size_t)(sq.q0 + tok) * A.ldo + (size_t)(me.z * A.c.grp + rr - tok * A.c.grp) * HD +
+                               4 * lane) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+// Raises a kernel's dynamic shared-memory limit, once on each device.
+template <typename T, int HD, bool STACK, typename Kern>
+cudaError_t smem_limit(Kern k, size_t bytes) {
+    constexpr int MAX_DEV = 64;
+    static std::mutex mu;
+    static bool done[MAX_DEV] = {};  // one array per instance, that is per kernel
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev < 0 || dev >= MAX_DEV) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> g(mu);
+    if (!done[dev]) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done[dev] = true;
+    return e;
+}
+
+template <typename T, int HD, bool STACK>
+cudaError_t attn_go(const PagedAttnArgs& A, cudaStream_t st) {
+    constexpr int RT = STACK ? 8 : 16;
+    cudaError_t e = smem_limit<T, HD, STACK>(k_paged_attn<T, HD, STACK>, sizeof(AttnSmem<T, HD, STACK>));
+    if (e != cudaSuccess) return e;
+    e = launch_pdl(k_paged_attn<T, HD, STACK>, dim3(A.grid), dim3(PA_NT), sizeof(AttnSmem<T, HD, STACK>), st, A);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(k_paged_merge<HD>, dim3(A.grid, RT), dim3(PM_NT), 0, st, A, RT);
+}
+template <typename T, int HD>
+cudaError_t attn_rows(const PagedAttnArgs& A, int max_q, cudaStream_t st) {
+    return max_q * A.c.grp <= 8 ? attn_go<T, HD, true>(A, st) : attn_go<T, HD, false>(A, st);
+}
+
+int attn_grid() { return 2 * sm_count(); }
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+}  // namespace
+
+size_t paged_attn_ws_bytes(int hd) {
+    return align256((size_t)attn_grid() * sizeof(int4)) + (size_t)attn_grid() * 2 * part_floats(hd) * sizeof(float);
+}
+
+cudaError_t launch_paged_attention(int type, int hd, int max_q, int max_kv, PagedAttnArgs A, void* ws, cudaStream_t st) {
+    (void)max_kv;
+    A.grid = attn_grid();
+    A.min_units = 4;
+    A.meta = static_cast<int4*>(ws);
+    A.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + align256((size_t)A.grid * sizeof(int4)));
+    if (type == T_F16) return hd == 128 ? attn_rows<__half, 128>(A, max_q, st) : attn_rows<__half, 64>(A, max_q, st);
+    return hd == 128 ? attn_rows<float, 128>(A, max_q, st) : attn_rows<float, 64>(A, max_q, st);
+}
+
+cudaError_t launch_rope_append(int type, int hd, const PagedArgs& a, const EahmmfRope& rope, const float* qkv, int ld,
+                               const float* qn, const float* kn, float eps, float* q, int ldq, cudaStream_t st) {
+    auto go = [&](auto kern) {
+        return launch_pdl(kern, dim3(a.n_tok), dim3(AP_NT), 0, st, a, rope, qkv, ld, qn, kn, eps, q, ldq);
+    };
+    if (type == T_F16) return hd == 128 ? go(k_rope_append<__half, 128>) : go(k_rope_append<__half, 64>);
+    return hd == 128 ? go(k_rope_append<float, 128>) : go(k_rope_append<float, 64>);
+}
+
+cudaError_t launch_pages_copy(const EahmmfPagedKv& kv, const int* pairs, int n, cudaStream_t st) {
+    const size_t es = kv.type == T_F16 ? 2 : 4;
+    const int vecs = (int)((size_t)kv.n_kv * kv.page * kv.hd * es / 16);
+    for (int i = 0; i < n; i += CP_PAIRS) {
+        const int m = std::min(CP_PAIRS, n - i);
+        CopyList list;
+        for (int j = 0; j < m; j++) list.p[j] = make_int2(pairs[2 * (i + j)], pairs[2 * (i + j) + 1]);
+        const cudaError_t e =
+            launch_pdl(k_pages_copy, dim3((vecs + CP_NT * CP_VEC - 1) / (CP_NT * CP_VEC), 2 * kv.n_layer, m), dim3(CP_NT), 0,
+                       st, static_cast<uint4*>(kv.d_k), static_cast<uint4*>(kv.d_v), kv.layer_stride * es / 16,
+                       kv.page_stride * es / 16, vecs, list);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+}  // namespace eb

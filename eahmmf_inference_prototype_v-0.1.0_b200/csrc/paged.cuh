@@ -1,0 +1,69 @@
+// paged.cuh -- launch-side declarations of the paged key/value cache (paged.cu) and the device helpers its
+// kernels share: a call's sequences, their pages and the positions a row sees.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/eahmmf_b200.h"
+#include "common.cuh"
+
+namespace eb {
+
+constexpr int PAGE_MIN = 16;      // positions per page: a multiple of this, so 16 positions never straddle pages
+constexpr int PAGED_MAX_GRP = 64;  // q heads per kv head
+
+// One layer of a cache and the sequences of a call, as the kernels take them.
+struct PagedArgs {
+    void* k;  // pool of the layer: page p at p * page_stride elements, [n_kv][page][hd] inside
+    void* v;
+    size_t page_stride;
+    int n_pages, n_kv, page, n_head, grp;
+    int n_seq, n_tok, table_ld;
+    const int* cu_q;    // [n_seq + 1] first activation row of each sequence
+    const int* kv_len;  // [n_seq] cached positions with the call's new ones
+    const int* table;   // [n_seq][table_ld] page ids
+    int* status;
+};
+
+__device__ __forceinline__ void paged_flag(int* status) {
+    if (status) atomicOr(status, (int)ST_BAD_INDEX);
+}
+
+// Sequence s of a call: its activation rows [q0, q0 + q) and kv cached positions. Lengths that do not fit the
+// buffers (rows past n_tok, more positions than the table row names) are cut to what does and flagged.
+struct Seq {
+    int q0, q, kv;
+};
+__device__ __forceinline__ Seq paged_seq(const PagedArgs& a, int s, bool flag) {
+    const int c0 = a.cu_q[s], c1 = a.cu_q[s + 1], n = a.kv_len[s];
+    const long long cap = (long long)a.table_ld * a.page;
+    Seq r;
+    r.q0 = min(max(c0, 0), a.n_tok);
+    r.q = min(max(c1, r.q0), a.n_tok) - r.q0;
+    r.kv = n < 0 ? 0 : (long long)n > cap ? (int)cap : n;
+    if (flag && (r.q0 != c0 || r.q != c1 - c0 || r.kv != n)) paged_flag(a.status);
+    return r;
+}
+
+cudaError_t launch_rope_append(int type, int hd, const PagedArgs& a, const EahmmfRope& rope, const float* qkv, int ld,
+                               const float* qn, const float* kn, float eps, float* q, int ldq, cudaStream_t st);
+
+struct PagedAttnArgs {
+    PagedArgs c;
+    const float* q;  // [n_tok][ldq]
+    float* out;      // [n_tok][ldo]
+    int ldq, ldo;
+    float scale;
+    int window, n_sink;  // window 0: every earlier position is visible
+    int grid;            // blocks of the split launch, also the records of `part`
+    int min_units;       // least share of a block
+    float* part;         // [grid][2] partial results
+    int4* meta;          // [grid] the row tile a block began and did not finish
+};
+size_t paged_attn_ws_bytes(int hd);
+cudaError_t launch_paged_attention(int type, int hd, int max_q, int max_kv, PagedAttnArgs a, void* ws, cudaStream_t st);
+
+cudaError_t launch_pages_copy(const EahmmfPagedKv& kv, const int* pairs, int n, cudaStream_t st);
+
+}  // namespace eb

@@ -41,7 +41,43 @@ class EahmmfMoeLayer(C.Structure):
                 ("d_gate", C.c_void_p), ("d_up", C.c_void_p), ("d_down", C.c_void_p), ("d_router", C.c_void_p)]
 
 
+class EahmmfPagedKv(C.Structure):
+    _fields_ = [("d_k", C.c_void_p), ("d_v", C.c_void_p), ("type", C.c_int), ("n_layer", C.c_int),
+                ("n_pages", C.c_int), ("n_kv", C.c_int), ("page", C.c_int), ("hd", C.c_int),
+                ("layer_stride", C.c_size_t), ("page_stride", C.c_size_t)]
+
+
+class EahmmfPagedSeqs(C.Structure):
+    _fields_ = [("n_seq", C.c_int), ("n_tok", C.c_int), ("max_q", C.c_int), ("max_kv", C.c_int),
+                ("d_cu_q", C.c_void_p), ("d_kv_len", C.c_void_p), ("d_table", C.c_void_p), ("table_ld", C.c_int)]
+
+
+class EahmmfRope(C.Structure):
+    _fields_ = [("style", C.c_int), ("n_rot", C.c_int), ("mscale", C.c_float), ("d_inv_freq", C.c_void_p)]
+
+
 EXPORTS = {
+    "eahmmf_cuda_rope_append": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int,
+                                          C.c_void_p, C.c_void_p, C.c_float, C.c_void_p, C.c_int, C.c_void_p,
+                                          C.c_void_p]),
+    "eahmmf_cuda_paged_attention_workspace_bytes": (C.c_size_t, [C.c_void_p, C.c_void_p, C.c_int]),
+    "eahmmf_cuda_paged_attention": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_float,
+                                              C.c_int, C.c_int, C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p,
+                                              C.c_void_p]),
+    "eahmmf_cuda_pages_copy": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "eahmmf_rope_inv_freq": (C.c_int, [C.c_int, C.c_int, C.c_double, C.c_double, C.c_int, C.c_double, C.c_double,
+                                       C.c_void_p, C.c_void_p]),
+    "eahmmf_pages_create": (C.c_void_p, [C.c_int, C.c_int, C.c_int, C.c_int]),
+    "eahmmf_pages_destroy": (None, [C.c_void_p]),
+    "eahmmf_pages_extend": (C.c_int, [C.c_void_p, C.c_int, C.c_int]),
+    "eahmmf_pages_fork": (C.c_int, [C.c_void_p, C.c_int, C.c_int]),
+    "eahmmf_pages_truncate": (C.c_int, [C.c_void_p, C.c_int, C.c_int]),
+    "eahmmf_pages_slide": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
+    "eahmmf_pages_compact": (C.c_int, [C.c_void_p]),
+    "eahmmf_pages_take_copies": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int]),
+    "eahmmf_pages_table": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
+    "eahmmf_pages_free_count": (C.c_int, [C.c_void_p]),
+    "eahmmf_pages_refs": (C.c_int, [C.c_void_p, C.c_int]),
     "eahmmf_cuda_matmul": (C.c_bool, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_size_t, C.c_void_p, C.c_int,
                                       C.c_int, C.c_void_p, C.c_int]),
     "eahmmf_cuda_matmul_pair": (C.c_bool, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_size_t, C.c_void_p, C.c_int,
@@ -475,6 +511,200 @@ def sample(d_logits, d_hist, params: EahmmfSamplerParams, u: float, d_token, d_w
     nh = 0 if d_hist is None else d_hist.numel()
     return lib().eahmmf_cuda_sample(_ptr(d_logits), n, _ptr(d_hist) if nh else None, nh, C.byref(params),
                                     C.c_float(u), _ptr(d_token), _ptr(d_ws), d_ws.numel(), _stream(stream))
+
+
+# ---- paged key/value cache ------------------------------------------------------------------------
+ROPE_STYLES = {"half": 0, "interleaved": 1}  # EAHMMF_ROPE_HALF, EAHMMF_ROPE_INTERLEAVED
+ROPE_SCALINGS = {"plain": 0, "linear": 1, "ntk": 2, "yarn": 3}  # EAHMMF_ROPE_PLAIN ..
+
+
+def rope_inv_freq(n_rot: int, base: float, scaling: str = "plain", factor: float = 1.0, ctx_orig: int = 0,
+                  beta_fast: float = 32.0, beta_slow: float = 1.0):
+    """eahmmf_rope_inv_freq: (frequencies [n_rot / 2] float32 on the host, mscale)."""
+    f = np.zeros(max(n_rot // 2, 1), np.float32)
+    m = C.c_float(1.0)
+    rc = lib().eahmmf_rope_inv_freq(ROPE_SCALINGS[scaling], n_rot, base, factor, ctx_orig, beta_fast, beta_slow,
+                                    f.ctypes.data, C.byref(m))
+    if rc:
+        raise RuntimeError(f"eahmmf_rope_inv_freq returned {rc}")
+    return f, float(m.value)
+
+
+class Rope:
+    """Rotary positions of PagedCache.append: the device frequency table [n_rot / 2] (float32), how pairs lie
+    ("half" or "interleaved") and the factor of the rotated elements."""
+
+    def __init__(self, inv_freq, style: str = "half", mscale: float = 1.0):
+        _dev_tensor(inv_freq, "inv_freq", "float32")
+        self._keep = inv_freq
+        self.desc = EahmmfRope(ROPE_STYLES[style], 2 * inv_freq.numel(), mscale, inv_freq.data_ptr())
+        self._ref = C.addressof(self.desc)
+
+
+def _dev_tensor(t, name: str, dtype: str, device=None):
+    if str(t.dtype) != "torch." + dtype or not t.is_cuda or not t.is_contiguous() or (device is not None and t.device != device):
+        raise ValueError(f"{name}: a contiguous {dtype} tensor on {device or 'a CUDA device'} is needed")
+
+
+class PagedBatch:
+    """The sequences of one call (EahmmfPagedSeqs): int32 device tensors table [n_seq x ld], cu_q [n_seq + 1] and
+    kv_len [n_seq]; rows of activations and the bounds max_q, max_kv of their lengths (they choose kernels, results do
+    not depend on them). The tensors may be rewritten between calls; the object keeps their addresses."""
+
+    def __init__(self, table, cu_q, kv_len, n_tok: int, max_q: int, max_kv: int):
+        for t, n in ((table, "table"), (cu_q, "cu_q"), (kv_len, "kv_len")):
+            _dev_tensor(t, n, "int32", kv_len.device)
+        n_seq = kv_len.numel()
+        if cu_q.numel() != n_seq + 1 or table.dim() != 2 or table.shape[0] != n_seq:
+            raise ValueError("table [n_seq x ld], cu_q [n_seq + 1] and kv_len [n_seq] are needed")
+        self._keep = (table, cu_q, kv_len)
+        self.n_tok, self.device = n_tok, kv_len.device
+        self.desc = EahmmfPagedSeqs(n_seq, n_tok, max_q, max_kv, cu_q.data_ptr(), kv_len.data_ptr(), table.data_ptr(),
+                                    table.shape[1])
+        self._ref = C.addressof(self.desc)
+
+
+class PagedCache:
+    """A paged key/value cache over torch tensors k, v [n_layer x n_pages x n_kv x page x hd], float32 or float16. Calls run
+    on `stream` (default: torch's current stream of the cache's device, which has to be the current one) and raise
+    on a refusal; d_status (int32) receives EAHMMF_ST_* bits raised inside kernels."""
+
+    def __init__(self, k, v):
+        import torch
+        self._torch = torch
+        if k.dtype not in (torch.float32, torch.float16) or k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype:
+            raise ValueError("k and v: two float32 or float16 tensors [n_layer x n_pages x n_kv x page x hd]")
+        if not k.is_cuda or v.device != k.device or k.stride() != v.stride():
+            raise ValueError("k and v: device tensors of the same strides on the same device")
+        n_layer, n_pages, n_kv, page, hd = k.shape
+        if k.stride()[2:] != (page * hd, hd, 1):
+            raise ValueError("k and v: a page [n_kv x page x hd] has to be contiguous")
+        self.k, self.v, self.n_kv, self.hd, self.device = k, v, n_kv, hd, k.device
+        self.desc = EahmmfPagedKv(k.data_ptr(), v.data_ptr(), 1 if k.dtype == torch.float16 else 0, n_layer, n_pages, n_kv,
+                                  page, hd, k.stride(0), k.stride(1))
+        self._ref = C.addressof(self.desc)
+        self._lib = lib()
+
+    def _go(self, stream):
+        idx = self.device.index
+        if self._torch.cuda.current_device() != idx:
+            raise ValueError(f"the cache lives on {self.device}: make it the current device")
+        return self._torch._C._cuda_getCurrentRawStream(idx) if stream is None else _stream(stream)
+
+    def _rows(self, x, name: str, batch, width: int):
+        if (x.dtype is not self._torch.float32 or x.device != self.device or x.dim() != 2 or x.shape[0] < batch.n_tok
+                or x.shape[1] != width or (x.stride(1) != 1 and width > 1)):
+            raise ValueError(f"{name}: float32 rows [{batch.n_tok} x {width}] on {self.device} are needed")
+        return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else width
+
+    def _check(self, rc: int, what: str):
+        if rc:
+            raise RuntimeError(f"{what} returned {rc}")
+
+    def append(self, layer: int, batch: PagedBatch, qkv, n_head: int, rope: Rope, q_out, q_norm=None, k_norm=None,
+               eps: float = 1e-6, stream=None, d_status=None) -> None:
+        """eahmmf_cuda_rope_append: rows qkv [n_tok x (n_head + 2 n_kv) hd] normalised (where weights are given) and
+        rotated; q into q_out [n_tok x n_head hd], k and v into the pages of their positions."""
+        st = self._go(stream)
+        x, ld = self._rows(qkv, "qkv", batch, (n_head + 2 * self.n_kv) * self.hd)
+        q, ldq = self._rows(q_out, "q_out", batch, n_head * self.hd)
+        for w, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+            if w is not None:
+                _dev_tensor(w, n, "float32", self.device)
+                if w.numel() != self.hd:
+                    raise ValueError(f"{n}: {self.hd} weights are needed")
+        self._check(self._lib.eahmmf_cuda_rope_append(self._ref, layer, batch._ref, rope._ref, n_head, x, ld, _ptr(q_norm),
+                                                      _ptr(k_norm), eps, q, ldq, st, _ptr(d_status)),
+                    "eahmmf_cuda_rope_append")
+
+    def attention_workspace(self, batch: PagedBatch, n_head: int):
+        """A device workspace for attention() of this batch (torch uint8 tensor); one per call in flight."""
+        n = self._lib.eahmmf_cuda_paged_attention_workspace_bytes(self._ref, batch._ref, n_head)
+        return self._torch.empty(n, dtype=self._torch.uint8, device=self.device)
+
+    def attention(self, layer: int, batch: PagedBatch, q, n_head: int, out, scale: float | None = None, window: int = 0,
+                  n_sink: int = 0, ws=None, stream=None, d_status=None) -> None:
+        """eahmmf_cuda_paged_attention: out [n_tok x n_head hd] from the rows q (scale: 1 / sqrt(hd))."""
+        st = self._go(stream)
+        x, ldq = self._rows(q, "q", batch, n_head * self.hd)
+        y, ldo = self._rows(out, "out", batch, n_head * self.hd)
+        if ws is None:
+            ws = self.attention_workspace(batch, n_head)
+        self._check(self._lib.eahmmf_cuda_paged_attention(self._ref, layer, batch._ref, n_head, x, ldq,
+                                                          self.hd ** -0.5 if scale is None else scale, window, n_sink, y,
+                                                          ldo, ws.data_ptr(), ws.numel(), st, _ptr(d_status)),
+                    "eahmmf_cuda_paged_attention")
+
+    def copy_pages(self, pairs, stream=None) -> None:
+        """eahmmf_cuda_pages_copy: pairs (from, to) [n x 2] on the host, every layer, k and v."""
+        st = self._go(stream)
+        p = np.ascontiguousarray(pairs, np.int32)
+        if p.size % 2:
+            raise ValueError("pairs: [n x 2] page ids are needed")
+        self._check(self._lib.eahmmf_cuda_pages_copy(self._ref, p.ctypes.data, p.size // 2, st), "eahmmf_cuda_pages_copy")
+
+
+class Pages:
+    """The pages of a cache on the host (eahmmf_pages_*): which sequence holds which pages, shared prefixes, the copies a
+    step needs. Calls raise on a refusal and then change nothing."""
+
+    def __init__(self, n_pages: int, page: int, n_seq: int, max_pages: int):
+        self._lib = lib()
+        self._free = self._lib.eahmmf_pages_destroy
+        self._h = self._lib.eahmmf_pages_create(n_pages, page, n_seq, max_pages)
+        if not self._h:
+            raise RuntimeError("eahmmf_pages_create failed")
+        self.n_pages, self.page, self.n_seq, self.max_pages = n_pages, page, n_seq, max_pages
+
+    def __del__(self):
+        try:
+            if self._h:
+                self._free(self._h)
+                self._h = None
+        except Exception:
+            pass
+
+    def _call(self, name: str, *args) -> None:
+        rc = getattr(self._lib, "eahmmf_pages_" + name)(self._h, *args)
+        if rc:
+            raise RuntimeError(f"eahmmf_pages_{name} returned {rc}")
+
+    def extend(self, seq: int, length: int) -> None:
+        self._call("extend", seq, length)
+
+    def fork(self, src: int, dst: int) -> None:
+        self._call("fork", src, dst)
+
+    def truncate(self, seq: int, length: int = 0) -> None:
+        self._call("truncate", seq, length)
+
+    def slide(self, seq: int, first_pos: int, n_sink: int = 0) -> None:
+        self._call("slide", seq, first_pos, n_sink)
+
+    def compact(self) -> None:
+        self._call("compact")
+
+    def take_copies(self) -> np.ndarray:
+        """The recorded copies (from, to) [n x 2], forgotten by this call."""
+        n = self._lib.eahmmf_pages_take_copies(self._h, None, 0)
+        pairs = np.zeros((n, 2), np.int32)
+        if n:
+            self._lib.eahmmf_pages_take_copies(self._h, pairs.ctypes.data, n)
+        return pairs
+
+    def table(self):
+        """(page ids [n_seq x max_pages], lengths [n_seq]) as int32 host arrays."""
+        t = np.zeros((self.n_seq, self.max_pages), np.int32)
+        n = np.zeros(self.n_seq, np.int32)
+        self._call("table", t.ctypes.data, self.max_pages, n.ctypes.data)
+        return t, n
+
+    @property
+    def free(self) -> int:
+        return self._lib.eahmmf_pages_free_count(self._h)
+
+    def refs(self, page_id: int) -> int:
+        return self._lib.eahmmf_pages_refs(self._h, page_id)
 
 
 def hash64(data) -> int:

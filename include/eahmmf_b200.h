@@ -209,6 +209,122 @@ EahmmfRng* eahmmf_rng_create(uint64_t seed);
 float eahmmf_rng_uniform(EahmmfRng* r);
 void eahmmf_rng_free(EahmmfRng* r);
 
+/* ---- paged key/value cache --------------------------------------------------------------------- */
+
+/* The reference keeps one contiguous fp32 cache of n_ctx positions (qwen3moe.cpp:791, :910-913); a paged cache
+ * takes memory as sequences grow, in 16 or 32 bits, lets sequences share the pages of a common prompt, and has
+ * no counterpart there. It is a pair of pools k, v with, in every layer, n_pages pages [n_kv][page][hd]. A sequence
+ * is a row of a block table: entry i names the page of positions i * page .. i * page + page - 1. */
+typedef struct EahmmfPagedKv {
+    void* d_k; /* layer l, page p at element l * layer_stride + p * page_stride; 16-byte aligned */
+    void* d_v;
+    int type; /* 0 F32 or 1 F16 */
+    int n_layer, n_pages, n_kv;
+    int page;            /* positions per page, a multiple of 16 up to 1024 */
+    int hd;              /* head size, 64 or 128 */
+    size_t layer_stride; /* elements, multiples of 8, >= a layer's (a page's) own */
+    size_t page_stride;
+} EahmmfPagedKv;
+
+/* The sequences of one call: n_tok activation rows, of which sequence s owns d_cu_q[s] .. d_cu_q[s + 1] (not
+ * decreasing; none is allowed). They are the last positions of its d_kv_len[s] cached ones: row i of q is at position
+ * d_kv_len[s] - q + i. Rows behind d_cu_q[n_seq] are left as they are. Lengths stay on the device; max_q and max_kv
+ * are the host's bounds on them, which only choose among kernels. Lengths that the buffers cannot
+ * hold are cut, pages outside the pool are skipped, and both raise EAHMMF_ST_BAD_INDEX in d_status. */
+typedef struct EahmmfPagedSeqs {
+    int n_seq, n_tok;
+    int max_q, max_kv;
+    const int* d_cu_q;   /* [n_seq + 1] */
+    const int* d_kv_len; /* [n_seq] */
+    const int* d_table;  /* [n_seq][table_ld] page ids; entries of positions that no row sees are not read */
+    int table_ld;
+} EahmmfPagedSeqs;
+
+/* Rotary positions: pair i < n_rot / 2 of a head, (x[i], x[i + n_rot/2]) or (x[2i], x[2i + 1]), is turned by the angle
+ * position * d_inv_freq[i] (product, sine and cosine in 64 bits) and multiplied by mscale; the rest of the head
+ * stays as it is. */
+#define EAHMMF_ROPE_HALF 0
+#define EAHMMF_ROPE_INTERLEAVED 1
+typedef struct EahmmfRope {
+    int style;
+    int n_rot; /* even, 2 .. hd */
+    float mscale;
+    const float* d_inv_freq; /* [n_rot / 2], device */
+} EahmmfRope;
+
+/* The table d_inv_freq for a context scaled beyond the trained one, on the host (double arithmetic, rounded once):
+ *   EAHMMF_ROPE_PLAIN   base^(-2i / n_rot)  (qwen3moe.cpp:913)
+ *   EAHMMF_ROPE_LINEAR  the same / factor
+ *   EAHMMF_ROPE_NTK     base replaced by base * factor^(n_rot / (n_rot - 2))
+ *   EAHMMF_ROPE_YARN    pairs that turn at least beta_fast times over ctx_orig keep their frequency, those that turn at
+ *                       most beta_slow times have it divided by factor, a linear ramp over i between; mscale
+ *                       (optional) is 0.1 ln(factor) + 1, 1 for the others
+ * Returns 0, or EAHMMF_ST_BAD_ARG. */
+#define EAHMMF_ROPE_PLAIN 0
+#define EAHMMF_ROPE_LINEAR 1
+#define EAHMMF_ROPE_NTK 2
+#define EAHMMF_ROPE_YARN 3
+int eahmmf_rope_inv_freq(int scaling, int n_rot, double base, double factor, int ctx_orig, double beta_fast,
+                         double beta_slow, float* inv_freq, float* mscale);
+
+/* Rows of a q|k|v projection (n_head + 2 n_kv heads of hd floats, row stride ld) into the cache: every q and k head
+ * x / sqrt(mean x^2 + eps) * w where d_qnorm (d_knorm) [hd] is given, then its rotation; q goes to d_q (row stride ldq,
+ * 32 bits), k and v to their positions' pages, rounded once to the pool's type. Row buffers and weights 16-byte
+ * aligned, strides multiples of 4. A row at a negative position (fewer cached positions than rows) gets a zero q row
+ * and appends nothing. Two rows of a call must not share a position of a page. Asynchronous. */
+int eahmmf_cuda_rope_append(const EahmmfPagedKv* kv, int layer, const EahmmfPagedSeqs* seqs, const EahmmfRope* rope,
+                            int n_head, const float* d_qkv, int ld, const float* d_qnorm, const float* d_knorm,
+                            float eps, float* d_q, int ldq, void* stream, int* d_status);
+
+/* Attention of every row over its sequence's cached positions (its own row appended before): for q head h of kv head
+ * h / (n_head / n_kv), out = softmax(scale q k^T) v over the positions j <= p of the row at p, and, where window > 0,
+ * of those j > p - window or j < n_sink. A row that sees nothing is zero. Positions that no row of a sequence's call
+ * sees may hold anything; a NaN or an infinity in v at a position that a later row of the same call sees can reach
+ * earlier rows of that sequence. n_head a multiple of n_kv, at most 64 q heads per kv head; row strides multiples of 4,
+ * buffers 16-byte aligned. The workspace (256-byte aligned) is written and read within the call: calls that may run at
+ * the same time need one each. Asynchronous; results do not depend on what else runs. */
+size_t eahmmf_cuda_paged_attention_workspace_bytes(const EahmmfPagedKv* kv, const EahmmfPagedSeqs* seqs, int n_head);
+int eahmmf_cuda_paged_attention(const EahmmfPagedKv* kv, int layer, const EahmmfPagedSeqs* seqs, int n_head,
+                                const float* d_q, int ldq, float scale, int window, int n_sink, float* d_out, int ldo,
+                                void* d_workspace, size_t workspace_bytes, void* stream, int* d_status);
+
+/* Copies of whole pages in every layer of both pools: pair i copies page pairs[2i] to page pairs[2i + 1]. The list is in
+ * HOST memory and is taken before the call returns. No page may be written twice, and none both read and written
+ * (EAHMMF_ST_BAD_ARG; a page id outside the pool: EAHMMF_ST_BAD_INDEX); nothing is launched then. Asynchronous. */
+int eahmmf_cuda_pages_copy(const EahmmfPagedKv* kv, const int* pairs, int n, void* stream);
+
+/* The pages of a cache on the host: which sequence holds which pages, how many share one, and the copies that a step
+ * needs before its kernels run. No device memory and no stream: the caller uploads the table (eahmmf_pages_table) and
+ * runs the recorded copies (eahmmf_pages_take_copies -> eahmmf_cuda_pages_copy) before the step's appends. Calls return
+ * EAHMMF_ST_* and change nothing unless 0; single-threaded use per handle.
+ *  - create: n_pages pages of `page` positions, n_seq sequences of at most max_pages pages; NULL on bad arguments;
+ *  - extend: positions up to len (not below the present length) get pages, the lowest free ones; a part-filled last
+ *    page that another sequence shares is replaced by a copy of it (recorded). EAHMMF_ST_CAPACITY: not enough free
+ *    pages, or more than max_pages;
+ *  - fork: the empty sequence dst takes src's length and shares its pages;
+ *  - truncate: the sequence is cut to len positions (0 empties it), pages behind them are given back; not into the
+ *    middle of a page that slide gave back (EAHMMF_ST_BAD_ARG);
+ *  - slide: pages wholly before first_pos and wholly behind the first n_sink positions are given back (a window has
+ *    left them); their table entries become -1 and the length stays;
+ *  - compact: pages move to the lowest places of the pool (recorded as copies, tables changed), so that what lies
+ *    behind the used ones is free; refused while copies are recorded;
+ *  - take_copies: writes the recorded pairs (from, to) and forgets them, returns their number; with cap too small it
+ *    returns the number and takes nothing. Pages given back while copies are recorded are free after this call;
+ *  - table: [n_seq][ld] page ids, -1 behind a sequence's pages, and (optional) the lengths;
+ *  - free_count: pages that extend can take now; refs: holders of a page (-1: no such page). */
+typedef struct EahmmfPages EahmmfPages;
+EahmmfPages* eahmmf_pages_create(int n_pages, int page, int n_seq, int max_pages);
+void eahmmf_pages_destroy(EahmmfPages* p);
+int eahmmf_pages_extend(EahmmfPages* p, int seq, int len);
+int eahmmf_pages_fork(EahmmfPages* p, int src, int dst);
+int eahmmf_pages_truncate(EahmmfPages* p, int seq, int len);
+int eahmmf_pages_slide(EahmmfPages* p, int seq, int first_pos, int n_sink);
+int eahmmf_pages_compact(EahmmfPages* p);
+int eahmmf_pages_take_copies(EahmmfPages* p, int* pairs, int cap);
+int eahmmf_pages_table(const EahmmfPages* p, int* table, int ld, int* len);
+int eahmmf_pages_free_count(const EahmmfPages* p);
+int eahmmf_pages_refs(const EahmmfPages* p, int id);
+
 /* ---- 3. device backend (eahmmf::B200Device) --------------------------------------------------- */
 
 typedef struct EahmmfDev EahmmfDev;
