@@ -192,6 +192,8 @@ __global__ void __launch_bounds__(CP_NT) k_pages_copy(uint4* __restrict__ k, uin
 //   16-bit pools   m16n8k16: (q_hi + q_lo) k and (p_hi + p_lo) v. Rows of q are first scaled by a power of two to
 //                  [2^8, 2^9), p by 2^15, so that the low parts stay above the smallest half
 //   32-bit pools   m16n8k8 on 11-bit parts of a 32-bit range: hi hi + lo hi + hi lo (lo lo is 2^-22 of it)
+// The matrix instructions cut their running sums where an addition would round, which biases long chains: a step's
+// products go to sums of their own (low parts first) and are added to the row's sums in the ordinary way.
 // Up to 8 rows (STACK) the two parts of a row lie in rows g and g + 8 of one instruction: no extra work, and the
 // thread that holds row g holds row g + 8 too. 16 rows take an instruction for each part.
 constexpr int PA_NW = 4, PA_NT = 32 * PA_NW;
@@ -245,6 +247,10 @@ __device__ __forceinline__ Units units_of(const Seq& sq, int window, int n_sink,
     return u;
 }
 
+__device__ __forceinline__ bool step_takes(const PagedAttnArgs& A, const Seq& sq) {
+    return sq.q > 0 && (long long)sq.q * A.c.grp <= A.rows_max;
+}
+
 template <typename T, int HD, bool STACK>
 struct AttnSmem {
     static constexpr int RT = STACK ? 8 : 16;
@@ -280,7 +286,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
     // ---- this block's share of the call: work items in (sequence, kv head, row tile, unit) order
     auto weight = [&](int s, bool flag) -> long long {
         const Seq sq = paged_seq(a, s, flag);
-        if (sq.q == 0) return 0;
+        if (!step_takes(A, sq)) return 0;
         return (long long)units_of(sq, A.window, A.n_sink, UNIT).n() * a.n_kv * ((sq.q * a.grp + RT - 1) / RT);
     };
     long long total = 0, mine = 0;
@@ -329,8 +335,9 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
         const Units un = units_of(sq, A.window, A.n_sink, UNIT);
         const int nu = un.n(), nrt = (sq.q * a.grp + RT - 1) / RT;
         const long long here = (long long)nu * nrt * a.n_kv;
-        if (sq.q == 0 || at >= seq_at + here) {
-            if (sq.q) seq_at += here;
+        const bool takes = step_takes(A, sq);
+        if (!takes || at >= seq_at + here) {
+            if (takes) seq_at += here;
             seq++;
             continue;
         }
@@ -457,9 +464,11 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                 for (int c = 0; c < VC; c++) vr[j][c] = ok ? __ldg(src + 8 * c) : make_uint4(0, 0, 0, 0);
             }
         };
-        float o[NT][4];
+        float o[NT][2 * NR];
 #pragma unroll
-        for (int n = 0; n < NT; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int i = 0; i < 2 * NR; i++) o[n][i] = 0.f;
         float m[NR], l[NR];
 #pragma unroll
         for (int i = 0; i < NR; i++) {
@@ -471,9 +480,11 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
         load_k(base, p);
         load_v(base, p);
         for (int it = 0; it < n_it; it++) {
-            float sacc[JT][4];
+            float sacc[JT][4], slow[JT][4];  // the high parts' product and the rest, joined once at the end
 #pragma unroll
-            for (int j = 0; j < JT; j++) sacc[j][0] = sacc[j][1] = sacc[j][2] = sacc[j][3] = 0.f;
+            for (int j = 0; j < JT; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) sacc[j][i] = slow[j][i] = 0.f;
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 uint32_t ah[4], al[4];
@@ -491,14 +502,14 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                     const uint32_t b0 = (k & 1) ? w.z : w.x, b1 = (k & 1) ? w.w : w.y;
                     if (H16) {
                         mma_f16(sacc[j], ah, b0, b1);
-                        if (!STACK) mma_f16(sacc[j], al, b0, b1);
+                        if (!STACK) mma_f16(slow[j], al, b0, b1);
                     } else {
                         uint32_t h0, l0, h1, l1;
                         split_tf32(__uint_as_float(b0), h0, l0);
                         split_tf32(__uint_as_float(b1), h1, l1);
                         mma_tf32(sacc[j], ah, h0, h1);
-                        mma_tf32(sacc[j], ah, l0, l1);
-                        if (!STACK) mma_tf32(sacc[j], al, h0, h1);
+                        mma_tf32(slow[j], ah, l0, l1);
+                        if (!STACK) mma_tf32(slow[j], al, h0, h1);
                     }
                 }
             }
@@ -515,7 +526,9 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
 #pragma unroll
                 for (int j = 0; j < PT; j++) {
                     const int pos = p_cur + 8 * (j >> 1) + 2 * t + (j & 1);
-                    const float raw = STACK ? sacc[j >> 1][j & 1] + sacc[j >> 1][(j & 1) + 2] : sacc[j >> 1][(j & 1) + 2 * i];
+                    const int e = (j & 1) + 2 * i;
+                    float raw = sacc[j >> 1][e] + slow[j >> 1][e];
+                    if (STACK) raw += sacc[j >> 1][e + 2];
                     const bool see = live && pos <= lim[i] && (pos >= low[i] || pos < A.n_sink);
                     sv[i][j] = see ? raw * cs[i] : -INFINITY;
                     mx[i] = fmaxf(mx[i], sv[i][j]);
@@ -535,12 +548,9 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                     m[i] = mx[i];
                 }
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    o[n][0] *= al[0];
-                    o[n][1] *= al[0];
-                    o[n][2] *= al[NR - 1];
-                    o[n][3] *= al[NR - 1];
-                }
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int i = 0; i < 2 * NR; i++) o[n][i] *= al[i >> 1];
             }
             uint32_t ph[4], pl[4];
 #pragma unroll
@@ -565,22 +575,25 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
 #pragma unroll
                 for (int e = 0; e < 16 / (int)sizeof(T); e++) {
                     const int n = c * (16 / (int)sizeof(T)) + e;
+                    float s[4] = {0.f, 0.f, 0.f, 0.f};  // this step's part of the sums, see "Numerics"
                     if (H16) {
                         const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
                         auto word = [&](const uint4& w) { return (e >> 1) == 0 ? w.x : (e >> 1) == 1 ? w.y : (e >> 1) == 2 ? w.z : w.w; };
                         const uint32_t b0 = __byte_perm(word(vr[0][c]), word(vr[1][c]), sel);
                         const uint32_t b1 = __byte_perm(word(vr[PT - 2][c]), word(vr[PT - 1][c]), sel);
-                        mma_f16(o[n], ph, b0, b1);
-                        if (!STACK) mma_f16(o[n], pl, b0, b1);
+                        if (!STACK) mma_f16(s, pl, b0, b1);
+                        mma_f16(s, ph, b0, b1);
                     } else {
                         auto word = [&](const uint4& w) { return e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w; };
                         uint32_t h0, l0, h1, l1;
                         split_tf32(__uint_as_float(word(vr[0][c])), h0, l0);
                         split_tf32(__uint_as_float(word(vr[1][c])), h1, l1);
-                        mma_tf32(o[n], ph, h0, h1);
-                        mma_tf32(o[n], ph, l0, l1);
-                        if (!STACK) mma_tf32(o[n], pl, h0, h1);
+                        if (!STACK) mma_tf32(s, pl, h0, h1);
+                        mma_tf32(s, ph, l0, l1);
+                        mma_tf32(s, ph, h0, h1);
                     }
+#pragma unroll
+                    for (int i = 0; i < 2 * NR; i++) o[n][i] += STACK ? s[i] + s[i + 2 * (STACK ? 1 : 0)] : s[i];
                 }
             load_v(base, p);
         }
@@ -599,13 +612,14 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
             constexpr int E = 16 / (int)sizeof(T);
             const int col = E * (2 * t + 8 * (n / E)) + n % E;
             if (STACK) {
-                S.o[warp][g][col] = o[n][0] + o[n][2];
-                S.o[warp][g][col + E] = o[n][1] + o[n][3];
-            } else {
                 S.o[warp][g][col] = o[n][0];
                 S.o[warp][g][col + E] = o[n][1];
-                S.o[warp][g + 8][col] = o[n][2];
-                S.o[warp][g + 8][col + E] = o[n][3];
+            } else {
+#pragma unroll
+                for (int i = 0; i < NR; i++) {
+                    S.o[warp][g + 8 * i][col] = o[n][2 * i];
+                    S.o[warp][g + 8 * i][col + E] = o[n][2 * i + 1];
+                }
             }
         }
         __syncthreads();
@@ -652,28 +666,34 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
     }
 }
 
-// Joins the records of the row tiles that the split cut: block (b, r) takes row r of the tile that block b of
-// k_paged_attn began and left to the blocks after it (meta: how many, sequence, kv head, row tile).
+// Joins the records of the row tiles that the split cut. Block (b, y) takes rows of the tile that block b of the
+// attention began and left to the blocks after it (meta: how many, sequence, kv head, row tile): with ONE one row, its
+// records dealt over the block (a long context is cut often), else a row to each group of hd / 4 threads.
 constexpr int PM_NT = 256;
-template <int HD>
-__global__ void __launch_bounds__(PM_NT) k_paged_merge(PagedAttnArgs A, int rt_rows) {
-    constexpr int LN = HD / 4, G = PM_NT / LN;  // lanes of a row, records taken at once
-    __shared__ __align__(16) float so[G][HD];
+struct MergeShape {
+    int tile_rows;  // rows from one row tile to the next
+    int cap;        // rows of a record: o [cap][hd], m [cap], sum [cap]
+};
+template <int HD, bool ONE>
+__global__ void __launch_bounds__(PM_NT) k_paged_merge(PagedAttnArgs A, MergeShape ms) {
+    constexpr int LN = HD / 4, G = PM_NT / LN;
+    __shared__ __align__(16) float so[ONE ? G : 1][HD];
     __shared__ float sm[G], sl[G];
-    const int b = blockIdx.x, r = blockIdx.y, lane = threadIdx.x % LN, grp = threadIdx.x / LN;
+    const int b = blockIdx.x, lane = threadIdx.x % LN, grp = threadIdx.x / LN;
+    const int r = ONE ? blockIdx.y : blockIdx.y * G + grp, step = ONE ? G : 1;
     pdl_wait();
     pdl_trigger();
     const int4 me = A.meta[b];
     if (me.x == 0) return;
     const Seq sq = paged_seq(A.c, me.y, false);
-    const int rr = me.w * rt_rows + r;
-    if (rr >= sq.q * A.c.grp) return;
+    const int rr = me.w * ms.tile_rows + r;
+    if (r >= ms.tile_rows || rr >= sq.q * A.c.grp) return;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int j = grp; j <= me.x; j += G) {
-        const float* rec = A.part + ((size_t)(b + j) * 2 + (j == 0 ? 1 : 0)) * part_floats(HD);
-        const float mj = rec[16 * HD + r], lj = rec[16 * HD + 16 + r];
+    for (int j = ONE ? grp : 0; j <= me.x; j += step) {
+        const float* rec = A.part + ((size_t)(b + j) * 2 + (j == 0 ? 1 : 0)) * ((size_t)ms.cap * (HD + 2));
+        const float mj = rec[ms.cap * HD + r], lj = rec[ms.cap * HD + ms.cap + r];
         const float4 f = reinterpret_cast<const float4*>(rec)[r * LN + lane];
         const float mn = fmaxf(m, mj);
         if (mn == -INFINITY) {  // nothing seen so far (a NaN sum stays one)
@@ -688,26 +708,30 @@ __global__ void __launch_bounds__(PM_NT) k_paged_merge(PagedAttnArgs A, int rt_r
         o.z = fmaf(o.z, ea, f.z * eb_);
         o.w = fmaf(o.w, ea, f.w * eb_);
     }
-    reinterpret_cast<float4*>(so[grp])[lane] = o;
-    if (lane == 0) {
-        sm[grp] = m;
-        sl[grp] = l;
-    }
-    __syncthreads();
-    if (grp) return;
-    float M = -INFINITY, L = 0.f;
+    float L = l;
+    if (ONE) {
+        reinterpret_cast<float4*>(so[grp])[lane] = o;
+        if (lane == 0) {
+            sm[grp] = m;
+            sl[grp] = l;
+        }
+        __syncthreads();
+        if (grp) return;
+        float M = -INFINITY;
+        L = 0.f;
 #pragma unroll
-    for (int j = 0; j < G; j++) M = fmaxf(M, sm[j]);
-    o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int j = 0; j < G; j++) M = fmaxf(M, sm[j]);
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < G; j++) {
-        const float e = sm[j] == -INFINITY ? 0.f : exp2f(sm[j] - M);
-        const float4 f = reinterpret_cast<const float4*>(so[j])[lane];
-        L = fmaf(sl[j], e, L);
-        o.x = fmaf(f.x, e, o.x);
-        o.y = fmaf(f.y, e, o.y);
-        o.z = fmaf(f.z, e, o.z);
-        o.w = fmaf(f.w, e, o.w);
+        for (int j = 0; j < G; j++) {
+            const float e = sm[j] == -INFINITY ? 0.f : exp2f(sm[j] - M);
+            const float4 f = reinterpret_cast<const float4*>(so[j])[lane];
+            L = sm[j] == -INFINITY ? L + sl[j] : fmaf(sl[j], e, L);
+            o.x = fmaf(f.x, e, o.x);
+            o.y = fmaf(f.y, e, o.y);
+            o.z = fmaf(f.z, e, o.z);
+            o.w = fmaf(f.w, e, o.w);
+        }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const int tok = rr / A.c.grp;
@@ -715,51 +739,64 @@ __global__ void __launch_bounds__(PM_NT) k_paged_merge(PagedAttnArgs A, int rt_r
                                4 * lane) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
-// Raises a kernel's dynamic shared-memory limit, once on each device.
-template <typename T, int HD, bool STACK, typename Kern>
-cudaError_t smem_limit(Kern k, size_t bytes) {
-    constexpr int MAX_DEV = 64;
-    static std::mutex mu;
-    static bool done[MAX_DEV] = {};  // one array per instance, that is per kernel
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess || dev < 0 || dev >= MAX_DEV) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
-    std::lock_guard<std::mutex> g(mu);
-    if (!done[dev]) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess) done[dev] = true;
-    return e;
-}
-
 template <typename T, int HD, bool STACK>
 cudaError_t attn_go(const PagedAttnArgs& A, cudaStream_t st) {
     constexpr int RT = STACK ? 8 : 16;
-    cudaError_t e = smem_limit<T, HD, STACK>(k_paged_attn<T, HD, STACK>, sizeof(AttnSmem<T, HD, STACK>));
+    cudaError_t e = smem_limit<AttnSmem<T, HD, STACK>>(k_paged_attn<T, HD, STACK>, sizeof(AttnSmem<T, HD, STACK>));
     if (e != cudaSuccess) return e;
     e = launch_pdl(k_paged_attn<T, HD, STACK>, dim3(A.grid), dim3(PA_NT), sizeof(AttnSmem<T, HD, STACK>), st, A);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_paged_merge<HD>, dim3(A.grid, RT), dim3(PM_NT), 0, st, A, RT);
+    return launch_pdl(k_paged_merge<HD, true>, dim3(A.grid, RT), dim3(PM_NT), 0, st, A, MergeShape{RT, 16});
 }
 template <typename T, int HD>
-cudaError_t attn_rows(const PagedAttnArgs& A, int max_q, cudaStream_t st) {
-    return max_q * A.c.grp <= 8 ? attn_go<T, HD, true>(A, st) : attn_go<T, HD, false>(A, st);
+cudaError_t attn_rows(const PagedAttnArgs& A, bool stack, cudaStream_t st) {
+    return stack ? attn_go<T, HD, true>(A, st) : attn_go<T, HD, false>(A, st);
 }
 
 int attn_grid() { return 2 * sm_count(); }
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+size_t step_ws_bytes(int hd) {
+    return align256((size_t)attn_grid() * sizeof(int4)) + align256((size_t)attn_grid() * 2 * part_floats(hd) * sizeof(float));
+}
+size_t tc_ws_bytes(int hd) {
+    return align256((size_t)paged_tc_grid() * sizeof(int4)) + (size_t)paged_tc_grid() * 2 * 256 * (hd + 2) * sizeof(float);
+}
+bool tc_call(int type, int grp, int max_q) { return type == T_F16 && max_q * grp > STEP_ROWS; }
+
+void carve(PagedAttnArgs& A, int grid, void* ws) {
+    A.grid = grid;
+    A.meta = static_cast<int4*>(ws);
+    A.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + align256((size_t)grid * sizeof(int4)));
+}
 }  // namespace
 
-size_t paged_attn_ws_bytes(int hd) {
-    return align256((size_t)attn_grid() * sizeof(int4)) + (size_t)attn_grid() * 2 * part_floats(hd) * sizeof(float);
+size_t paged_attn_ws_bytes(int type, int hd, int grp, int max_q) {
+    return step_ws_bytes(hd) + (tc_call(type, grp, max_q) ? tc_ws_bytes(hd) : 0);
 }
 
 cudaError_t launch_paged_attention(int type, int hd, int max_q, int max_kv, PagedAttnArgs A, void* ws, cudaStream_t st) {
     (void)max_kv;
-    A.grid = attn_grid();
+    const bool tc = tc_call(type, A.c.grp, max_q);
+    A.rows_min = 0;
+    A.rows_max = 0x7fffffff;
+    if (tc) {
+        // sequences of more than STEP_ROWS rows as chunks; the others, if there may be any, by the step kernel
+        A.rows_min = A.c.n_seq > 1 ? STEP_ROWS : 0;
+        A.rows_max = A.rows_min;
+        A.min_units = 1;
+        carve(A, paged_tc_grid(), static_cast<uint8_t*>(ws) + step_ws_bytes(hd));
+        cudaError_t e = launch_paged_attn_tc(hd, A, st);
+        if (e != cudaSuccess) return e;
+        const MergeShape ms{2 * (128 / A.c.grp) * A.c.grp, 256};
+        e = hd == 128 ? launch_pdl(k_paged_merge<128, false>, dim3(A.grid, 256 / (PM_NT / 32)), dim3(PM_NT), 0, st, A, ms)
+                      : launch_pdl(k_paged_merge<64, false>, dim3(A.grid, 256 / (PM_NT / 16)), dim3(PM_NT), 0, st, A, ms);
+        if (e != cudaSuccess || A.c.n_seq == 1) return e;
+    }
     A.min_units = 4;
-    A.meta = static_cast<int4*>(ws);
-    A.part = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + align256((size_t)A.grid * sizeof(int4)));
-    if (type == T_F16) return hd == 128 ? attn_rows<__half, 128>(A, max_q, st) : attn_rows<__half, 64>(A, max_q, st);
-    return hd == 128 ? attn_rows<float, 128>(A, max_q, st) : attn_rows<float, 64>(A, max_q, st);
+    carve(A, attn_grid(), ws);
+    const bool stack = max_q * A.c.grp <= 8;
+    if (type == T_F16) return hd == 128 ? attn_rows<__half, 128>(A, stack, st) : attn_rows<__half, 64>(A, stack, st);
+    return hd == 128 ? attn_rows<float, 128>(A, stack, st) : attn_rows<float, 64>(A, stack, st);
 }
 
 cudaError_t launch_rope_append(int type, int hd, const PagedArgs& a, const EahmmfRope& rope, const float* qkv, int ld,

@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "../../include/eahmmf_b200.h"
 #include "common.cuh"
 
@@ -58,11 +60,32 @@ struct PagedAttnArgs {
     int window, n_sink;  // window 0: every earlier position is visible
     int grid;            // blocks of the split launch, also the records of `part`
     int min_units;       // least share of a block
+    int rows_min, rows_max;  // sequences of more rows (tokens x q heads of a kv head) than rows_min go to the chunk
+                             // kernel, of at most rows_max to the step kernel
     float* part;         // [grid][2] partial results
     int4* meta;          // [grid] the row tile a block began and did not finish
 };
-size_t paged_attn_ws_bytes(int hd);
+constexpr int STEP_ROWS = 16;  // rows of a sequence that the step kernel takes in one row tile
+size_t paged_attn_ws_bytes(int type, int hd, int grp, int max_q);
 cudaError_t launch_paged_attention(int type, int hd, int max_q, int max_kv, PagedAttnArgs a, void* ws, cudaStream_t st);
+
+int paged_tc_grid();  // blocks of the chunk kernel
+cudaError_t launch_paged_attn_tc(int hd, const PagedAttnArgs& A, cudaStream_t st);
+
+// Raises a kernel's dynamic shared-memory limit, once on each device; Tag: a type of the kernel's own.
+template <typename Tag, typename Kern>
+cudaError_t smem_limit(Kern k, size_t bytes) {
+    constexpr int MAX_DEV = 64;
+    static std::mutex mu;
+    static bool done[MAX_DEV] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev < 0 || dev >= MAX_DEV) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> g(mu);
+    if (!done[dev]) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done[dev] = true;
+    return e;
+}
 
 cudaError_t launch_pages_copy(const EahmmfPagedKv& kv, const int* pairs, int n, cudaStream_t st);
 

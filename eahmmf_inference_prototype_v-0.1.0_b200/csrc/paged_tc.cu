@@ -1,0 +1,607 @@
+// paged_tc.cu -- attention of chunks of new tokens over 16-bit pages with the 5th-generation tensor cores.
+//
+// The mathematics is paged.cu's. A block takes two tiles of 128 rows (tokens x the q heads of one kv head) of a
+// sequence and walks units of 128 positions; per tile and unit
+//   S = q_lo k^T + q_hi k^T   (128 x 128, tensor memory)
+//   p = 2^(S c - m + 15) in two 11-bit parts, written over S
+//   O = p_lo v + p_hi v       (128 x hd, tensor memory, started afresh for every unit)
+// O is added to the row's sums in registers: the tensor cores cut their sums, and one chain over a long context would
+// bias them (12,289 positions in one chain: 5.7e-6 relative; in chains of one unit: see the table of measurements).
+//
+// Operands: k and v by TMA from the pages (boxes of gcd(page, 128) positions, 128-byte swizzle), k read with hd
+// contiguous, v with hd contiguous as the transposed operand; q scaled and split by the softmax warps; p from tensor memory.
+//
+// Bound: 4 hd flops per row and position, twice because of the two parts: 2 * 2 * 2 * 128 * 128 * hd per tile and unit. Two
+// tiles share every k and v tile and take turns: while one tile's scores are in the softmax the other's products run.
+//
+// Warps: 0-3 softmax of tile 0, 4-7 of tile 1 (thread = row = tensor-memory lane), 8 loads, 9 issues the products,
+// 10 and 11 only give their registers to the softmax warps.
+#include <cuda.h>
+
+#include <mutex>
+
+#include "kernels.cuh"
+#include "paged.cuh"
+#include "tc.cuh"
+
+namespace eb {
+namespace {
+
+constexpr int TC_NT = 384;
+// Registers: 384 threads are launched with 168 each; a softmax thread holds its row's hd sums beside its scores. Shares
+// after the split: 2 x 128 x 224 + 128 x 56 = 384 x 168, the launch's own total (checked before the launch).
+constexpr int REGS_LAUNCH = 168;
+#define EB_REGS_MORE() asm volatile("setmaxnreg.inc.sync.aligned.u32 224;")
+#define EB_REGS_LESS() asm volatile("setmaxnreg.dec.sync.aligned.u32 56;")
+constexpr int UNIT = 128;  // positions of a unit
+constexpr int MROWS = 128;
+constexpr int VALID_RING = 8;
+
+template <int HD>
+struct Tc {
+    static constexpr int HALVES = HD / 64;               // 128-byte column blocks of an operand tile
+    static constexpr int BLK = 128 * 128;                // bytes of a column block of 128 rows
+    static constexpr int TILE = HALVES * BLK;            // bytes of a 128 x hd operand tile
+    static constexpr int NST = HD == 128 ? 3 : 8;        // tiles of k and v in flight
+    static constexpr int Q_BYTES = 2 * 2 * TILE;         // two row tiles, two parts
+    static constexpr int SMEM = 1024 + Q_BYTES + NST * TILE + 512;
+    static constexpr uint32_t S_COL = 0, O_COL = 256;    // tensor memory: S0 S1 O0 O1
+    static constexpr uint32_t COLS = 512;
+};
+struct Bars {
+    uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2], pv_done[2];
+    uint32_t valid[VALID_RING];  // by unit: which boxes lie in pages of the pool
+    uint32_t tmem;
+    int seq;
+    long long start, scan[TC_NT / 32];
+};
+static_assert(sizeof(Bars) <= 512, "");
+
+// Shared-memory matrix descriptors, 128-byte swizzle: rows of 128 bytes, groups of 8 rows 1024 bytes apart; lbo: distance of
+// the 64-element blocks of a transposed operand. The high word is the same for every operand, so that a product costs
+// one 32-bit addition for each descriptor.
+constexpr uint32_t DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
+__device__ __forceinline__ void mma_smem_a(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(DESC_HI));
+}
+__device__ __forceinline__ void mma_tmem_a(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "n"(DESC_HI));
+}
+#define EB_R16(r, o)                                                                                                        \
+    "=r"(r[o + 0]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]),         \
+        "=r"(r[o + 7]), "=r"(r[o + 8]), "=r"(r[o + 9]), "=r"(r[o + 10]), "=r"(r[o + 11]), "=r"(r[o + 12]), "=r"(r[o + 13]), \
+        "=r"(r[o + 14]), "=r"(r[o + 15])
+#define EB_W16(r, o)                                                                                                    \
+    "r"(r[o + 0]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]),            \
+        "r"(r[o + 7]), "r"(r[o + 8]), "r"(r[o + 9]), "r"(r[o + 10]), "r"(r[o + 11]), "r"(r[o + 12]), "r"(r[o + 13]),    \
+        "r"(r[o + 14]), "r"(r[o + 15])
+// 32 columns of this warp's 32 lanes; the wait names the registers, so that nothing uses them before it
+__device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : EB_R16(r, 0), EB_R16(r, 16)
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
+    asm volatile(""
+                 : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+        EB_W16(r, 0), EB_W16(r, 16)
+        : "memory");
+}
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tma_box(const CUtensorMap* map, void* dst, uint64_t* bar, int x, int row, int head, int page) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(row), "r"(head), "r"(page)
+        : "memory");
+}
+
+// The walk of a block through its share: work in (sequence, pair of row tiles, kv head, unit) order.
+struct Pair {
+    int t0, t1;                   // tokens of the pair
+    int low_min, lim_max;         // positions that some row sees: [low_min, lim_max] and the first n_sink
+    int us, uw, ue;               // their units
+    __device__ __forceinline__ int n() const { return max(1, us + ue - uw); }
+    __device__ __forceinline__ int unit(int i) const { return i < us ? i : uw + (i - us); }
+};
+__device__ __forceinline__ Pair pair_of(const PagedAttnArgs& A, const Seq& sq, int pair, int tpt) {
+    Pair p;
+    p.t0 = pair * 2 * tpt;
+    p.t1 = min(sq.q, p.t0 + 2 * tpt);
+    const int first = sq.kv - sq.q + p.t0;
+    p.lim_max = sq.kv - sq.q + p.t1 - 1;
+    p.low_min = A.window > 0 ? first - A.window + 1 : 0;
+    p.ue = (max(p.lim_max, -1) + UNIT) / UNIT;
+    p.uw = min(max(0, p.low_min) / UNIT, p.ue);
+    p.us = A.window > 0 ? min((min(A.n_sink, max(p.lim_max, -1) + 1) + UNIT - 1) / UNIT, p.uw) : 0;
+    return p;
+}
+__device__ __forceinline__ bool tc_takes(const PagedAttnArgs& A, const Seq& sq) { return sq.q > 0 && sq.q * A.c.grp > A.rows_min; }
+
+struct Walk {
+    const PagedAttnArgs& A;
+    int tpt, seq, pair = 0;
+    long long at, end, base;
+    Seq sq;
+    Pair pr;
+    int kvh, u0, n_it, nu;
+    __device__ Walk(const PagedAttnArgs& A_, int tpt_, int seq_, long long base_, long long at_, long long end_)
+        : A(A_), tpt(tpt_), seq(seq_), at(at_), end(end_), base(base_) {
+        sq.q = 0;
+    }
+    __device__ bool next() {
+        while (at < end) {
+            if (seq >= A.c.n_seq) return false;
+            sq = paged_seq(A.c, seq, false);
+            if (!tc_takes(A, sq) || pair * 2 * tpt >= sq.q) {
+                seq++;
+                pair = 0;
+                continue;
+            }
+            pr = pair_of(A, sq, pair, tpt);
+            nu = pr.n();
+            const long long w = (long long)nu * A.c.n_kv;
+            if (at >= base + w) {
+                base += w;
+                pair++;
+                continue;
+            }
+            const int idx = (int)(at - base);
+            kvh = idx / nu;
+            u0 = idx - kvh * nu;
+            n_it = (int)min((long long)(nu - u0), end - at);
+            at += n_it;
+            return true;
+        }
+        return false;
+    }
+};
+
+template <int HD>
+__global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, const __grid_constant__ CUtensorMap kmap,
+                                                            const __grid_constant__ CUtensorMap vmap, int box) {
+    using C = Tc<HD>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* sq_ = sm;                      // q: [tile][lo, hi][column block][128 rows][128 bytes]
+    uint8_t* skv = sm + C::Q_BYTES;         // k, v tiles
+    Bars& B = *reinterpret_cast<Bars*>(skv + C::NST * C::TILE);
+    const PagedArgs& a = A.c;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tpt = MROWS / a.grp;  // tokens of a row tile
+    if (tid == 0) {
+        for (int i = 0; i < C::NST; i++) {
+            mbar_init(&B.kv_full[i], 1);
+            mbar_init(&B.kv_empty[i], 1);
+        }
+        for (int m = 0; m < 2; m++) {
+            mbar_init(&B.q_full[m], MROWS);
+            mbar_init(&B.s_full[m], 2);
+            mbar_init(&B.p_full[m], MROWS);
+            mbar_init(&B.pv_done[m], 1);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 8) tc_alloc(&B.tmem, C::COLS);
+    pdl_wait();
+    pdl_trigger();
+    // ---- this block's share
+    auto weight = [&](int s, bool flag) -> long long {
+        const Seq sq = paged_seq(a, s, flag);
+        if (!tc_takes(A, sq)) return 0;
+        long long n = 0;
+        for (int p = 0; p * 2 * tpt < sq.q; p++) n += pair_of(A, sq, p, tpt).n();
+        return n * a.n_kv;
+    };
+    long long total = 0, mine = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += TC_NT) {
+        mine = s0 + tid < a.n_seq ? weight(s0 + tid, blockIdx.x == 0) : 0;
+        long long v = mine;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane == 0) B.scan[warp] = v;
+        __syncthreads();
+        for (int w = 0; w < TC_NT / 32; w++) total += B.scan[w];
+        __syncthreads();
+    }
+    const long long share = max((total + gridDim.x - 1) / gridDim.x, (long long)A.min_units);
+    const long long begin = share * blockIdx.x, end = min(total, begin + share);
+    if (tid == 0) {
+        A.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+        B.seq = a.n_seq;
+        B.start = 0;
+    }
+    __syncthreads();
+    long long run = 0;
+    for (int s0 = 0; s0 < a.n_seq && begin < total; s0 += TC_NT) {
+        if (a.n_seq > TC_NT) mine = s0 + tid < a.n_seq ? weight(s0 + tid, false) : 0;
+        long long v = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long n = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += n;
+        }
+        if (lane == 31) B.scan[warp] = v;
+        __syncthreads();
+        for (int w = 0; w < warp; w++) v += B.scan[w];
+        v += run;
+        if (mine > 0 && v - mine <= begin && begin < v) {
+            B.seq = s0 + tid;
+            B.start = v - mine;
+        }
+        for (int w = 0; w < TC_NT / 32; w++) run += B.scan[w];
+        __syncthreads();
+        if (run > begin) break;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = B.tmem;
+    Walk w(A, tpt, B.seq, B.start, begin, end);
+    bool ok = true;  // a bounded wait that gives up ends the walk; the other warps' own waits then give up too
+
+    if (warp < 8) {
+        EB_REGS_MORE();
+        // ---------------------------------------------------------------- softmax and sums of row tile mt
+        const int mt = warp >> 2, r = tid & 127;
+        uint8_t* q_lo = sq_ + mt * 2 * C::TILE;
+        uint8_t* q_hi = q_lo + C::TILE;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t s_tm = tmem + lanes + C::S_COL + mt * UNIT, o_tm = tmem + lanes + C::O_COL + mt * 128;
+        uint32_t n_s = 0, n_pv = 0, n_valid = 0;  // uses of the barriers so far
+        while (ok && w.next()) {
+            const int tok = w.pr.t0 + mt * tpt + r / a.grp;
+            if (w.pr.t0 + mt * tpt >= w.pr.t1) {  // the pair has one row tile
+                n_valid += w.n_it;
+                continue;
+            }
+            const bool row_ok = r < tpt * a.grp && tok < w.pr.t1;
+            const int head = w.kvh * a.grp + r % a.grp;
+            const int lim = row_ok ? w.sq.kv - w.sq.q + tok : -1;
+            const int low = A.window > 0 ? lim - A.window + 1 : 0;
+            // ---- q row: a power of two that brings its largest to [2^8, 2^9), then its two parts
+            float cs;
+            {
+                const float4* qr = reinterpret_cast<const float4*>(A.q + (size_t)(w.sq.q0 + (row_ok ? tok : w.pr.t0)) * A.ldq +
+                                                                   (size_t)head * HD);
+                float mx = 0.f;
+#pragma unroll 8
+                for (int c = 0; c < HD / 4; c++) {
+                    const float4 f = qr[c];
+                    mx = fmaxf(fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
+                }
+                const int ex = (int)((__float_as_uint(mx) >> 23) & 255) - 127;
+                float sc = ex < 128 && mx > 0.f ? pow2f(min(max(8 - ex, -100), 100)) : 1.f;
+                cs = fabsf(A.scale) * 1.4426950408889634f / sc;
+                if (A.scale < 0.f) sc = -sc;  // the running maximum is that of +c S
+                if (!row_ok) sc = 0.f;
+#pragma unroll 4
+                for (int c = 0; c < HD / 8; c++) {
+                    const float4 f0 = qr[2 * c], f1 = qr[2 * c + 1];
+                    const float x[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float u = row_ok ? x[2 * i] * sc : 0.f, v = row_ok ? x[2 * i + 1] * sc : 0.f;
+                        const __half2 h = __floats2half2_rn(u, v);
+                        const float2 b = __half22float2(h);
+                        const __half2 l2 = __floats2half2_rn(u - b.x, v - b.y);
+                        hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+                        lo[i] = *reinterpret_cast<const uint32_t*>(&l2);
+                    }
+                    const int at = (c >> 3) * C::BLK + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4*>(q_hi + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    *reinterpret_cast<uint4*>(q_lo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&B.q_full[mt]);
+            }
+            float acc[HD];
+#pragma unroll
+            for (int c = 0; c < HD; c++) acc[c] = 0.f;
+            float m = -INFINITY, l = 0.f, alpha = 1.f;
+            auto add_o = [&]() {  // acc <- acc alpha + O of the unit before
+#pragma unroll
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t o[32];
+                    tm_ld32(o_tm + c, o);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) acc[c + j] = fmaf(acc[c + j], alpha, __uint_as_float(o[j]));
+                }
+            };
+            for (int i = 0; i < w.n_it; i++, n_valid++) {
+                if (i > 0) {
+                    ok = mbar_wait_bounded(&B.pv_done[mt], n_pv++ & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    add_o();
+                }
+                ok = mbar_wait_bounded(&B.s_full[mt], n_s++ & 1);
+                if (!ok) break;
+                tc_fence_after();
+                const int p0 = w.pr.unit(w.u0 + i) * UNIT;
+                const uint32_t valid = B.valid[n_valid % VALID_RING];
+                const int n_box = UNIT / box;
+                const bool all = p0 + UNIT - 1 <= lim && (p0 >= low || p0 + UNIT <= A.n_sink) && valid == (1u << n_box) - 1;
+                float mx = -INFINITY;
+                auto see = [&](int j) {
+                    const int p = p0 + j;
+                    return p <= lim && (p >= low || p < A.n_sink) && ((valid >> (j / box)) & 1);
+                };
+                const bool plain = __all_sync(0xffffffffu, all);
+#pragma unroll
+                for (int c = 0; c < UNIT; c += 32) {
+                    uint32_t s[32];
+                    tm_ld32(s_tm + c, s);
+                    if (plain) {
+#pragma unroll
+                        for (int j = 0; j < 32; j++) mx = fmaxf(mx, __uint_as_float(s[j]));
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; j++) mx = see(c + j) ? fmaxf(mx, __uint_as_float(s[j])) : mx;
+                    }
+                }
+                const float mn = mx == -INFINITY ? m : fmaxf(m, mx * cs);
+                alpha = mn == -INFINITY ? 1.f : exp2f(m - mn);
+                m = mn;
+                const float mo = mn == -INFINITY ? 0.f : mn - 15.f;
+                float ls = 0.f;
+#pragma unroll
+                for (int c = 0; c < UNIT; c += 32) {
+                    uint32_t s[32];
+                    tm_ld32(s_tm + c, s);
+                    uint32_t out[32];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        float u = exp2f(fmaf(__uint_as_float(s[j]), cs, -mo)), v = exp2f(fmaf(__uint_as_float(s[j + 1]), cs, -mo));
+                        if (!plain) {
+                            u = see(c + j) ? u : 0.f;
+                            v = see(c + j + 1) ? v : 0.f;
+                        }
+                        ls += u + v;
+                        const __half2 h = __floats2half2_rn(u, v);
+                        const float2 b = __half22float2(h);
+                        const __half2 l2 = __floats2half2_rn(u - b.x, v - b.y);
+                        out[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
+                        out[16 + j / 2] = *reinterpret_cast<const uint32_t*>(&l2);
+                    }
+                    tm_st32(s_tm + c, out);
+                }
+                l = fmaf(l, alpha, ls);
+                tm_wait_st();
+                tc_fence_before();
+                mbar_arrive(&B.p_full[mt]);
+            }
+            if (ok) ok = mbar_wait_bounded(&B.pv_done[mt], n_pv++ & 1);
+            if (!ok) break;
+            tc_fence_after();
+            add_o();
+            tc_fence_before();
+            const bool whole = w.u0 == 0 && w.n_it == w.nu;
+            if (whole) {
+                if (row_ok) {
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    float4* o = reinterpret_cast<float4*>(A.out + (size_t)(w.sq.q0 + tok) * A.ldo + (size_t)head * HD);
+#pragma unroll
+                    for (int c = 0; c < HD; c += 4)
+                        o[c / 4] = make_float4(acc[c] * inv, acc[c + 1] * inv, acc[c + 2] * inv, acc[c + 3] * inv);
+                }
+            } else {  // records hold rows in (token, head) order: the two tiles' rows follow each other
+                const int rr = mt * tpt * a.grp + r;
+                float* rec = A.part + ((size_t)blockIdx.x * 2 + (w.u0 == 0 ? 1 : 0)) * (256 * (HD + 2));
+                if (row_ok) {
+#pragma unroll
+                    for (int c = 0; c < HD; c += 4)
+                        *reinterpret_cast<float4*>(rec + rr * HD + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+                    rec[256 * HD + rr] = m;
+                    rec[256 * HD + 256 + rr] = l;
+                }
+                if (w.u0 == 0 && tid == 0) {
+                    const long long tile_end = w.at - w.n_it + w.nu;
+                    A.meta[blockIdx.x] = make_int4((int)((tile_end - 1) / share) - blockIdx.x, w.seq, w.kvh, w.pair);
+                }
+            }
+        }
+    } else {
+        EB_REGS_LESS();
+        if (warp == 8) {
+        // ---------------------------------------------------------------- k and v tiles
+        uint32_t n = 0, n_valid = 0;
+        const int n_box = UNIT / box;
+        while (ok && w.next()) {
+            for (int i = 0; i < w.n_it && ok; i++) {
+                const int p = w.pr.unit(w.u0 + i) * UNIT + lane * box;
+                int id = a.n_pages;  // outside the pool: the box is filled with zeros
+                bool good = lane < n_box;
+                if (good && p <= w.pr.lim_max && (p + box - 1 >= w.pr.low_min || p < A.n_sink)) {
+                    id = a.table[(size_t)w.seq * a.table_ld + p / a.page];
+                    if ((unsigned)id >= (unsigned)a.n_pages) {
+                        paged_flag(a.status);
+                        id = a.n_pages;
+                        good = false;
+                    }
+                }
+                const uint32_t valid = __ballot_sync(0xffffffffu, good);
+                if (lane == 0) B.valid[n_valid % VALID_RING] = valid;
+                n_valid++;
+#pragma unroll 1
+                for (int kv = 0; kv < 2 && ok; kv++, n++) {
+                    const uint32_t st = n % C::NST, use = n / C::NST;
+                    if (use > 0) ok = mbar_wait_bounded(&B.kv_empty[st], (use - 1) & 1);
+                    if (!ok) break;
+                    if (lane == 0) mbar_expect_tx(&B.kv_full[st], C::TILE);
+                    __syncwarp();
+                    if (lane < n_box) {
+#pragma unroll
+                        for (int h = 0; h < C::HALVES; h++)
+                            tma_box(kv ? &vmap : &kmap, skv + st * C::TILE + h * C::BLK + lane * box * 128, &B.kv_full[st], 64 * h,
+                                    p % a.page, w.kvh, id);
+                    }
+                }
+            }
+        }
+        // copies in flight land before the block ends
+        for (uint32_t k = n > (uint32_t)C::NST ? n - C::NST : 0; k < n; k++) mbar_wait_bounded(&B.kv_full[k % C::NST], (k / C::NST) & 1);
+        } else if (warp == 9) {
+        // ---------------------------------------------------------------- products
+        constexpr uint32_t ID_S = tc_idesc_f16(128, UNIT), ID_O = tc_idesc_f16(128, HD) | (1u << 16);
+        uint32_t n = 0, n_q[2] = {0, 0}, n_s[2] = {0, 0}, n_p[2] = {0, 0}, n_pv[2] = {0, 0};
+        const uint32_t q_addr = smem_u32(sq_), kv_addr = smem_u32(skv);
+        auto scores = [&](int mt, uint32_t st) {  // S of row tile mt from the k tile in st: the low parts first
+            if (lane == 0) {
+                const uint32_t qd = desc_lo(q_addr + mt * 2 * C::TILE, 0), kd = desc_lo(kv_addr + st * C::TILE, 0);
+                const uint32_t d = tmem + C::S_COL + mt * UNIT;
+#pragma unroll
+                for (int part = 0; part < 2; part++)
+#pragma unroll
+                    for (int k = 0; k < HD / 16; k++) {
+                        const uint32_t off = ((k >> 2) * C::BLK + (k & 3) * 32) >> 4;
+                        mma_smem_a(d, qd + ((part * C::TILE) >> 4) + off, kd + off, ID_S, part | k);
+                    }
+                tc_commit(&B.s_full[mt]);
+                mbar_arrive(&B.s_full[mt]);
+            }
+            n_s[mt]++;
+            __syncwarp();
+        };
+        auto values = [&](int mt, uint32_t st) {
+            if (lane == 0) {
+                const uint32_t vd = desc_lo(kv_addr + st * C::TILE, C::BLK), p = tmem + C::S_COL + mt * UNIT;
+#pragma unroll
+                for (int part = 0; part < 2; part++)  // low parts first
+#pragma unroll
+                    for (int k = 0; k < UNIT / 16; k++)
+                        mma_tmem_a(tmem + C::O_COL + mt * 128, p + 32 * (k >> 1) + (part ? 0 : 16) + 8 * (k & 1),
+                                   vd + ((k * 2048) >> 4), ID_O, part | k);
+                tc_commit(&B.pv_done[mt]);
+            }
+            __syncwarp();
+        };
+        auto release = [&](uint32_t st) {
+            if (lane == 0) tc_commit(&B.kv_empty[st]);
+            __syncwarp();
+        };
+        while (ok && w.next()) {
+            const int n_m = w.pr.t0 + tpt < w.pr.t1 ? 2 : 1;
+            for (int mt = 0; mt < n_m && ok; mt++) ok = mbar_wait_bounded(&B.q_full[mt], n_q[mt]++ & 1);
+            if (ok) ok = mbar_wait_bounded(&B.kv_full[n % C::NST], (n / C::NST) & 1);
+            if (!ok) break;
+            tc_fence_after();
+            for (int mt = 0; mt < n_m; mt++) scores(mt, n % C::NST);
+            release(n % C::NST);
+            n++;
+            for (int i = 0; i < w.n_it && ok; i++) {
+                const uint32_t nv = n, nk = n + 1;
+                const bool more = i + 1 < w.n_it;
+                ok = mbar_wait_bounded(&B.kv_full[nv % C::NST], (nv / C::NST) & 1);
+                if (!ok) break;
+                const int p0 = w.pr.unit(w.u0 + i) * UNIT;
+                if (p0 + UNIT - 1 > w.pr.lim_max || (p0 < w.pr.low_min && p0 + UNIT > A.n_sink)) {
+                    // positions that no row sees may hold anything: their v rows become zero, as their p are
+                    uint8_t* vt = skv + (nv % C::NST) * C::TILE;
+                    for (int j = lane; j < UNIT; j += 32) {
+                        const int p = p0 + j;
+                        if (p <= w.pr.lim_max && (p >= w.pr.low_min || p < A.n_sink)) continue;
+                        for (int h = 0; h < C::HALVES; h++)
+#pragma unroll
+                            for (int c = 0; c < 8; c++)
+                                *reinterpret_cast<uint4*>(vt + h * C::BLK + j * 128 + 16 * c) = make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                for (int mt = 0; mt < n_m && ok; mt++) {
+                    ok = mbar_wait_bounded(&B.p_full[mt], n_p[mt]++ & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    values(mt, nv % C::NST);
+                    if (mt == n_m - 1) release(nv % C::NST);
+                    if (more) {  // the next scores overwrite p: not before its product is done
+                        if (mt == 0) ok = mbar_wait_bounded(&B.kv_full[nk % C::NST], (nk / C::NST) & 1);
+                        if (ok) ok = mbar_wait_bounded(&B.pv_done[mt], n_pv[mt] & 1);
+                        if (!ok) break;
+                        scores(mt, nk % C::NST);
+                        if (mt == n_m - 1) release(nk % C::NST);
+                    }
+                    n_pv[mt]++;
+                }
+                n += more ? 2 : 1;
+            }
+        }
+        // whatever was issued is done before the tensor memory goes back
+        for (int mt = 0; mt < 2; mt++) {
+            if (n_s[mt]) mbar_wait_bounded(&B.s_full[mt], (n_s[mt] - 1) & 1);
+            if (n_pv[mt]) mbar_wait_bounded(&B.pv_done[mt], (n_pv[mt] - 1) & 1);
+        }
+        }
+    }
+    if (!ok && lane == 0 && a.status) atomicOr(a.status, (int)ST_WAIT_TIMEOUT);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) tc_dealloc(tmem, C::COLS);
+}
+
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encoder() {
+    static EncodeFn fn = []() -> EncodeFn {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+// A layer's pool as [page][kv head][position][hd]; a box: 64 elements (128 bytes, swizzled) of `box` positions.
+bool pool_map(CUtensorMap* m, const PagedArgs& a, const void* base, int hd, int box) {
+    const EncodeFn fn = encoder();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)a.page, (cuuint64_t)a.n_kv, (cuuint64_t)a.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)hd * 2, (cuuint64_t)a.page * hd * 2, (cuuint64_t)a.page_stride * 2};
+    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, steps[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), dims, strides, boxes, steps,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HD>
+cudaError_t tc_go(const PagedAttnArgs& A, cudaStream_t st) {
+    int box = UNIT;
+    while (A.c.page % box) box /= 2;  // gcd(page, 128): at least 16
+    CUtensorMap km, vm;
+    if (!pool_map(&km, A.c, A.c.k, HD, box) || !pool_map(&vm, A.c, A.c.v, HD, box)) return cudaErrorInvalidValue;
+    cudaFuncAttributes at;
+    cudaError_t e = cudaFuncGetAttributes(&at, k_paged_attn_tc<HD>);
+    if (e != cudaSuccess || at.numRegs != REGS_LAUNCH) return e != cudaSuccess ? e : cudaErrorInvalidConfiguration;
+    e = smem_limit<Tc<HD>>(k_paged_attn_tc<HD>, Tc<HD>::SMEM);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(k_paged_attn_tc<HD>, dim3(A.grid), dim3(TC_NT), Tc<HD>::SMEM, st, A, km, vm, box);
+}
+}  // namespace
+
+int paged_tc_grid() { return sm_count(); }
+cudaError_t launch_paged_attn_tc(int hd, const PagedAttnArgs& A, cudaStream_t st) {
+    return hd == 128 ? tc_go<128>(A, st) : tc_go<64>(A, st);
+}
+
+}  // namespace eb

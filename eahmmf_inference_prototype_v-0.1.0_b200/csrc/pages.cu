@@ -89,7 +89,7 @@ extern "C" int eahmmf_cuda_rope_append(const EahmmfPagedKv* kv, int layer, const
 extern "C" size_t eahmmf_cuda_paged_attention_workspace_bytes(const EahmmfPagedKv* kv, const EahmmfPagedSeqs* seqs,
                                                               int n_head) {
     if (check_kv(kv) != ST_OK || check_seqs(seqs) != ST_OK || !heads_ok(kv, n_head)) return 0;
-    return paged_attn_ws_bytes(kv->hd);
+    return paged_attn_ws_bytes(kv->type, kv->hd, n_head / kv->n_kv, seqs->max_q);
 }
 
 extern "C" int eahmmf_cuda_paged_attention(const EahmmfPagedKv* kv, int layer, const EahmmfPagedSeqs* seqs, int n_head,
