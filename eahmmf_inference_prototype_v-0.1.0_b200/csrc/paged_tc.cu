@@ -29,10 +29,10 @@ namespace {
 
 constexpr int TC_NT = 384;
 // Registers: 384 threads are launched with 168 each; a softmax thread holds its row's hd sums beside its scores. Shares
-// after the split: 2 x 128 x 224 + 128 x 56 = 384 x 168, the launch's own total (checked before the launch).
+// after the split: 2 x 128 x 208 + 128 x 88 = 384 x 168, the launch's own total (checked before the launch).
 constexpr int REGS_LAUNCH = 168;
-#define EB_REGS_MORE() asm volatile("setmaxnreg.inc.sync.aligned.u32 224;")
-#define EB_REGS_LESS() asm volatile("setmaxnreg.dec.sync.aligned.u32 56;")
+#define EB_REGS_MORE() asm volatile("setmaxnreg.inc.sync.aligned.u32 208;")
+#define EB_REGS_LESS() asm volatile("setmaxnreg.dec.sync.aligned.u32 88;")
 constexpr int UNIT = 128;  // positions of a unit
 constexpr int MROWS = 128;
 constexpr int VALID_RING = 8;
@@ -45,11 +45,11 @@ struct Tc {
     static constexpr int NST = HD == 128 ? 3 : 8;        // tiles of k and v in flight
     static constexpr int Q_BYTES = 2 * 2 * TILE;         // two row tiles, two parts
     static constexpr int SMEM = 1024 + Q_BYTES + NST * TILE + 512;
-    static constexpr uint32_t S_COL = 0, O_COL = 256;    // tensor memory: S0 S1 O0 O1
+    static constexpr uint32_t O_COL = 384;               // tensor memory: three S, one O
     static constexpr uint32_t COLS = 512;
 };
 struct Bars {
-    uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2], pv_done[2];
+    uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2], pv_done[2], o_free;
     uint32_t valid[VALID_RING];  // by unit: which boxes lie in pages of the pool
     uint32_t tmem;
     int seq;
@@ -57,6 +57,25 @@ struct Bars {
 };
 static_assert(sizeof(Bars) <= 512, "");
 
+// Bounded wait, as mbar_wait_bounded, without its suspend hint: these waits last a few hundred cycles.
+__device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity) {
+    for (int i = 0; i < 64; i++)
+        if (bar_try(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (;;) {
+        if (bar_try(bar, parity)) return true;
+        if (globaltimer_ns() - t0 > WAIT_LIMIT_NS) return false;
+    }
+}
 // Shared-memory matrix descriptors, 128-byte swizzle: rows of 128 bytes, groups of 8 rows 1024 bytes apart; lbo: distance of
 // the 64-element blocks of a transposed operand. The high word is the same for every operand, so that a product costs
 // one 32-bit addition for each descriptor.
@@ -96,6 +115,24 @@ __device__ __forceinline__ void tm_ld32(uint32_t addr, uint32_t (&r)[32]) {
                  : "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
                    "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]));
 }
+// 64 columns, both loads in flight together
+__device__ __forceinline__ void tm_ld64(uint32_t addr, uint32_t (&r)[64]) {
+#define EB_LD32(o)                                                                                                            \
+    asm volatile(                                                                                                             \
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"  \
+        "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"                                                                \
+        : EB_R16(r, o), EB_R16(r, o + 16)                                                                                     \
+        : "r"(addr + o))
+    EB_LD32(0);
+    EB_LD32(32);
+#undef EB_LD32
+#define EB_RW8(o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), "+r"(r[o + 6]), "+r"(r[o + 7])
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : EB_RW8(0), EB_RW8(8)::"memory");
+    asm volatile("" : EB_RW8(16), EB_RW8(24));
+    asm volatile("" : EB_RW8(32), EB_RW8(40));
+    asm volatile("" : EB_RW8(48), EB_RW8(56));
+#undef EB_RW8
+}
 __device__ __forceinline__ void tm_st32(uint32_t addr, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
@@ -111,6 +148,35 @@ __device__ __forceinline__ void tma_box(const CUtensorMap* map, void* dst, uint6
         "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(row), "r"(head), "r"(page)
         : "memory");
 }
+
+__device__ __forceinline__ float ex2(float v) {  // 2 units of 32 bits; results below 2^-126 are zero, as weights of them may be
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// two 32-bit operations in one instruction
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void un2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ bool elect() {  // one lane of a converged warp
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(p));
+    return p != 0;
+}
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
 
 // The walk of a block through its share: work in (sequence, pair of row tiles, kv head, unit) order.
 struct Pair {
@@ -196,6 +262,7 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
             mbar_init(&B.p_full[m], MROWS);
             mbar_init(&B.pv_done[m], 1);
         }
+        mbar_init(&B.o_free, MROWS);
         mbar_fence_init();
     }
     if (warp == 8) tc_alloc(&B.tmem, C::COLS);
@@ -263,158 +330,199 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
         uint8_t* q_lo = sq_ + mt * 2 * C::TILE;
         uint8_t* q_hi = q_lo + C::TILE;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t s_tm = tmem + lanes + C::S_COL + mt * UNIT, o_tm = tmem + lanes + C::O_COL + mt * 128;
-        uint32_t n_s = 0, n_pv = 0, n_valid = 0;  // uses of the barriers so far
+        const uint32_t o_tm = tmem + lanes + C::O_COL;
+        const int n_box = UNIT / box;
+        uint32_t n_s = 0, n_pv = 0, n_valid = 0, n_buf = 0;  // uses of the barriers, units and score buffers so far
         while (ok && w.next()) {
             const int tok = w.pr.t0 + mt * tpt + r / a.grp;
-            if (w.pr.t0 + mt * tpt >= w.pr.t1) {  // the pair has one row tile
+            const int n_m = w.pr.t0 + tpt < w.pr.t1 ? 2 : 1;
+            if (mt >= n_m) {  // the pair has one row tile
                 n_valid += w.n_it;
+                n_buf += w.n_it;
                 continue;
             }
             const bool row_ok = r < tpt * a.grp && tok < w.pr.t1;
             const int head = w.kvh * a.grp + r % a.grp;
             const int lim = row_ok ? w.sq.kv - w.sq.q + tok : -1;
             const int low = A.window > 0 ? lim - A.window + 1 : 0;
-            // ---- q row: a power of two that brings its largest to [2^8, 2^9), then its two parts
+            // ---- q: a warp's rows scaled by the power of two that brings their largest to [2^14, 2^15), then split. The low
+            // parts are exact to 2^-25 of that, 2^-39 of the largest row: in a score an absolute error of 2^-39 of the
+            // warp's largest, far below that of 32 bits. Rows come one (hd 128) or two (hd 64) to a load instruction.
             float cs;
             {
-                const float4* qr = reinterpret_cast<const float4*>(A.q + (size_t)(w.sq.q0 + (row_ok ? tok : w.pr.t0)) * A.ldq +
-                                                                   (size_t)head * HD);
+                constexpr int LPR = HD / 4, RPP = 32 / LPR;
+                const int el = lane % LPR, sub = lane / LPR;
+                const float* mine = A.q + (size_t)(w.sq.q0 + (row_ok ? tok : w.pr.t0)) * A.ldq + (size_t)head * HD;  // lane = row
+                const uint32_t rows_ok = __ballot_sync(0xffffffffu, row_ok);
+                auto load = [&](int row, float4& f) {
+                    const float* src =
+                        reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(mine), row + sub));
+                    asm volatile("ld.global.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "l"(src + 4 * el));
+                };
                 float mx = 0.f;
-#pragma unroll 8
-                for (int c = 0; c < HD / 4; c++) {
-                    const float4 f = qr[c];
-                    mx = fmaxf(fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y))), fmaxf(fabsf(f.z), fabsf(f.w)));
-                }
-                const int ex = (int)((__float_as_uint(mx) >> 23) & 255) - 127;
-                float sc = ex < 128 && mx > 0.f ? pow2f(min(max(8 - ex, -100), 100)) : 1.f;
-                cs = fabsf(A.scale) * 1.4426950408889634f / sc;
-                if (A.scale < 0.f) sc = -sc;  // the running maximum is that of +c S
-                if (!row_ok) sc = 0.f;
-#pragma unroll 4
-                for (int c = 0; c < HD / 8; c++) {
-                    const float4 f0 = qr[2 * c], f1 = qr[2 * c + 1];
-                    const float x[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
-                    uint32_t hi[4], lo[4];
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32; i0 += 16) {
+                    float4 f[16 / RPP];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float u = row_ok ? x[2 * i] * sc : 0.f, v = row_ok ? x[2 * i + 1] * sc : 0.f;
-                        const __half2 h = __floats2half2_rn(u, v);
-                        const float2 b = __half22float2(h);
-                        const __half2 l2 = __floats2half2_rn(u - b.x, v - b.y);
-                        hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-                        lo[i] = *reinterpret_cast<const uint32_t*>(&l2);
+                    for (int i = 0; i < 16 / RPP; i++) load(i0 + i * RPP, f[i]);
+#pragma unroll
+                    for (int i = 0; i < 16 / RPP; i++) {
+                        const float v = fmaxf(fmaxf(fabsf(f[i].x), fabsf(f[i].y)), fmaxf(fabsf(f[i].z), fabsf(f[i].w)));
+                        if (v < INFINITY) mx = fmaxf(mx, v);  // a row that is not finite does not disturb the others
                     }
-                    const int at = (c >> 3) * C::BLK + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-                    *reinterpret_cast<uint4*>(q_hi + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                    *reinterpret_cast<uint4*>(q_lo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                const int ex = (int)((__float_as_uint(mx) >> 23) & 255) - 127;
+                float sc = mx > 0.f ? pow2f(min(max(14 - ex, -100), 100)) : 1.f;
+                cs = fmaxf(fabsf(A.scale) * 1.4426950408889634f / sc, 1e-37f);  // never zero: c times -infinity
+                if (A.scale <= 0.f) sc = A.scale < 0.f ? -sc : 0.f;             // the running maximum is that of +c S
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32; i0 += 8) {
+                    float4 f[8 / RPP];
+#pragma unroll
+                    for (int i = 0; i < 8 / RPP; i++) load(i0 + i * RPP, f[i]);
+#pragma unroll
+                    for (int i = 0; i < 8 / RPP; i++) {
+                        const int ro = i0 + i * RPP + sub, row = 32 * (warp & 3) + ro;
+                        if (!((rows_ok >> ro) & 1)) f[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        const __half2 h0 = __floats2half2_rn(f[i].x * sc, f[i].y * sc), h1 = __floats2half2_rn(f[i].z * sc, f[i].w * sc);
+                        const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+                        const __half2 l0 = __floats2half2_rn(f[i].x * sc - b0.x, f[i].y * sc - b0.y),
+                                      l1 = __floats2half2_rn(f[i].z * sc - b1.x, f[i].w * sc - b1.y);
+                        const int ch = el >> 1;  // 16-byte chunk
+                        const int at = (ch >> 3) * C::BLK + row * 128 + (((ch & 7) ^ (row & 7)) << 4) + (el & 1) * 8;
+                        *reinterpret_cast<uint2*>(q_hi + at) =
+                            make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+                        *reinterpret_cast<uint2*>(q_lo + at) =
+                            make_uint2(*reinterpret_cast<const uint32_t*>(&l0), *reinterpret_cast<const uint32_t*>(&l1));
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(&B.q_full[mt]);
             }
-            float acc[HD];
+            uint64_t acc[HD / 2];
 #pragma unroll
-            for (int c = 0; c < HD; c++) acc[c] = 0.f;
+            for (int c = 0; c < HD / 2; c++) acc[c] = 0;
             float m = -INFINITY, l = 0.f, alpha = 1.f;
-            auto add_o = [&]() {  // acc <- acc alpha + O of the unit before
-#pragma unroll
-                for (int c = 0; c < HD; c += 32) {
-                    uint32_t o[32];
-                    tm_ld32(o_tm + c, o);
-#pragma unroll
-                    for (int j = 0; j < 32; j++) acc[c + j] = fmaf(acc[c + j], alpha, __uint_as_float(o[j]));
-                }
-            };
-            for (int i = 0; i < w.n_it; i++, n_valid++) {
-                if (i > 0) {
-                    ok = mbar_wait_bounded(&B.pv_done[mt], n_pv++ & 1);
+            n_buf += mt;
+#pragma unroll 1
+            for (int i = 0;; i++) {
+                if (i > 0) {  // acc <- acc alpha + O of the unit before
+                    ok = bar_wait(&B.pv_done[mt], n_pv++ & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    add_o();
+                    const uint64_t al = f2(alpha, alpha);
+#pragma unroll
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tm_ld32(o_tm + c, o);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2)
+                            acc[(c + j) / 2] = fma2(acc[(c + j) / 2], al, f2(__uint_as_float(o[j]), __uint_as_float(o[j + 1])));
+                    }
+                    tc_fence_before();
+                    mbar_arrive(&B.o_free);
                 }
-                ok = mbar_wait_bounded(&B.s_full[mt], n_s++ & 1);
+                if (i == w.n_it) break;
+                const int p0 = w.pr.unit(w.u0 + i) * UNIT;
+                ok = bar_wait(&B.s_full[mt], n_s++ & 1);
                 if (!ok) break;
                 tc_fence_after();
-                const int p0 = w.pr.unit(w.u0 + i) * UNIT;
-                const uint32_t valid = B.valid[n_valid % VALID_RING];
-                const int n_box = UNIT / box;
+                const uint32_t s_tm = tmem + lanes + (n_buf % 3) * UNIT, valid = B.valid[n_valid % VALID_RING];
+                n_valid++;
+                n_buf += n_m;
                 const bool all = p0 + UNIT - 1 <= lim && (p0 >= low || p0 + UNIT <= A.n_sink) && valid == (1u << n_box) - 1;
-                float mx = -INFINITY;
-                auto see = [&](int j) {
-                    const int p = p0 + j;
-                    return p <= lim && (p >= low || p < A.n_sink) && ((valid >> (j / box)) & 1);
-                };
-                const bool plain = __all_sync(0xffffffffu, all);
+                if (!__all_sync(0xffffffffu, all)) {  // hidden positions' scores become -infinity
+#pragma unroll 1
+                    for (int c = 0; c < UNIT; c += 32) {
+                        const int p = p0 + c;
+                        uint32_t ok32 = 0;
+                        if (box >= 32)
+                            ok32 = (valid >> (c / box)) & 1 ? 0xffffffffu : 0u;
+                        else
+                            ok32 = ((valid >> (c / 16)) & 1 ? 0xffffu : 0u) | ((valid >> (c / 16 + 1)) & 1 ? 0xffff0000u : 0u);
+                        ok32 &= low_bits(lim - p + 1) & (~low_bits(low - p) | low_bits(A.n_sink - p));
+                        uint32_t s[32];
+                        tm_ld32(s_tm + c, s);
 #pragma unroll
-                for (int c = 0; c < UNIT; c += 32) {
-                    uint32_t s[32];
-                    tm_ld32(s_tm + c, s);
-                    if (plain) {
-#pragma unroll
-                        for (int j = 0; j < 32; j++) mx = fmaxf(mx, __uint_as_float(s[j]));
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 32; j++) mx = see(c + j) ? fmaxf(mx, __uint_as_float(s[j])) : mx;
+                        for (int j = 0; j < 32; j++)
+                            if (!((ok32 >> j) & 1)) s[j] = 0xff800000u;
+                        tm_st32(s_tm + c, s);
                     }
+                    tm_wait_st();
+                }
+                float mx = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < UNIT; c += 64) {
+                    uint32_t s[64];
+                    tm_ld64(s_tm + c, s);
+                    float m2 = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < 64; j += 4) {
+                        mx = fmaxf(mx, fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
+                        m2 = fmaxf(m2, fmaxf(__uint_as_float(s[j + 2]), __uint_as_float(s[j + 3])));
+                    }
+                    mx = fmaxf(mx, m2);
                 }
                 const float mn = mx == -INFINITY ? m : fmaxf(m, mx * cs);
-                alpha = mn == -INFINITY ? 1.f : exp2f(m - mn);
+                alpha = mn == -INFINITY ? 1.f : ex2(m - mn);
                 m = mn;
                 const float mo = mn == -INFINITY ? 0.f : mn - 15.f;
-                float ls = 0.f;
-#pragma unroll
+                const uint64_t cs2 = f2(cs, cs), mo2 = f2(-mo, -mo);
+                uint64_t ls2 = 0;
+#pragma unroll 1
                 for (int c = 0; c < UNIT; c += 32) {
-                    uint32_t s[32];
+                    uint32_t s[32], out[32];
                     tm_ld32(s_tm + c, s);
-                    uint32_t out[32];
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
-                        float u = exp2f(fmaf(__uint_as_float(s[j]), cs, -mo)), v = exp2f(fmaf(__uint_as_float(s[j + 1]), cs, -mo));
-                        if (!plain) {
-                            u = see(c + j) ? u : 0.f;
-                            v = see(c + j + 1) ? v : 0.f;
-                        }
-                        ls += u + v;
+                        float u, v, d0, d1;
+                        un2(fma2(f2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), cs2, mo2), u, v);
+                        u = ex2(u);
+                        v = ex2(v);
+                        const uint64_t uv = f2(u, v);
+                        ls2 = add2(ls2, uv);
                         const __half2 h = __floats2half2_rn(u, v);
                         const float2 b = __half22float2(h);
-                        const __half2 l2 = __floats2half2_rn(u - b.x, v - b.y);
+                        un2(add2(uv, f2(-b.x, -b.y)), d0, d1);
+                        const __half2 l2 = __floats2half2_rn(d0, d1);
                         out[j / 2] = *reinterpret_cast<const uint32_t*>(&h);
                         out[16 + j / 2] = *reinterpret_cast<const uint32_t*>(&l2);
                     }
                     tm_st32(s_tm + c, out);
                 }
-                l = fmaf(l, alpha, ls);
+                float ls, ls_b;
+                un2(ls2, ls, ls_b);
+                l = fmaf(l, alpha, ls + ls_b);
                 tm_wait_st();
                 tc_fence_before();
                 mbar_arrive(&B.p_full[mt]);
             }
-            if (ok) ok = mbar_wait_bounded(&B.pv_done[mt], n_pv++ & 1);
+            n_buf -= mt;
             if (!ok) break;
-            tc_fence_after();
-            add_o();
-            tc_fence_before();
             const bool whole = w.u0 == 0 && w.n_it == w.nu;
-            if (whole) {
-                if (row_ok) {
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-                    float4* o = reinterpret_cast<float4*>(A.out + (size_t)(w.sq.q0 + tok) * A.ldo + (size_t)head * HD);
-#pragma unroll
-                    for (int c = 0; c < HD; c += 4)
-                        o[c / 4] = make_float4(acc[c] * inv, acc[c + 1] * inv, acc[c + 2] * inv, acc[c + 3] * inv);
-                }
-            } else {  // records hold rows in (token, head) order: the two tiles' rows follow each other
+            if (!whole && w.u0 == 0 && tid == 0) {
+                const long long tile_end = w.at - w.n_it + w.nu;
+                A.meta[blockIdx.x] = make_int4((int)((tile_end - 1) / share) - blockIdx.x, w.seq, w.kvh, w.pair);
+            }
+            if (row_ok) {
+                // the output row, or the row of this block's record (rows in (token, head) order: the tiles' follow each other)
                 const int rr = mt * tpt * a.grp + r;
                 float* rec = A.part + ((size_t)blockIdx.x * 2 + (w.u0 == 0 ? 1 : 0)) * (256 * (HD + 2));
-                if (row_ok) {
+                float* o = whole ? A.out + (size_t)(w.sq.q0 + tok) * A.ldo + (size_t)head * HD : rec + (size_t)rr * HD;
+                const float f = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+                const uint64_t ff = f2(f, f);
 #pragma unroll
-                    for (int c = 0; c < HD; c += 4)
-                        *reinterpret_cast<float4*>(rec + rr * HD + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
+                for (int c = 0; c < HD; c += 4) {
+                    float4 v;
+                    un2(fma2(acc[c / 2], ff, 0), v.x, v.y);
+                    un2(fma2(acc[c / 2 + 1], ff, 0), v.z, v.w);
+                    *reinterpret_cast<float4*>(o + c) = v;
+                }
+                if (!whole) {
                     rec[256 * HD + rr] = m;
                     rec[256 * HD + 256 + rr] = l;
-                }
-                if (w.u0 == 0 && tid == 0) {
-                    const long long tile_end = w.at - w.n_it + w.nu;
-                    A.meta[blockIdx.x] = make_int4((int)((tile_end - 1) / share) - blockIdx.x, w.seq, w.kvh, w.pair);
                 }
             }
         }
@@ -443,7 +551,7 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
 #pragma unroll 1
                 for (int kv = 0; kv < 2 && ok; kv++, n++) {
                     const uint32_t st = n % C::NST, use = n / C::NST;
-                    if (use > 0) ok = mbar_wait_bounded(&B.kv_empty[st], (use - 1) & 1);
+                    if (use > 0) ok = bar_wait(&B.kv_empty[st], (use - 1) & 1);
                     if (!ok) break;
                     if (lane == 0) mbar_expect_tx(&B.kv_full[st], C::TILE);
                     __syncwarp();
@@ -457,16 +565,21 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
             }
         }
         // copies in flight land before the block ends
-        for (uint32_t k = n > (uint32_t)C::NST ? n - C::NST : 0; k < n; k++) mbar_wait_bounded(&B.kv_full[k % C::NST], (k / C::NST) & 1);
+        for (uint32_t k = n > (uint32_t)C::NST ? n - C::NST : 0; k < n; k++) bar_wait(&B.kv_full[k % C::NST], (k / C::NST) & 1);
         } else if (warp == 9) {
         // ---------------------------------------------------------------- products
+        // Order: S0 S1 | O0 S0' O1 S1' | O0' S0'' ...: while one tile's scores are in the softmax the other's two products
+        // run. Scores rotate through three buffers, so that new ones never wait for the product that reads the last p of
+        // their tile; the one that read their buffer came two products earlier. O is one buffer, read by its softmax
+        // warps while the product after it runs.
         constexpr uint32_t ID_S = tc_idesc_f16(128, UNIT), ID_O = tc_idesc_f16(128, HD) | (1u << 16);
-        uint32_t n = 0, n_q[2] = {0, 0}, n_s[2] = {0, 0}, n_p[2] = {0, 0}, n_pv[2] = {0, 0};
-        const uint32_t q_addr = smem_u32(sq_), kv_addr = smem_u32(skv);
+        uint32_t n = 0, n_q0 = 0, n_q1 = 0, n_p0 = 0, n_p1 = 0, n_s0 = 0, n_s1 = 0, n_pv0 = 0, n_pv1 = 0, n_o = 0, n_buf = 0;
+        const uint32_t q_addr = __shfl_sync(0xffffffffu, smem_u32(sq_), 0), kv_addr = __shfl_sync(0xffffffffu, smem_u32(skv), 0);
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
         auto scores = [&](int mt, uint32_t st) {  // S of row tile mt from the k tile in st: the low parts first
-            if (lane == 0) {
-                const uint32_t qd = desc_lo(q_addr + mt * 2 * C::TILE, 0), kd = desc_lo(kv_addr + st * C::TILE, 0);
-                const uint32_t d = tmem + C::S_COL + mt * UNIT;
+            const uint32_t d = tm + (n_buf % 3) * UNIT;
+            const uint32_t qd = desc_lo(q_addr + mt * 2 * C::TILE, 0), kd = desc_lo(kv_addr + st * C::TILE, 0);
+            if (elect()) {
 #pragma unroll
                 for (int part = 0; part < 2; part++)
 #pragma unroll
@@ -477,78 +590,92 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
                 tc_commit(&B.s_full[mt]);
                 mbar_arrive(&B.s_full[mt]);
             }
-            n_s[mt]++;
             __syncwarp();
+            n_buf++;
+            (mt ? n_s1 : n_s0)++;
         };
-        auto values = [&](int mt, uint32_t st) {
-            if (lane == 0) {
-                const uint32_t vd = desc_lo(kv_addr + st * C::TILE, C::BLK), p = tmem + C::S_COL + mt * UNIT;
+        auto values = [&](int mt, uint32_t st, uint32_t buf) {
+            const uint32_t vd = desc_lo(kv_addr + st * C::TILE, C::BLK), p = tm + (buf % 3) * UNIT;
+            if (elect()) {
 #pragma unroll
                 for (int part = 0; part < 2; part++)  // low parts first
 #pragma unroll
                     for (int k = 0; k < UNIT / 16; k++)
-                        mma_tmem_a(tmem + C::O_COL + mt * 128, p + 32 * (k >> 1) + (part ? 0 : 16) + 8 * (k & 1),
-                                   vd + ((k * 2048) >> 4), ID_O, part | k);
+                        mma_tmem_a(tm + C::O_COL, p + 32 * (k >> 1) + (part ? 0 : 16) + 8 * (k & 1), vd + ((k * 2048) >> 4), ID_O,
+                                   part | k);
                 tc_commit(&B.pv_done[mt]);
             }
             __syncwarp();
+            (mt ? n_pv1 : n_pv0)++;
         };
         auto release = [&](uint32_t st) {
-            if (lane == 0) tc_commit(&B.kv_empty[st]);
+            if (elect()) tc_commit(&B.kv_empty[st]);
             __syncwarp();
         };
+        auto read = [&](int mt) {  // the last product that read p of tile mt is done
+            const uint32_t k = mt ? n_pv1 : n_pv0;
+            return k == 0 || bar_wait(&B.pv_done[mt], (k - 1) & 1);
+        };
         while (ok && w.next()) {
-            const int n_m = w.pr.t0 + tpt < w.pr.t1 ? 2 : 1;
-            for (int mt = 0; mt < n_m && ok; mt++) ok = mbar_wait_bounded(&B.q_full[mt], n_q[mt]++ & 1);
-            if (ok) ok = mbar_wait_bounded(&B.kv_full[n % C::NST], (n / C::NST) & 1);
+            const bool two = w.pr.t0 + tpt < w.pr.t1;
+            ok = bar_wait(&B.q_full[0], n_q0++ & 1);
+            if (ok && two) ok = bar_wait(&B.q_full[1], n_q1++ & 1);
+            if (ok) ok = read(0) && read(1) && bar_wait(&B.kv_full[n % C::NST], (n / C::NST) & 1);
             if (!ok) break;
             tc_fence_after();
-            for (int mt = 0; mt < n_m; mt++) scores(mt, n % C::NST);
+            uint32_t buf = n_buf;  // of the next p
+#pragma unroll 1
+            for (int mt = 0; mt < (two ? 2 : 1); mt++) scores(mt, n % C::NST);
             release(n % C::NST);
             n++;
+#pragma unroll 1
             for (int i = 0; i < w.n_it && ok; i++) {
                 const uint32_t nv = n, nk = n + 1;
                 const bool more = i + 1 < w.n_it;
-                ok = mbar_wait_bounded(&B.kv_full[nv % C::NST], (nv / C::NST) & 1);
+                ok = bar_wait(&B.kv_full[nv % C::NST], (nv / C::NST) & 1);
                 if (!ok) break;
                 const int p0 = w.pr.unit(w.u0 + i) * UNIT;
                 if (p0 + UNIT - 1 > w.pr.lim_max || (p0 < w.pr.low_min && p0 + UNIT > A.n_sink)) {
                     // positions that no row sees may hold anything: their v rows become zero, as their p are
                     uint8_t* vt = skv + (nv % C::NST) * C::TILE;
-                    for (int j = lane; j < UNIT; j += 32) {
+#pragma unroll 4
+                    for (int j = lane >> 3; j < UNIT; j += 4) {  // 8 lanes a row
                         const int p = p0 + j;
                         if (p <= w.pr.lim_max && (p >= w.pr.low_min || p < A.n_sink)) continue;
-                        for (int h = 0; h < C::HALVES; h++)
 #pragma unroll
-                            for (int c = 0; c < 8; c++)
-                                *reinterpret_cast<uint4*>(vt + h * C::BLK + j * 128 + 16 * c) = make_uint4(0, 0, 0, 0);
+                        for (int h = 0; h < C::HALVES; h++)
+                            *reinterpret_cast<uint4*>(vt + h * C::BLK + j * 128 + 16 * (lane & 7)) = make_uint4(0, 0, 0, 0);
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
-                for (int mt = 0; mt < n_m && ok; mt++) {
-                    ok = mbar_wait_bounded(&B.p_full[mt], n_p[mt]++ & 1);
+#pragma unroll 1
+                for (int mt = 0; mt < (two ? 2 : 1); mt++) {
+                    ok = bar_wait(&B.p_full[mt], (mt ? n_p1++ : n_p0++) & 1);
+                    if (ok && n_o > 0) ok = bar_wait(&B.o_free, (n_o - 1) & 1);
                     if (!ok) break;
+                    n_o++;
                     tc_fence_after();
-                    values(mt, nv % C::NST);
-                    if (mt == n_m - 1) release(nv % C::NST);
-                    if (more) {  // the next scores overwrite p: not before its product is done
-                        if (mt == 0) ok = mbar_wait_bounded(&B.kv_full[nk % C::NST], (nk / C::NST) & 1);
-                        if (ok) ok = mbar_wait_bounded(&B.pv_done[mt], n_pv[mt] & 1);
+                    values(mt, nv % C::NST, buf++);
+                    const bool last = mt == 1 || !two;
+                    if (last) release(nv % C::NST);
+                    if (more) {
+                        if (mt == 0) ok = bar_wait(&B.kv_full[nk % C::NST], (nk / C::NST) & 1);
+                        if (ok && two) ok = read(1 - mt);
                         if (!ok) break;
+                        tc_fence_after();
                         scores(mt, nk % C::NST);
-                        if (mt == n_m - 1) release(nk % C::NST);
+                        if (last) release(nk % C::NST);
                     }
-                    n_pv[mt]++;
                 }
                 n += more ? 2 : 1;
             }
         }
         // whatever was issued is done before the tensor memory goes back
-        for (int mt = 0; mt < 2; mt++) {
-            if (n_s[mt]) mbar_wait_bounded(&B.s_full[mt], (n_s[mt] - 1) & 1);
-            if (n_pv[mt]) mbar_wait_bounded(&B.pv_done[mt], (n_pv[mt] - 1) & 1);
-        }
+        read(0);
+        read(1);
+        if (n_s0) bar_wait(&B.s_full[0], (n_s0 - 1) & 1);
+        if (n_s1) bar_wait(&B.s_full[1], (n_s1 - 1) & 1);
         }
     }
     if (!ok && lane == 0 && a.status) atomicOr(a.status, (int)ST_WAIT_TIMEOUT);
