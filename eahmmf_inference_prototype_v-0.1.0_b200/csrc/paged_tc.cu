@@ -14,8 +14,9 @@
 // Bound: 4 hd flops per row and position, twice because of the two parts: 2 * 2 * 2 * 128 * 128 * hd per tile and unit. Two
 // tiles share every k and v tile and take turns: while one tile's scores are in the softmax the other's products run.
 //
-// Warps: 0-3 softmax of tile 0, 4-7 of tile 1 (thread = row = tensor-memory lane), 8 loads, 9 issues the products,
-// 10 and 11 only give their registers to the softmax warps.
+// Warps: 0-3 softmax of tile 0, 4-7 of tile 1 (thread = row = tensor-memory lane), 8 loads, 9 issues q k, 10 issues p v
+// (one warp for both left the tensor cores idle a third of the time: each wait costs it some 150 cycles), 11 only gives its
+// registers to the softmax warps.
 #include <cuda.h>
 
 #include <mutex>
@@ -49,7 +50,7 @@ struct Tc {
     static constexpr uint32_t COLS = 512;
 };
 struct Bars {
-    uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2], pv_done[2], o_free;
+    uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2], pv_done[2], s_free[3], o_free;
     uint32_t valid[VALID_RING];  // by unit: which boxes lie in pages of the pool
     uint32_t tmem;
     int seq;
@@ -178,7 +179,9 @@ __device__ __forceinline__ bool elect() {  // one lane of a converged warp
 }
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
 
-// The walk of a block through its share: work in (sequence, pair of row tiles, kv head, unit) order.
+// The walk of a block through its share: work in (sequence, pair of row tiles, kv head, unit) order. Shares are even in
+// ticks: one for a unit and TILE_TICKS for a pair's q and output.
+constexpr int TILE_TICKS = 3;
 struct Pair {
     int t0, t1;                   // tokens of the pair
     int low_min, lim_max;         // positions that some row sees: [low_min, lim_max] and the first n_sink
@@ -222,18 +225,20 @@ struct Walk {
             }
             pr = pair_of(A, sq, pair, tpt);
             nu = pr.n();
-            const long long w = (long long)nu * A.c.n_kv;
+            const int ticks = nu + TILE_TICKS;
+            const long long w = (long long)ticks * A.c.n_kv;
             if (at >= base + w) {
                 base += w;
                 pair++;
                 continue;
             }
             const int idx = (int)(at - base);
-            kvh = idx / nu;
-            u0 = idx - kvh * nu;
-            n_it = (int)min((long long)(nu - u0), end - at);
-            at += n_it;
-            return true;
+            kvh = idx / ticks;
+            const int t0 = idx - kvh * ticks, t1 = (int)min((long long)ticks, t0 + (end - at));
+            at += t1 - t0;
+            u0 = max(0, t0 - TILE_TICKS);
+            n_it = max(0, t1 - TILE_TICKS) - u0;
+            if (n_it > 0) return true;  // else this block's share ends before the tile's first unit
         }
         return false;
     }
@@ -263,6 +268,7 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
             mbar_init(&B.pv_done[m], 1);
         }
         mbar_init(&B.o_free, MROWS);
+        for (int b = 0; b < 3; b++) mbar_init(&B.s_free[b], 1);
         mbar_fence_init();
     }
     if (warp == 8) tc_alloc(&B.tmem, C::COLS);
@@ -273,7 +279,7 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
         const Seq sq = paged_seq(a, s, flag);
         if (!tc_takes(A, sq)) return 0;
         long long n = 0;
-        for (int p = 0; p * 2 * tpt < sq.q; p++) n += pair_of(A, sq, p, tpt).n();
+        for (int p = 0; p * 2 * tpt < sq.q; p++) n += pair_of(A, sq, p, tpt).n() + TILE_TICKS;
         return n * a.n_kv;
     };
     long long total = 0, mine = 0;
@@ -503,28 +509,42 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
             if (!ok) break;
             const bool whole = w.u0 == 0 && w.n_it == w.nu;
             if (!whole && w.u0 == 0 && tid == 0) {
-                const long long tile_end = w.at - w.n_it + w.nu;
+                const long long tile_end = w.at + (w.nu - w.n_it);
                 A.meta[blockIdx.x] = make_int4((int)((tile_end - 1) / share) - blockIdx.x, w.seq, w.kvh, w.pair);
             }
-            if (row_ok) {
-                // the output row, or the row of this block's record (rows in (token, head) order: the tiles' follow each other)
-                const int rr = mt * tpt * a.grp + r;
-                float* rec = A.part + ((size_t)blockIdx.x * 2 + (w.u0 == 0 ? 1 : 0)) * (256 * (HD + 2));
-                float* o = whole ? A.out + (size_t)(w.sq.q0 + tok) * A.ldo + (size_t)head * HD : rec + (size_t)rr * HD;
-                const float f = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
-                const uint64_t ff = f2(f, f);
+            // ---- the warp's rows through shared memory (their q is read), so that a row leaves as one run: to the output, or to
+            // this block's record (rows in (token, head) order: the two tiles' rows follow each other)
+            const int rr = mt * tpt * a.grp + r;
+            float* rec = A.part + ((size_t)blockIdx.x * 2 + (w.u0 == 0 ? 1 : 0)) * (256 * (HD + 2));
+            float* dst = whole ? A.out + (size_t)(w.sq.q0 + (row_ok ? tok : w.pr.t0)) * A.ldo + (size_t)head * HD : rec + (size_t)rr * HD;
+            if (!whole && row_ok) {
+                rec[256 * HD + rr] = m;
+                rec[256 * HD + 256 + rr] = l;
+            }
+            const float f = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+            const uint64_t ff = f2(f, f);
+            float4* st = reinterpret_cast<float4*>(q_lo) + (size_t)32 * (warp & 3) * (HD / 4);  // [32 rows][hd / 4], chunks exchanged
 #pragma unroll
-                for (int c = 0; c < HD; c += 4) {
-                    float4 v;
-                    un2(fma2(acc[c / 2], ff, 0), v.x, v.y);
-                    un2(fma2(acc[c / 2 + 1], ff, 0), v.z, v.w);
-                    *reinterpret_cast<float4*>(o + c) = v;
-                }
-                if (!whole) {
-                    rec[256 * HD + rr] = m;
-                    rec[256 * HD + 256 + rr] = l;
+            for (int c = 0; c < HD / 4; c++) {
+                float4 v;
+                un2(fma2(acc[2 * c], ff, 0), v.x, v.y);
+                un2(fma2(acc[2 * c + 1], ff, 0), v.z, v.w);
+                st[lane * (HD / 4) + (c ^ (lane & 7))] = v;
+            }
+            __syncwarp();
+            {
+                constexpr int LPR = HD / 4, RPP = 32 / LPR;
+                const int el = lane % LPR, sub = lane / LPR;
+                const uint32_t rows_ok = __ballot_sync(0xffffffffu, row_ok);
+#pragma unroll 4
+                for (int i = 0; i < 32; i += RPP) {
+                    const int row = i + sub;
+                    float* d = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), row));
+                    const float4 v = st[row * (HD / 4) + (el ^ (row & 7))];
+                    if ((rows_ok >> row) & 1) *reinterpret_cast<float4*>(d + 4 * el) = v;
                 }
             }
+            __syncwarp();
         }
     } else {
         EB_REGS_LESS();
@@ -567,77 +587,65 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
         // copies in flight land before the block ends
         for (uint32_t k = n > (uint32_t)C::NST ? n - C::NST : 0; k < n; k++) bar_wait(&B.kv_full[k % C::NST], (k / C::NST) & 1);
         } else if (warp == 9) {
-        // ---------------------------------------------------------------- products
-        // Order: S0 S1 | O0 S0' O1 S1' | O0' S0'' ...: while one tile's scores are in the softmax the other's two products
-        // run. Scores rotate through three buffers, so that new ones never wait for the product that reads the last p of
-        // their tile; the one that read their buffer came two products earlier. O is one buffer, read by its softmax
-        // warps while the product after it runs.
-        constexpr uint32_t ID_S = tc_idesc_f16(128, UNIT), ID_O = tc_idesc_f16(128, HD) | (1u << 16);
-        uint32_t n = 0, n_q0 = 0, n_q1 = 0, n_p0 = 0, n_p1 = 0, n_s0 = 0, n_s1 = 0, n_pv0 = 0, n_pv1 = 0, n_o = 0, n_buf = 0;
+        // ---------------------------------------------------------------- products q k
+        // Scores rotate through three buffers, so that new ones wait for the product p v that read their buffer, two
+        // products before, and not for the last one of their own tile.
+        constexpr uint32_t ID_S = tc_idesc_f16(128, UNIT);
+        uint32_t n = 0, n_q0 = 0, n_q1 = 0, n_buf = 0;
         const uint32_t q_addr = __shfl_sync(0xffffffffu, smem_u32(sq_), 0), kv_addr = __shfl_sync(0xffffffffu, smem_u32(skv), 0);
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        auto scores = [&](int mt, uint32_t st) {  // S of row tile mt from the k tile in st: the low parts first
-            const uint32_t d = tm + (n_buf % 3) * UNIT;
-            const uint32_t qd = desc_lo(q_addr + mt * 2 * C::TILE, 0), kd = desc_lo(kv_addr + st * C::TILE, 0);
-            if (elect()) {
-#pragma unroll
-                for (int part = 0; part < 2; part++)
-#pragma unroll
-                    for (int k = 0; k < HD / 16; k++) {
-                        const uint32_t off = ((k >> 2) * C::BLK + (k & 3) * 32) >> 4;
-                        mma_smem_a(d, qd + ((part * C::TILE) >> 4) + off, kd + off, ID_S, part | k);
-                    }
-                tc_commit(&B.s_full[mt]);
-                mbar_arrive(&B.s_full[mt]);
-            }
-            __syncwarp();
-            n_buf++;
-            (mt ? n_s1 : n_s0)++;
-        };
-        auto values = [&](int mt, uint32_t st, uint32_t buf) {
-            const uint32_t vd = desc_lo(kv_addr + st * C::TILE, C::BLK), p = tm + (buf % 3) * UNIT;
-            if (elect()) {
-#pragma unroll
-                for (int part = 0; part < 2; part++)  // low parts first
-#pragma unroll
-                    for (int k = 0; k < UNIT / 16; k++)
-                        mma_tmem_a(tm + C::O_COL, p + 32 * (k >> 1) + (part ? 0 : 16) + 8 * (k & 1), vd + ((k * 2048) >> 4), ID_O,
-                                   part | k);
-                tc_commit(&B.pv_done[mt]);
-            }
-            __syncwarp();
-            (mt ? n_pv1 : n_pv0)++;
-        };
-        auto release = [&](uint32_t st) {
-            if (elect()) tc_commit(&B.kv_empty[st]);
-            __syncwarp();
-        };
-        auto read = [&](int mt) {  // the last product that read p of tile mt is done
-            const uint32_t k = mt ? n_pv1 : n_pv0;
-            return k == 0 || bar_wait(&B.pv_done[mt], (k - 1) & 1);
-        };
         while (ok && w.next()) {
             const bool two = w.pr.t0 + tpt < w.pr.t1;
             ok = bar_wait(&B.q_full[0], n_q0++ & 1);
             if (ok && two) ok = bar_wait(&B.q_full[1], n_q1++ & 1);
-            if (ok) ok = read(0) && read(1) && bar_wait(&B.kv_full[n % C::NST], (n / C::NST) & 1);
-            if (!ok) break;
-            tc_fence_after();
-            uint32_t buf = n_buf;  // of the next p
 #pragma unroll 1
-            for (int mt = 0; mt < (two ? 2 : 1); mt++) scores(mt, n % C::NST);
-            release(n % C::NST);
-            n++;
+            for (int i = 0; i < w.n_it && ok; i++, n += 2) {
+                const uint32_t st = n % C::NST;
+                ok = bar_wait(&B.kv_full[st], (n / C::NST) & 1);
 #pragma unroll 1
-            for (int i = 0; i < w.n_it && ok; i++) {
-                const uint32_t nv = n, nk = n + 1;
-                const bool more = i + 1 < w.n_it;
-                ok = bar_wait(&B.kv_full[nv % C::NST], (nv / C::NST) & 1);
+                for (int mt = 0; mt < (two ? 2 : 1) && ok; mt++) {
+                    const uint32_t b = n_buf % 3, use = n_buf / 3;
+                    if (use > 0) ok = bar_wait(&B.s_free[b], (use - 1) & 1);
+                    if (!ok) break;
+                    n_buf++;
+                    tc_fence_after();
+                    const uint32_t d = tm + b * UNIT;
+                    const uint32_t qd = desc_lo(q_addr + mt * 2 * C::TILE, 0), kd = desc_lo(kv_addr + st * C::TILE, 0);
+                    if (elect()) {
+#pragma unroll
+                        for (int part = 0; part < 2; part++)  // low parts first
+#pragma unroll
+                            for (int k = 0; k < HD / 16; k++) {
+                                const uint32_t off = ((k >> 2) * C::BLK + (k & 3) * 32) >> 4;
+                                mma_smem_a(d, qd + ((part * C::TILE) >> 4) + off, kd + off, ID_S, part | k);
+                            }
+                        tc_commit(&B.s_full[mt]);
+                        mbar_arrive(&B.s_full[mt]);  // what this warp saw of the loads (B.valid) is passed on
+                        if (mt == 1 || !two) tc_commit(&B.kv_empty[st]);
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        // whatever was issued is done before the tensor memory goes back: the last k tile's release follows its products
+        if (n > 0) bar_wait(&B.kv_empty[(n - 2) % C::NST], ((n - 2) / C::NST) & 1);
+        } else if (warp == 10) {
+        // ---------------------------------------------------------------- products p v
+        // O is one buffer, read by the tile's softmax warps while the other products run.
+        constexpr uint32_t ID_O = tc_idesc_f16(128, HD) | (1u << 16);
+        uint32_t n = 1, n_p0 = 0, n_p1 = 0, n_buf = 0;
+        const uint32_t kv_addr = __shfl_sync(0xffffffffu, smem_u32(skv), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
+        while (ok && w.next()) {
+            const bool two = w.pr.t0 + tpt < w.pr.t1;
+#pragma unroll 1
+            for (int i = 0; i < w.n_it && ok; i++, n += 2) {
+                const uint32_t st = n % C::NST;
+                ok = bar_wait(&B.kv_full[st], (n / C::NST) & 1);
                 if (!ok) break;
                 const int p0 = w.pr.unit(w.u0 + i) * UNIT;
                 if (p0 + UNIT - 1 > w.pr.lim_max || (p0 < w.pr.low_min && p0 + UNIT > A.n_sink)) {
                     // positions that no row sees may hold anything: their v rows become zero, as their p are
-                    uint8_t* vt = skv + (nv % C::NST) * C::TILE;
+                    uint8_t* vt = skv + st * C::TILE;
 #pragma unroll 4
                     for (int j = lane >> 3; j < UNIT; j += 4) {  // 8 lanes a row
                         const int p = p0 + j;
@@ -651,31 +659,28 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
                 }
 #pragma unroll 1
                 for (int mt = 0; mt < (two ? 2 : 1); mt++) {
-                    ok = bar_wait(&B.p_full[mt], (mt ? n_p1++ : n_p0++) & 1);
-                    if (ok && n_o > 0) ok = bar_wait(&B.o_free, (n_o - 1) & 1);
+                    if (n_buf > 0) ok = bar_wait(&B.o_free, (n_buf - 1) & 1);
+                    if (ok) ok = bar_wait(&B.p_full[mt], (mt ? n_p1++ : n_p0++) & 1);
                     if (!ok) break;
-                    n_o++;
+                    const uint32_t b = n_buf++ % 3;
                     tc_fence_after();
-                    values(mt, nv % C::NST, buf++);
-                    const bool last = mt == 1 || !two;
-                    if (last) release(nv % C::NST);
-                    if (more) {
-                        if (mt == 0) ok = bar_wait(&B.kv_full[nk % C::NST], (nk / C::NST) & 1);
-                        if (ok && two) ok = read(1 - mt);
-                        if (!ok) break;
-                        tc_fence_after();
-                        scores(mt, nk % C::NST);
-                        if (last) release(nk % C::NST);
+                    const uint32_t vd = desc_lo(kv_addr + st * C::TILE, C::BLK), p = tm + b * UNIT;
+                    if (elect()) {
+#pragma unroll
+                        for (int part = 0; part < 2; part++)  // low parts first
+#pragma unroll
+                            for (int k = 0; k < UNIT / 16; k++)
+                                mma_tmem_a(tm + C::O_COL, p + 32 * (k >> 1) + (part ? 0 : 16) + 8 * (k & 1),
+                                           vd + ((k * 2048) >> 4), ID_O, part | k);
+                        tc_commit(&B.pv_done[mt]);
+                        tc_commit(&B.s_free[b]);
+                        if (mt == 1 || !two) tc_commit(&B.kv_empty[st]);
                     }
+                    __syncwarp();
                 }
-                n += more ? 2 : 1;
             }
         }
-        // whatever was issued is done before the tensor memory goes back
-        read(0);
-        read(1);
-        if (n_s0) bar_wait(&B.s_full[0], (n_s0 - 1) & 1);
-        if (n_s1) bar_wait(&B.s_full[1], (n_s1 - 1) & 1);
+        if (n > 1) bar_wait(&B.kv_empty[(n - 2) % C::NST], ((n - 2) / C::NST) & 1);
         }
     }
     if (!ok && lane == 0 && a.status) atomicOr(a.status, (int)ST_WAIT_TIMEOUT);
