@@ -183,9 +183,10 @@ __global__ void __launch_bounds__(CP_NT) k_pages_copy(uint4* __restrict__ k, uin
 // joined by their (m, sum, o).
 //
 // A step reads 2 hd es bytes per position and kv head and does 4 hd flops per q head with them: it is bound by
-// the reads, so every operand goes from memory straight into the registers of the matrix instructions, in the
-// order in which it lies (the sums run over hd and over positions, whose order is free, and so is the order of
-// the output's columns): no shared memory, no barrier, 16-byte loads.
+// the reads. Every warp has its own positions and its own ring of tiles in shared memory, which it fills ahead by
+// asynchronous 16-byte copies: no barrier between warps. A tile keeps rows of 128 bytes with exchanged 16-byte chunks
+// (chunk c of row r at c ^ (r mod 8)); the sums run over hd and over positions, whose order is free, and so is the order of
+// the output's columns, so a thread's operands of several instructions are one 16-byte load without bank conflicts.
 //
 // Numerics. Activations are 32-bit and the pools hold 11 or 24 bits. q and p are split in two parts of 11 bits
 // (hi + lo: 22 bits, 2^-23 relative), which the matrix instructions multiply exactly and add in 32 bits:
@@ -215,6 +216,9 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
         "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, int bytes) {  // bytes 16, or 0: zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ uint32_t h2(__half a, __half b) {
     const __half2 v = __halves2half2(a, b);
@@ -255,8 +259,10 @@ template <typename T, int HD, bool STACK>
 struct AttnSmem {
     static constexpr int RT = STACK ? 8 : 16;
     static constexpr int KS = sizeof(T) == 2 ? HD / 16 : HD / 8;  // k steps of a score
+    static constexpr int TILE = 32 * HD;                          // bytes of a step's k (v) rows
+    static constexpr int NS = HD == 128 ? 3 : 6;                  // tiles of a warp's ring: 24 KB, 96 KB a block, two blocks an SM
+    uint8_t ring[PA_NW][NS][2][TILE];                             // at a tile's end the warp's sums [RT][HD + 4]
     uint4 qf[STACK ? 1 : KS * 32 * 2];                            // 16 rows: q in fragment order, hi then lo
-    float o[PA_NW][RT][HD + 4];
     float m[PA_NW][RT], l[PA_NW][RT];
     float cs[RT];  // score scale of each row
 };
@@ -270,12 +276,15 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
     constexpr int STEP = pos_step<T>(), UNIT = STEP * PA_NW, RT = STACK ? 8 : 16, NR = STACK ? 1 : 2;
     constexpr int KS = AttnSmem<T, HD, STACK>::KS;  // k steps of q k
     constexpr int NT = HD / 8;                      // column tiles of p v
-    constexpr int KC = HD * (int)sizeof(T) / 64;    // 16-byte chunks of a K row a thread loads (4 threads a row)
-    constexpr int VC = HD * (int)sizeof(T) / 128;   // of a V row (8 threads a row)
+    constexpr int PA_NS = AttnSmem<T, HD, STACK>::NS;
+    constexpr int NB = HD * (int)sizeof(T) / 128;   // 128-byte blocks of a row
+    constexpr int CPL = STEP * NB * 8 / 32;         // 16-byte chunks of a step's k (v) that a lane copies
     constexpr int JT = STEP / 8;                    // score tiles of a step
-    constexpr int PT = 2 * JT;                      // positions whose V rows a thread loads
+    constexpr int PT = 2 * JT;                      // positions whose v rows a thread reads
+    constexpr int BLK = STEP * 128;                 // bytes of a block of a tile
     extern __shared__ __align__(16) uint8_t smem_raw[];
     AttnSmem<T, HD, STACK>& S = *reinterpret_cast<AttnSmem<T, HD, STACK>*>(smem_raw);
+    auto sums = [&](int w, int r) { return reinterpret_cast<float*>(S.ring[w]) + r * (HD + 4); };
     __shared__ long long s_scan[PA_NW], s_start;
     __shared__ int s_seq;
     const PagedArgs& a = A.c;
@@ -365,7 +374,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
             constexpr int PER = H16 ? 4 : 2;
 #pragma unroll
             for (int c = 0; c < (int)(sizeof(x) / 16); c++) {
-                const int e = H16 ? 8 * (t + 4 * (c >> 1)) + 4 * (c & 1) : 4 * (t + 4 * c);
+                const int e = H16 ? 64 * (c >> 2) + 8 * (2 * t + ((c >> 1) & 1)) + 4 * (c & 1) : 32 * (c >> 1) + 4 * (2 * t + (c & 1));
                 const float4 f = ok ? *reinterpret_cast<const float4*>(qr + e) : make_float4(0.f, 0.f, 0.f, 0.f);
                 x[4 * c] = f.x;
                 x[4 * c + 1] = f.y;
@@ -420,49 +429,47 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
         const int low_min = A.window > 0 ? first_pos - A.window + 1 : 0;
         auto any = [&](int j) { return j <= lim_max && (j >= low_min || j < A.n_sink); };
 
-        // ---- K and V of a step: page ids of 32 steps at a time, one per lane
-        int ids = -1;
+        // ---- k and v of a step: page ids of 32 steps at a time, one per lane, the next 32 fetched ahead
         auto fetch_ids = [&](int it) {
             const int i = it + lane;
-            ids = -1;
+            int id = -1;
             if (i < n_it) {
                 const int p = un.unit(u0 + i) * UNIT + warp * STEP;
-                if (p < sq.kv && (any(p) || any(p + STEP - 1) || (p < low_min && p + STEP > low_min))) {
-                    ids = a.table[(size_t)seq * a.table_ld + p / a.page];
-                    if ((unsigned)ids >= (unsigned)a.n_pages) {
+                if (any(p) || any(p + STEP - 1) || (p < low_min && p + STEP > low_min && low_min <= lim_max)) {
+                    id = a.table[(size_t)seq * a.table_ld + p / a.page];
+                    if ((unsigned)id >= (unsigned)a.n_pages) {
                         paged_flag(a.status);
-                        ids = -1;
+                        id = -1;
                     }
                 }
             }
+            return id;
         };
-        uint4 kr[JT][KC], vr[PT][VC];
-        auto base_of = [&](int it, int& p) -> long long {  // element offset of the step's first position, or -1
-            if ((it & 31) == 0) fetch_ids(it);
-            const int id = __shfl_sync(0xffffffffu, ids, it & 31);
-            p = un.unit(u0 + it) * UNIT + warp * STEP;
-            if (it >= n_it || id < 0) return -1;
-            return (long long)((size_t)id * a.page_stride + ((size_t)kvh * a.page + p % a.page) * HD);
-        };
-        auto load_k = [&](long long base, int p) {
+        int ids = fetch_ids(0), ids_next = n_it > 32 ? fetch_ids(32) : -1;
+        uint32_t live = 0;  // steps in the ring (bit: it mod 32) whose page is one of the pool's
+        const uint32_t ring = smem_u32(S.ring[warp]);
+        auto load = [&](int it) {  // rows of positions that no row sees become zero: 0 * NaN is NaN
+            if (it < n_it) {
+                if ((it & 31) == 0 && it > 0) {
+                    ids = ids_next;
+                    if (it + 32 < n_it) ids_next = fetch_ids(it + 32);
+                }
+                const int id = __shfl_sync(0xffffffffu, ids, it & 31), p = un.unit(u0 + it) * UNIT + warp * STEP;
+                live = id >= 0 ? live | 1u << (it & 31) : live & ~(1u << (it & 31));
+                const size_t at = (size_t)(id >= 0 ? id : 0) * a.page_stride + ((size_t)kvh * a.page + p % a.page) * HD;
+                const uint8_t* ks = reinterpret_cast<const uint8_t*>(kp + at) + 16 * lane;
+                const uint8_t* vs = reinterpret_cast<const uint8_t*>(vp + at) + 16 * lane;
+                const uint32_t slot = ring + (it % PA_NS) * 2 * AttnSmem<T, HD, STACK>::TILE;
 #pragma unroll
-            for (int j = 0; j < JT; j++) {
-                const int r = 8 * j + g;
-                const bool ok = base >= 0 && any(p + r);
-                const uint4* src = reinterpret_cast<const uint4*>(kp + base + (size_t)r * HD) + t;
-#pragma unroll
-                for (int c = 0; c < KC; c++) kr[j][c] = ok ? __ldg(src + 4 * c) : make_uint4(0, 0, 0, 0);
+                for (int j = 0; j < CPL; j++) {
+                    const int x = lane + 32 * j, row = x / (NB * 8), c = x % (NB * 8);
+                    const uint32_t d = slot + (c >> 3) * BLK + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+                    const int n = id >= 0 && any(p + row) ? 16 : 0;
+                    cp_async16_or_zero(d, ks + 512 * j, n);
+                    cp_async16_or_zero(d + AttnSmem<T, HD, STACK>::TILE, vs + 512 * j, n);
+                }
             }
-        };
-        auto load_v = [&](long long base, int p) {  // rows of positions no row sees stay zero: 0 * NaN is NaN
-#pragma unroll
-            for (int j = 0; j < PT; j++) {
-                const int r = 8 * (j >> 1) + 2 * t + (j & 1);
-                const bool ok = base >= 0 && any(p + r);
-                const uint4* src = reinterpret_cast<const uint4*>(vp + base + (size_t)r * HD) + g;
-#pragma unroll
-                for (int c = 0; c < VC; c++) vr[j][c] = ok ? __ldg(src + 8 * c) : make_uint4(0, 0, 0, 0);
-            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
         float o[NT][2 * NR];
 #pragma unroll
@@ -475,48 +482,57 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
             m[i] = -INFINITY;
             l[i] = 0.f;
         }
-        int p;
-        long long base = base_of(0, p);
-        load_k(base, p);
-        load_v(base, p);
+#pragma unroll
+        for (int i = 0; i < PA_NS - 1; i++) load(i);
         for (int it = 0; it < n_it; it++) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(PA_NS - 2) : "memory");
+            __syncwarp();  // every lane's copies have landed, and every lane is done with the tile that comes free
+            load(it + PA_NS - 1);
+            const uint8_t* kt = S.ring[warp][it % PA_NS][0];
+            const uint8_t* vt = S.ring[warp][it % PA_NS][1];
+            const int p_cur = un.unit(u0 + it) * UNIT + warp * STEP;
+            const bool on = (live >> (it & 31)) & 1;
+            if (!on) continue;  // warp-uniform: no row sees any of the step's positions
             float sacc[JT][4], slow[JT][4];  // the high parts' product and the rest, joined once at the end
 #pragma unroll
             for (int j = 0; j < JT; j++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) sacc[j][i] = slow[j][i] = 0.f;
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                uint32_t ah[4], al[4];
-                if (STACK) {
+            for (int c = 0; c < KS / 2; c++) {  // a 16-byte chunk of the k rows: two k steps
+                uint4 w[JT];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) ah[i] = qa[k][i];
-                } else {
-                    const uint4 h = S.qf[(k * 32 + lane) * 2], lo4 = S.qf[(k * 32 + lane) * 2 + 1];
-                    ah[0] = h.x, ah[1] = h.y, ah[2] = h.z, ah[3] = h.w;
-                    al[0] = lo4.x, al[1] = lo4.y, al[2] = lo4.z, al[3] = lo4.w;
-                }
+                for (int j = 0; j < JT; j++)
+                    w[j] = *reinterpret_cast<const uint4*>(kt + (c >> 1) * BLK + (8 * j + g) * 128 + (((2 * t + (c & 1)) ^ g) << 4));
 #pragma unroll
-                for (int j = 0; j < JT; j++) {
-                    const uint4& w = kr[j][k >> 1];
-                    const uint32_t b0 = (k & 1) ? w.z : w.x, b1 = (k & 1) ? w.w : w.y;
-                    if (H16) {
-                        mma_f16(sacc[j], ah, b0, b1);
-                        if (!STACK) mma_f16(slow[j], al, b0, b1);
+                for (int h = 0; h < 2; h++) {
+                    const int k = 2 * c + h;
+                    uint32_t ah[4], al[4];
+                    if (STACK) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) ah[i] = qa[k][i];
                     } else {
-                        uint32_t h0, l0, h1, l1;
-                        split_tf32(__uint_as_float(b0), h0, l0);
-                        split_tf32(__uint_as_float(b1), h1, l1);
-                        mma_tf32(sacc[j], ah, h0, h1);
-                        mma_tf32(slow[j], ah, l0, l1);
-                        if (!STACK) mma_tf32(slow[j], al, h0, h1);
+                        const uint4 f = S.qf[(k * 32 + lane) * 2], lo4 = S.qf[(k * 32 + lane) * 2 + 1];
+                        ah[0] = f.x, ah[1] = f.y, ah[2] = f.z, ah[3] = f.w;
+                        al[0] = lo4.x, al[1] = lo4.y, al[2] = lo4.z, al[3] = lo4.w;
+                    }
+#pragma unroll
+                    for (int j = 0; j < JT; j++) {
+                        const uint32_t b0 = h ? w[j].z : w[j].x, b1 = h ? w[j].w : w[j].y;
+                        if (H16) {
+                            mma_f16(sacc[j], ah, b0, b1);
+                            if (!STACK) mma_f16(slow[j], al, b0, b1);
+                        } else {
+                            uint32_t h0, l0, h1, l1;
+                            split_tf32(__uint_as_float(b0), h0, l0);
+                            split_tf32(__uint_as_float(b1), h1, l1);
+                            mma_tf32(sacc[j], ah, h0, h1);
+                            mma_tf32(slow[j], ah, l0, l1);
+                            if (!STACK) mma_tf32(slow[j], al, h0, h1);
+                        }
                     }
                 }
             }
-            const int p_cur = p;
-            const bool live = base >= 0;
-            base = base_of(it + 1, p);
-            load_k(base, p);  // the next K rows travel during the softmax and p v
             // ---- scores of this thread's rows: positions p + 8 j + 2 t + c
             float sv[NR][PT];
             float mx[NR];
@@ -529,7 +545,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                     const int e = (j & 1) + 2 * i;
                     float raw = sacc[j >> 1][e] + slow[j >> 1][e];
                     if (STACK) raw += sacc[j >> 1][e + 2];
-                    const bool see = live && pos <= lim[i] && (pos >= low[i] || pos < A.n_sink);
+                    const bool see = pos <= lim[i] && (pos >= low[i] || pos < A.n_sink);
                     sv[i][j] = see ? raw * cs[i] : -INFINITY;
                     mx[i] = fmaxf(mx[i], sv[i][j]);
                 }
@@ -571,7 +587,13 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                 }
             }
 #pragma unroll
-            for (int c = 0; c < VC; c++)
+            for (int c = 0; c < NB; c++) {
+                uint4 vr[PT];  // rows 2t, 2t + 1 (and 8 on): chunk g of the block
+#pragma unroll
+                for (int j = 0; j < PT; j++) {
+                    const int row = 8 * (j >> 1) + 2 * t + (j & 1);
+                    vr[j] = *reinterpret_cast<const uint4*>(vt + c * BLK + row * 128 + ((g ^ (row & 7)) << 4));
+                }
 #pragma unroll
                 for (int e = 0; e < 16 / (int)sizeof(T); e++) {
                     const int n = c * (16 / (int)sizeof(T)) + e;
@@ -579,15 +601,15 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                     if (H16) {
                         const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
                         auto word = [&](const uint4& w) { return (e >> 1) == 0 ? w.x : (e >> 1) == 1 ? w.y : (e >> 1) == 2 ? w.z : w.w; };
-                        const uint32_t b0 = __byte_perm(word(vr[0][c]), word(vr[1][c]), sel);
-                        const uint32_t b1 = __byte_perm(word(vr[PT - 2][c]), word(vr[PT - 1][c]), sel);
+                        const uint32_t b0 = __byte_perm(word(vr[0]), word(vr[1]), sel);
+                        const uint32_t b1 = __byte_perm(word(vr[PT - 2]), word(vr[PT - 1]), sel);
                         if (!STACK) mma_f16(s, pl, b0, b1);
                         mma_f16(s, ph, b0, b1);
                     } else {
                         auto word = [&](const uint4& w) { return e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w; };
                         uint32_t h0, l0, h1, l1;
-                        split_tf32(__uint_as_float(word(vr[0][c])), h0, l0);
-                        split_tf32(__uint_as_float(word(vr[1][c])), h1, l1);
+                        split_tf32(__uint_as_float(word(vr[0])), h0, l0);
+                        split_tf32(__uint_as_float(word(vr[1])), h1, l1);
                         if (!STACK) mma_tf32(s, pl, h0, h1);
                         mma_tf32(s, ph, l0, l1);
                         mma_tf32(s, ph, h0, h1);
@@ -595,8 +617,9 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
 #pragma unroll
                     for (int i = 0; i < 2 * NR; i++) o[n][i] += STACK ? s[i] + s[i + 2 * (STACK ? 1 : 0)] : s[i];
                 }
-            load_v(base, p);
+            }
         }
+        __syncwarp();  // the ring is read
         // ---- the four warps' parts joined, then the output or this block's partial record
 #pragma unroll
         for (int i = 0; i < NR; i++) {
@@ -612,13 +635,13 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
             constexpr int E = 16 / (int)sizeof(T);
             const int col = E * (2 * t + 8 * (n / E)) + n % E;
             if (STACK) {
-                S.o[warp][g][col] = o[n][0];
-                S.o[warp][g][col + E] = o[n][1];
+                sums(warp, g)[col] = o[n][0];
+                sums(warp, g)[col + E] = o[n][1];
             } else {
 #pragma unroll
                 for (int i = 0; i < NR; i++) {
-                    S.o[warp][g + 8 * i][col] = o[n][2 * i];
-                    S.o[warp][g + 8 * i][col + E] = o[n][2 * i + 1];
+                    sums(warp, g + 8 * i)[col] = o[n][2 * i];
+                    sums(warp, g + 8 * i)[col + E] = o[n][2 * i + 1];
                 }
             }
         }
@@ -636,7 +659,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
             for (int w = 0; w < PA_NW; w++) {
                 const float e = S.m[w][r] == -INFINITY ? 0.f : exp2f(S.m[w][r] - M);
                 if (S.m[w][r] == -INFINITY && !(S.l[w][r] != S.l[w][r])) continue;
-                const float4 f = *reinterpret_cast<const float4*>(&S.o[w][r][4 * c4]);
+                const float4 f = *reinterpret_cast<const float4*>(sums(w, r) + 4 * c4);
                 L = fmaf(S.l[w][r], e, L);
                 acc.x = fmaf(f.x, e, acc.x);
                 acc.y = fmaf(f.y, e, acc.y);
