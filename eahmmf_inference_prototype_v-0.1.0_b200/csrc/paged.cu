@@ -230,10 +230,28 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
     hi = h2(hx, hy);
     lo = h2(__float2half_rn(x - __half2float(hx)), __float2half_rn(y - __half2float(hy)));
 }
+// x as two parts of 11 bits, both cut (the conversion instruction that rounds runs at a quarter of the rate): 2^-21 of x at
+// most is left out. An infinity or NaN keeps its kind in hi.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    const float r = x - __uint_as_float(hi);
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(r));
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+}
+__device__ __forceinline__ float ex2(float v) {  // 2 units of 32 bits; results below 2^-126 are zero, as weights of them may be
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ void add2(float& a, float& b, float c, float d) {  // (a, b) += (c, d) in one instruction
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(a), "+f"(b)
+        : "f"(c), "f"(d));
+}
+// Two 8 x 8 blocks of 16-bit elements below each other, twice, transposed: the right operands of two column tiles
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
 }
 
 // Units of positions that some row of a sequence sees: sink units [0, us), then units [uw, ue).
@@ -282,7 +300,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
     constexpr int JT = STEP / 8;                    // score tiles of a step
     constexpr int PT = 2 * JT;                      // positions whose v rows a thread reads
     constexpr int BLK = STEP * 128;                 // bytes of a block of a tile
-    extern __shared__ __align__(16) uint8_t smem_raw[];
+    extern __shared__ __align__(128) uint8_t smem_raw[];
     AttnSmem<T, HD, STACK>& S = *reinterpret_cast<AttnSmem<T, HD, STACK>*>(smem_raw);
     auto sums = [&](int w, int r) { return reinterpret_cast<float*>(S.ring[w]) + r * (HD + 4); };
     __shared__ long long s_scan[PA_NW], s_start;
@@ -427,6 +445,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
         if (!STACK) __syncthreads();
         const int lim_max = p_first + (r0 + n_rows - 1) / a.grp, first_pos = p_first + r0 / a.grp;
         const int low_min = A.window > 0 ? first_pos - A.window + 1 : 0;
+        const int lim_min = first_pos, low_max = A.window > 0 ? lim_max - A.window + 1 : 0;
         auto any = [&](int j) { return j <= lim_max && (j >= low_min || j < A.n_sink); };
 
         // ---- k and v of a step: page ids of 32 steps at a time, one per lane, the next 32 fetched ahead
@@ -448,6 +467,8 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
         int ids = fetch_ids(0), ids_next = n_it > 32 ? fetch_ids(32) : -1;
         uint32_t live = 0;  // steps in the ring (bit: it mod 32) whose page is one of the pool's
         const uint32_t ring = smem_u32(S.ring[warp]);
+        constexpr int RPP = 32 / (NB * 8);  // rows that a warp's copies of one instruction cover
+        const uint32_t lane_at = ((lane % (NB * 8)) >> 3) * BLK + lane / (NB * 8) * 128 + (((lane & 7) ^ (lane / (NB * 8))) << 4);
         auto load = [&](int it) {  // rows of positions that no row sees become zero: 0 * NaN is NaN
             if (it < n_it) {
                 if ((it & 31) == 0 && it > 0) {
@@ -460,11 +481,11 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                 const uint8_t* ks = reinterpret_cast<const uint8_t*>(kp + at) + 16 * lane;
                 const uint8_t* vs = reinterpret_cast<const uint8_t*>(vp + at) + 16 * lane;
                 const uint32_t slot = ring + (it % PA_NS) * 2 * AttnSmem<T, HD, STACK>::TILE;
+                const bool full = id >= 0 && p + STEP - 1 <= lim_max && (p >= low_min || p + STEP <= A.n_sink);
 #pragma unroll
-                for (int j = 0; j < CPL; j++) {
-                    const int x = lane + 32 * j, row = x / (NB * 8), c = x % (NB * 8);
-                    const uint32_t d = slot + (c >> 3) * BLK + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-                    const int n = id >= 0 && any(p + row) ? 16 : 0;
+                for (int j = 0; j < CPL; j++) {  // rows lane / (8 NB) + RPP j: the exchange of chunks splits into lane's and j's part
+                    const uint32_t d = (slot + lane_at + j * RPP * 128) ^ (((j * RPP) & 7) << 4);
+                    const int n = full || (id >= 0 && any(p + lane / (NB * 8) + j * RPP)) ? 16 : 0;
                     cp_async16_or_zero(d, ks + 512 * j, n);
                     cp_async16_or_zero(d + AttnSmem<T, HD, STACK>::TILE, vs + 512 * j, n);
                 }
@@ -534,6 +555,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                 }
             }
             // ---- scores of this thread's rows: positions p + 8 j + 2 t + c
+            const bool plain = p_cur + STEP - 1 <= lim_min && (p_cur >= low_max || p_cur + STEP <= A.n_sink);  // all rows see all
             float sv[NR][PT];
             float mx[NR];
 #pragma unroll
@@ -545,7 +567,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                     const int e = (j & 1) + 2 * i;
                     float raw = sacc[j >> 1][e] + slow[j >> 1][e];
                     if (STACK) raw += sacc[j >> 1][e + 2];
-                    const bool see = pos <= lim[i] && (pos >= low[i] || pos < A.n_sink);
+                    const bool see = plain || (pos <= lim[i] && (pos >= low[i] || pos < A.n_sink));
                     sv[i][j] = see ? raw * cs[i] : -INFINITY;
                     mx[i] = fmaxf(mx[i], sv[i][j]);
                 }
@@ -559,7 +581,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                 float al[NR];
 #pragma unroll
                 for (int i = 0; i < NR; i++) {
-                    al[i] = mx[i] == -INFINITY ? 1.f : exp2f(m[i] - mx[i]);
+                    al[i] = mx[i] == -INFINITY ? 1.f : ex2(m[i] - mx[i]);
                     l[i] *= al[i];
                     m[i] = mx[i];
                 }
@@ -574,7 +596,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                 const float mo = m[i] == -INFINITY ? 0.f : m[i] - P_SHIFT;
 #pragma unroll
                 for (int j = 0; j < PT; j++) {
-                    sv[i][j] = exp2f(sv[i][j] - mo);
+                    sv[i][j] = ex2(sv[i][j] - mo);
                     l[i] += sv[i][j];
                 }
                 if (H16) {
@@ -586,36 +608,50 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                     for (int j = 0; j < PT; j++) split_tf32(sv[i][j], ph[2 * j + i], STACK ? ph[2 * j + 1] : pl[2 * j + i]);
                 }
             }
-#pragma unroll
-            for (int c = 0; c < NB; c++) {
-                uint4 vr[PT];  // rows 2t, 2t + 1 (and 8 on): chunk g of the block
-#pragma unroll
-                for (int j = 0; j < PT; j++) {
-                    const int row = 8 * (j >> 1) + 2 * t + (j & 1);
-                    vr[j] = *reinterpret_cast<const uint4*>(vt + c * BLK + row * 128 + ((g ^ (row & 7)) << 4));
+            // this step's part of the sums apart, see "Numerics"
+            auto join = [&](int n, const float (&s)[4]) {
+                if (STACK) {
+                    float x = s[0], y = s[1];
+                    add2(x, y, s[2], s[3]);
+                    add2(o[n][0], o[n][1], x, y);
+                } else {
+                    add2(o[n][0], o[n][1], s[0], s[1]);
+                    add2(o[n][2 * NR - 2], o[n][2 * NR - 1], s[2], s[3]);
                 }
+            };
+            if (H16) {
+                const uint32_t va = smem_u32(vt) + (lane & 15) * 128;  // lanes 0-15: rows of a column tile's chunk, 16-31: the next chunk
 #pragma unroll
-                for (int e = 0; e < 16 / (int)sizeof(T); e++) {
-                    const int n = c * (16 / (int)sizeof(T)) + e;
-                    float s[4] = {0.f, 0.f, 0.f, 0.f};  // this step's part of the sums, see "Numerics"
-                    if (H16) {
-                        const uint32_t sel = (e & 1) ? 0x7632u : 0x5410u;
-                        auto word = [&](const uint4& w) { return (e >> 1) == 0 ? w.x : (e >> 1) == 1 ? w.y : (e >> 1) == 2 ? w.z : w.w; };
-                        const uint32_t b0 = __byte_perm(word(vr[0]), word(vr[1]), sel);
-                        const uint32_t b1 = __byte_perm(word(vr[PT - 2]), word(vr[PT - 1]), sel);
-                        if (!STACK) mma_f16(s, pl, b0, b1);
-                        mma_f16(s, ph, b0, b1);
-                    } else {
+                for (int n = 0; n < NT; n += 2) {
+                    uint32_t b[4];
+                    ldsm_t(b, va + (n >> 3) * BLK + ((((n & 7) + (lane >> 4)) ^ (lane & 7)) << 4));
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float s[4] = {0.f, 0.f, 0.f, 0.f};
+                        if (!STACK) mma_f16(s, pl, b[2 * h], b[2 * h + 1]);
+                        mma_f16(s, ph, b[2 * h], b[2 * h + 1]);
+                        join(n + h, s);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < NB; c++) {
+                    uint4 vr[2];  // rows 2t and 2t + 1: chunk g of the block
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+                        vr[j] = *reinterpret_cast<const uint4*>(vt + c * BLK + (2 * t + j) * 128 + ((g ^ (2 * t + j)) << 4));
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
                         auto word = [&](const uint4& w) { return e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w; };
+                        float s[4] = {0.f, 0.f, 0.f, 0.f};
                         uint32_t h0, l0, h1, l1;
                         split_tf32(__uint_as_float(word(vr[0])), h0, l0);
                         split_tf32(__uint_as_float(word(vr[1])), h1, l1);
                         if (!STACK) mma_tf32(s, pl, h0, h1);
                         mma_tf32(s, ph, l0, l1);
                         mma_tf32(s, ph, h0, h1);
+                        join(4 * c + e, s);
                     }
-#pragma unroll
-                    for (int i = 0; i < 2 * NR; i++) o[n][i] += STACK ? s[i] + s[i + 2 * (STACK ? 1 : 0)] : s[i];
                 }
             }
         }
@@ -632,17 +668,12 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
         }
 #pragma unroll
         for (int n = 0; n < NT; n++) {
-            constexpr int E = 16 / (int)sizeof(T);
-            const int col = E * (2 * t + 8 * (n / E)) + n % E;
-            if (STACK) {
-                sums(warp, g)[col] = o[n][0];
-                sums(warp, g)[col + E] = o[n][1];
-            } else {
+            // 16-bit v: columns 8 n + 2t, + 1; 32-bit v: columns 4 (2t + 8 (n / 4)) + n % 4, + 4
+            const int col = H16 ? 8 * n + 2 * t : 4 * (2 * t + 8 * (n / 4)) + n % 4, next = H16 ? 1 : 4;
 #pragma unroll
-                for (int i = 0; i < NR; i++) {
-                    sums(warp, g + 8 * i)[col] = o[n][2 * i];
-                    sums(warp, g + 8 * i)[col + E] = o[n][2 * i + 1];
-                }
+            for (int i = 0; i < NR; i++) {
+                sums(warp, g + 8 * i)[col] = o[n][2 * i];
+                sums(warp, g + 8 * i)[col + next] = o[n][2 * i + 1];
             }
         }
         __syncthreads();
