@@ -217,6 +217,9 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, int bytes) {  // bytes 16, or 0: zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -278,7 +281,7 @@ struct AttnSmem {
     static constexpr int RT = STACK ? 8 : 16;
     static constexpr int KS = sizeof(T) == 2 ? HD / 16 : HD / 8;  // k steps of a score
     static constexpr int TILE = 32 * HD;                          // bytes of a step's k (v) rows
-    static constexpr int NS = HD == 128 ? 3 : 6;                  // tiles of a warp's ring: 24 KB, 96 KB a block, two blocks an SM
+    static constexpr int NS = HD == 128 ? 2 : 4;                  // tiles of a warp's ring: 16 KB, 64 KB a block
     uint8_t ring[PA_NW][NS][2][TILE];                             // at a tile's end the warp's sums [RT][HD + 4]
     uint4 qf[STACK ? 1 : KS * 32 * 2];                            // 16 rows: q in fragment order, hi then lo
     float m[PA_NW][RT], l[PA_NW][RT];
@@ -310,48 +313,48 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
     pdl_wait();
     pdl_trigger();
 
-    // ---- this block's share of the call: work items in (sequence, kv head, row tile, unit) order
+    // ---- this block's share of the call: work items in (sequence, kv head, row tile, unit) order, or whole row tiles
     auto weight = [&](int s, bool flag) -> long long {
         const Seq sq = paged_seq(a, s, flag);
         if (!step_takes(A, sq)) return 0;
-        return (long long)units_of(sq, A.window, A.n_sink, UNIT).n() * a.n_kv * ((sq.q * a.grp + RT - 1) / RT);
+        const int n = A.whole ? 1 : units_of(sq, A.window, A.n_sink, UNIT).n();
+        return (long long)n * a.n_kv * ((sq.q * a.grp + RT - 1) / RT);
     };
-    long long total = 0, mine = 0;
-    for (int s0 = 0; s0 < a.n_seq; s0 += PA_NT) {
-        mine = s0 + tid < a.n_seq ? weight(s0 + tid, blockIdx.x == 0) : 0;
-        long long v = mine;
-#pragma unroll
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == 0) s_scan[warp] = v;
-        __syncthreads();
-        total += s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
-        __syncthreads();
-    }
-    const long long share = max((total + gridDim.x - 1) / gridDim.x, (long long)(A.min_units));
-    const long long begin = share * blockIdx.x, end = min(total, begin + share);
-    if (tid == 0) A.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-    if (begin >= total) return;
-    long long run = 0;
-    for (int s0 = 0; s0 < a.n_seq; s0 += PA_NT) {  // the sequence that holds `begin`
-        if (a.n_seq > PA_NT) mine = s0 + tid < a.n_seq ? weight(s0 + tid, false) : 0;
-        long long v = mine;
+    long long total = 0, mine = 0, upto = 0;  // of thread's sequence s0 + tid: its weight, and the sum with it
+    auto scan = [&](int s0, bool flag) {
+        mine = s0 + tid < a.n_seq ? weight(s0 + tid, flag) : 0;
+        upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long n = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += n;
+            const long long n = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += n;
         }
-        if (lane == 31) s_scan[warp] = v;
+        __syncthreads();  // s_scan is read
+        if (lane == 31) s_scan[warp] = upto;
         __syncthreads();
-        for (int w = 0; w < warp; w++) v += s_scan[w];
-        v += run;
-        if (mine > 0 && v - mine <= begin && begin < v) {
+        upto += total;
+        for (int w = 0; w < PA_NW; w++) {
+            if (w < warp) upto += s_scan[w];
+            total += s_scan[w];
+        }
+    };
+    for (int s0 = 0; s0 < a.n_seq; s0 += PA_NT) scan(s0, blockIdx.x == 0);
+    const long long all = total, share = max((all + gridDim.x - 1) / gridDim.x, (long long)(A.min_units));
+    const long long begin = share * blockIdx.x, end = min(all, begin + share);
+    if (tid == 0) A.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (begin >= all) return;
+    total = 0;
+    for (int s0 = 0; s0 < a.n_seq && total <= begin; s0 += PA_NT) {  // the sequence that holds `begin`
+        if (a.n_seq > PA_NT)
+            scan(s0, false);
+        else
+            total = all;
+        if (mine > 0 && upto - mine <= begin && begin < upto) {
             s_seq = s0 + tid;
-            s_start = v - mine;
+            s_start = upto - mine;
         }
-        run += s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
-        __syncthreads();
-        if (run > begin) break;
     }
+    __syncthreads();
     int seq = s_seq;
     long long seq_at = s_start;
     const T* kp = static_cast<const T*>(a.k);
@@ -360,8 +363,8 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
     for (long long at = begin; at < end && seq < a.n_seq;) {
         const Seq sq = paged_seq(a, seq, false);
         const Units un = units_of(sq, A.window, A.n_sink, UNIT);
-        const int nu = un.n(), nrt = (sq.q * a.grp + RT - 1) / RT;
-        const long long here = (long long)nu * nrt * a.n_kv;
+        const int nu = un.n(), ticks = A.whole ? 1 : nu, nrt = (sq.q * a.grp + RT - 1) / RT;
+        const long long here = (long long)ticks * nrt * a.n_kv;
         const bool takes = step_takes(A, sq);
         if (!takes || at >= seq_at + here) {
             if (takes) seq_at += here;
@@ -369,11 +372,71 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
             continue;
         }
         const long long idx = at - seq_at;
-        const int item = (int)(idx / nu), u0 = (int)(idx - (long long)item * nu);
+        const int item = (int)(idx / ticks), u0 = (int)(idx - (long long)item * ticks);
         const int kvh = item / nrt, rt = item - kvh * nrt;
-        const int n_it = (int)min((long long)(nu - u0), end - at);
+        const int n_it = A.whole ? nu : (int)min((long long)(nu - u0), end - at);
         // ---- the row tile: rows r0 .. of (token, q head of the group)
         const int r0 = rt * RT, n_rows = min(RT, sq.q * a.grp - r0), p_first = sq.kv - sq.q;
+        const int lim_max = p_first + (r0 + n_rows - 1) / a.grp, first_pos = p_first + r0 / a.grp;
+        const int low_min = A.window > 0 ? first_pos - A.window + 1 : 0;
+        const int lim_min = first_pos, low_max = A.window > 0 ? lim_max - A.window + 1 : 0;
+        auto any = [&](int j) { return j <= lim_max && (j >= low_min || j < A.n_sink); };
+
+        // ---- k and v of a step: page ids of 32 steps at a time, one per lane, the next 32 fetched ahead
+        auto fetch_ids = [&](int it) {
+            const int i = it + lane;
+            int id = -1;
+            if (i < n_it) {
+                const int p = un.unit(u0 + i) * UNIT + warp * STEP;
+                if (any(p) || any(p + STEP - 1) || (p < low_min && p + STEP > low_min && low_min <= lim_max)) {
+                    id = a.table[(size_t)seq * a.table_ld + p / a.page];
+                    if ((unsigned)id >= (unsigned)a.n_pages) {
+                        paged_flag(a.status);
+                        id = -1;
+                    }
+                }
+            }
+            return id;
+        };
+        int ids = fetch_ids(0), ids_next = n_it > 32 ? fetch_ids(32) : -1;
+        uint32_t live = 0;  // steps in the ring (bit: it mod 32) whose page is one of the pool's
+        const uint32_t ring = smem_u32(S.ring[warp]);
+        constexpr int RPP = 32 / (NB * 8);  // rows that a warp's copies of one instruction cover
+        const uint32_t lane_at = ((lane % (NB * 8)) >> 3) * BLK + lane / (NB * 8) * 128 + (((lane & 7) ^ (lane / (NB * 8))) << 4);
+        auto load = [&](int it) {  // rows of positions that no row sees become zero: 0 * NaN is NaN
+            if (it < n_it) {
+                if ((it & 31) == 0 && it > 0) {
+                    ids = ids_next;
+                    if (it + 32 < n_it) ids_next = fetch_ids(it + 32);
+                }
+                const int id = __shfl_sync(0xffffffffu, ids, it & 31), p = un.unit(u0 + it) * UNIT + warp * STEP;
+                live = id >= 0 ? live | 1u << (it & 31) : live & ~(1u << (it & 31));
+                const size_t at = (size_t)(id >= 0 ? id : 0) * a.page_stride + ((size_t)kvh * a.page + p % a.page) * HD;
+                const uint8_t* ks = reinterpret_cast<const uint8_t*>(kp + at) + 16 * lane;
+                const uint8_t* vs = reinterpret_cast<const uint8_t*>(vp + at) + 16 * lane;
+                const uint32_t slot = ring + (it % PA_NS) * 2 * AttnSmem<T, HD, STACK>::TILE;
+                // rows lane / (8 NB) + RPP j: the exchange of chunks splits into the lane's and j's part
+                if (id >= 0 && p + STEP - 1 <= lim_max && (p >= low_min || p + STEP <= A.n_sink)) {
+#pragma unroll
+                    for (int j = 0; j < CPL; j++) {
+                        const uint32_t d = (slot + lane_at + j * RPP * 128) ^ (((j * RPP) & 7) << 4);
+                        cp_async16(d, ks + 512 * j);
+                        cp_async16(d + AttnSmem<T, HD, STACK>::TILE, vs + 512 * j);
+                    }
+                } else {
+#pragma unroll 2
+                    for (int j = 0; j < CPL; j++) {
+                        const uint32_t d = (slot + lane_at + j * RPP * 128) ^ (((j * RPP) & 7) << 4);
+                        const int n = id >= 0 && any(p + lane / (NB * 8) + j * RPP) ? 16 : 0;
+                        cp_async16_or_zero(d, ks + 512 * j, n);
+                        cp_async16_or_zero(d + AttnSmem<T, HD, STACK>::TILE, vs + 512 * j, n);
+                    }
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < PA_NS - 1; i++) load(i);
         auto q_row = [&](int r) {
             const int rr = r0 + r, tok = rr / a.grp;
             return A.q + (size_t)(sq.q0 + tok) * A.ldq + (size_t)(kvh * a.grp + (rr - tok * a.grp)) * HD;
@@ -443,55 +506,6 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
             }
         }
         if (!STACK) __syncthreads();
-        const int lim_max = p_first + (r0 + n_rows - 1) / a.grp, first_pos = p_first + r0 / a.grp;
-        const int low_min = A.window > 0 ? first_pos - A.window + 1 : 0;
-        const int lim_min = first_pos, low_max = A.window > 0 ? lim_max - A.window + 1 : 0;
-        auto any = [&](int j) { return j <= lim_max && (j >= low_min || j < A.n_sink); };
-
-        // ---- k and v of a step: page ids of 32 steps at a time, one per lane, the next 32 fetched ahead
-        auto fetch_ids = [&](int it) {
-            const int i = it + lane;
-            int id = -1;
-            if (i < n_it) {
-                const int p = un.unit(u0 + i) * UNIT + warp * STEP;
-                if (any(p) || any(p + STEP - 1) || (p < low_min && p + STEP > low_min && low_min <= lim_max)) {
-                    id = a.table[(size_t)seq * a.table_ld + p / a.page];
-                    if ((unsigned)id >= (unsigned)a.n_pages) {
-                        paged_flag(a.status);
-                        id = -1;
-                    }
-                }
-            }
-            return id;
-        };
-        int ids = fetch_ids(0), ids_next = n_it > 32 ? fetch_ids(32) : -1;
-        uint32_t live = 0;  // steps in the ring (bit: it mod 32) whose page is one of the pool's
-        const uint32_t ring = smem_u32(S.ring[warp]);
-        constexpr int RPP = 32 / (NB * 8);  // rows that a warp's copies of one instruction cover
-        const uint32_t lane_at = ((lane % (NB * 8)) >> 3) * BLK + lane / (NB * 8) * 128 + (((lane & 7) ^ (lane / (NB * 8))) << 4);
-        auto load = [&](int it) {  // rows of positions that no row sees become zero: 0 * NaN is NaN
-            if (it < n_it) {
-                if ((it & 31) == 0 && it > 0) {
-                    ids = ids_next;
-                    if (it + 32 < n_it) ids_next = fetch_ids(it + 32);
-                }
-                const int id = __shfl_sync(0xffffffffu, ids, it & 31), p = un.unit(u0 + it) * UNIT + warp * STEP;
-                live = id >= 0 ? live | 1u << (it & 31) : live & ~(1u << (it & 31));
-                const size_t at = (size_t)(id >= 0 ? id : 0) * a.page_stride + ((size_t)kvh * a.page + p % a.page) * HD;
-                const uint8_t* ks = reinterpret_cast<const uint8_t*>(kp + at) + 16 * lane;
-                const uint8_t* vs = reinterpret_cast<const uint8_t*>(vp + at) + 16 * lane;
-                const uint32_t slot = ring + (it % PA_NS) * 2 * AttnSmem<T, HD, STACK>::TILE;
-                const bool full = id >= 0 && p + STEP - 1 <= lim_max && (p >= low_min || p + STEP <= A.n_sink);
-#pragma unroll
-                for (int j = 0; j < CPL; j++) {  // rows lane / (8 NB) + RPP j: the exchange of chunks splits into lane's and j's part
-                    const uint32_t d = (slot + lane_at + j * RPP * 128) ^ (((j * RPP) & 7) << 4);
-                    const int n = full || (id >= 0 && any(p + lane / (NB * 8) + j * RPP)) ? 16 : 0;
-                    cp_async16_or_zero(d, ks + 512 * j, n);
-                    cp_async16_or_zero(d + AttnSmem<T, HD, STACK>::TILE, vs + 512 * j, n);
-                }
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
         float o[NT][2 * NR];
 #pragma unroll
         for (int n = 0; n < NT; n++)
@@ -503,8 +517,6 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
             m[i] = -INFINITY;
             l[i] = 0.f;
         }
-#pragma unroll
-        for (int i = 0; i < PA_NS - 1; i++) load(i);
         for (int it = 0; it < n_it; it++) {
             asm volatile("cp.async.wait_group %0;" ::"n"(PA_NS - 2) : "memory");
             __syncwarp();  // every lane's copies have landed, and every lane is done with the tile that comes free
@@ -559,18 +571,28 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
             float sv[NR][PT];
             float mx[NR];
 #pragma unroll
-            for (int i = 0; i < NR; i++) {
-                mx[i] = -INFINITY;
+            for (int i = 0; i < NR; i++)
 #pragma unroll
                 for (int j = 0; j < PT; j++) {
-                    const int pos = p_cur + 8 * (j >> 1) + 2 * t + (j & 1);
                     const int e = (j & 1) + 2 * i;
-                    float raw = sacc[j >> 1][e] + slow[j >> 1][e];
+                    float raw = H16 && STACK ? sacc[j >> 1][e] : sacc[j >> 1][e] + slow[j >> 1][e];
                     if (STACK) raw += sacc[j >> 1][e + 2];
-                    const bool see = plain || (pos <= lim[i] && (pos >= low[i] || pos < A.n_sink));
-                    sv[i][j] = see ? raw * cs[i] : -INFINITY;
-                    mx[i] = fmaxf(mx[i], sv[i][j]);
+                    sv[i][j] = raw * cs[i];
                 }
+            if (!plain) {
+#pragma unroll
+                for (int i = 0; i < NR; i++)
+#pragma unroll
+                    for (int j = 0; j < PT; j++) {
+                        const int pos = p_cur + 8 * (j >> 1) + 2 * t + (j & 1);
+                        if (!(pos <= lim[i] && (pos >= low[i] || pos < A.n_sink))) sv[i][j] = -INFINITY;
+                    }
+            }
+#pragma unroll
+            for (int i = 0; i < NR; i++) {
+                mx[i] = sv[i][0];
+#pragma unroll
+                for (int j = 1; j < PT; j++) mx[i] = fmaxf(mx[i], sv[i][j]);
                 mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
                 mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
                 mx[i] = fmaxf(mx[i], m[i]);
@@ -716,7 +738,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
             A.meta[blockIdx.x] = make_int4((int)((tile_end - 1) / share) - blockIdx.x, seq, kvh, rt);
         }
         __syncthreads();
-        at += n_it;
+        at += A.whole ? 1 : n_it;
     }
 }
 
@@ -793,24 +815,39 @@ __global__ void __launch_bounds__(PM_NT) k_paged_merge(PagedAttnArgs A, MergeSha
                                4 * lane) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
+// Up to this many positions a row tile is one block's work: cutting it would save less than the joining launch costs.
+constexpr int WHOLE_KV = 512;
+// Blocks of the step kernel that an SM holds: by registers and by the rings' shared memory.
 template <typename T, int HD, bool STACK>
-cudaError_t attn_go(const PagedAttnArgs& A, cudaStream_t st) {
+constexpr int step_blocks() {
+    return sizeof(T) == 2 ? 3 : 2;
+}
+constexpr int STEP_BLOCKS_MAX = 3;
+int step_grid_max() { return STEP_BLOCKS_MAX * sm_count(); }
+
+template <typename T, int HD, bool STACK>
+cudaError_t attn_go(PagedAttnArgs A, int max_kv, cudaStream_t st) {
     constexpr int RT = STACK ? 8 : 16;
     cudaError_t e = smem_limit<AttnSmem<T, HD, STACK>>(k_paged_attn<T, HD, STACK>, sizeof(AttnSmem<T, HD, STACK>));
     if (e != cudaSuccess) return e;
+    A.grid = step_blocks<T, HD, STACK>() * sm_count();
+    A.whole = max_kv <= WHOLE_KV;
+    A.min_units = A.whole ? 1 : 4;
     e = launch_pdl(k_paged_attn<T, HD, STACK>, dim3(A.grid), dim3(PA_NT), sizeof(AttnSmem<T, HD, STACK>), st, A);
-    if (e != cudaSuccess) return e;
-    return launch_pdl(k_paged_merge<HD, true>, dim3(A.grid, RT), dim3(PM_NT), 0, st, A, MergeShape{RT, 16});
+    if (e != cudaSuccess || A.whole) return e;
+    // few tiles are cut often: their records dealt over blocks; many tiles, each cut once or twice: a row to a group
+    if ((long long)A.c.n_seq * A.c.n_kv * 8 <= A.grid)
+        return launch_pdl(k_paged_merge<HD, true>, dim3(A.grid, RT), dim3(PM_NT), 0, st, A, MergeShape{RT, 16});
+    return launch_pdl(k_paged_merge<HD, false>, dim3(A.grid, (RT * HD / 4 + PM_NT - 1) / PM_NT), dim3(PM_NT), 0, st, A, MergeShape{RT, 16});
 }
 template <typename T, int HD>
-cudaError_t attn_rows(const PagedAttnArgs& A, bool stack, cudaStream_t st) {
-    return stack ? attn_go<T, HD, true>(A, st) : attn_go<T, HD, false>(A, st);
+cudaError_t attn_rows(const PagedAttnArgs& A, bool stack, int max_kv, cudaStream_t st) {
+    return stack ? attn_go<T, HD, true>(A, max_kv, st) : attn_go<T, HD, false>(A, max_kv, st);
 }
 
-int attn_grid() { return 2 * sm_count(); }
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 size_t step_ws_bytes(int hd) {
-    return align256((size_t)attn_grid() * sizeof(int4)) + align256((size_t)attn_grid() * 2 * part_floats(hd) * sizeof(float));
+    return align256((size_t)step_grid_max() * sizeof(int4)) + align256((size_t)step_grid_max() * 2 * part_floats(hd) * sizeof(float));
 }
 size_t tc_ws_bytes(int hd) {
     return align256((size_t)paged_tc_grid() * sizeof(int4)) + (size_t)paged_tc_grid() * 2 * 256 * (hd + 2) * sizeof(float);
@@ -829,7 +866,6 @@ size_t paged_attn_ws_bytes(int type, int hd, int grp, int max_q) {
 }
 
 cudaError_t launch_paged_attention(int type, int hd, int max_q, int max_kv, PagedAttnArgs A, void* ws, cudaStream_t st) {
-    (void)max_kv;
     const bool tc = tc_call(type, A.c.grp, max_q);
     A.rows_min = 0;
     A.rows_max = 0x7fffffff;
@@ -846,11 +882,10 @@ cudaError_t launch_paged_attention(int type, int hd, int max_q, int max_kv, Page
                       : launch_pdl(k_paged_merge<64, false>, dim3(A.grid, 256 / (PM_NT / 16)), dim3(PM_NT), 0, st, A, ms);
         if (e != cudaSuccess || A.c.n_seq == 1) return e;
     }
-    A.min_units = 4;
-    carve(A, attn_grid(), ws);
+    carve(A, step_grid_max(), ws);
     const bool stack = max_q * A.c.grp <= 8;
-    if (type == T_F16) return hd == 128 ? attn_rows<__half, 128>(A, stack, st) : attn_rows<__half, 64>(A, stack, st);
-    return hd == 128 ? attn_rows<float, 128>(A, stack, st) : attn_rows<float, 64>(A, stack, st);
+    if (type == T_F16) return hd == 128 ? attn_rows<__half, 128>(A, stack, max_kv, st) : attn_rows<__half, 64>(A, stack, max_kv, st);
+    return hd == 128 ? attn_rows<float, 128>(A, stack, max_kv, st) : attn_rows<float, 64>(A, stack, max_kv, st);
 }
 
 cudaError_t launch_rope_append(int type, int hd, const PagedArgs& a, const EahmmfRope& rope, const float* qkv, int ld,

@@ -60,6 +60,7 @@ struct PagedAttnArgs {
     int window, n_sink;  // window 0: every earlier position is visible
     int grid;            // blocks of the split launch, also the records of `part`
     int min_units;       // least share of a block
+    bool whole;          // step kernel: row tiles are not cut
     int rows_min, rows_max;  // sequences of more rows (tokens x q heads of a kv head) than rows_min go to the chunk
                              // kernel, of at most rows_max to the step kernel
     float* part;         // [grid][2] partial results
