@@ -21,9 +21,11 @@ namespace {
 // rotary positions + append
 // ------------------------------------------------------------------------------------------------
 // Row r of sequence s is at position p = kv - q + (r - q0). Each q and k head x: x <- x / sqrt(mean x^2 + eps) * w
-// when weights are given; then for pair i < n_rot / 2 with angle p * inv_freq[i] (the product and its sine and cosine
-// in 64 bits: at p = 1e5 a 32-bit product is off by 4e-3 rad):
+// when weights are given; then for pair i < n_rot / 2 with angle p * inv_freq[i]:
 //   (a, b) <- (a cos - b sin, a sin + b cos),  (a, b) = (x[i], x[i + n_rot/2]) or (x[2i], x[2i + 1]).
+// The angle and what is left of it after whole turns are in 64 bits (at p = 1e5 a 32-bit product is off by 4e-3 rad), its
+// sine and cosine in 32 bits, with the part of the remainder that 32 bits lose added to first order: within 2^-23. A
+// sincos in 64 bits cost 1.1 us of a step's 8 us and a seventh of a prompt's rate.
 // Bytes: 4 hd (n_head + 2 n_kv) in, 4 hd n_head + 2 hd n_kv es out per row; nothing is read twice.
 constexpr int AP_NT = 256;
 constexpr int AP_PF = 4;  // head vectors a thread loads before it needs the row's sequence
@@ -73,9 +75,12 @@ __global__ void __launch_bounds__(AP_NT) k_rope_append(PagedArgs a, EahmmfRope r
     }
     const int id = a.table[(size_t)seq * a.table_ld + pos / a.page];
     if (tid < half) {
-        double sn, co;
-        sincos((double)pos * (double)fr, &sn, &co);
-        cs[tid] = make_float2((float)co * rope.mscale, (float)sn * rope.mscale);
+        const double ang = (double)pos * (double)fr, turns = rint(ang * 0.15915494309189535);
+        const double rest = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, ang));  // 2 pi in two parts
+        const float r = (float)rest, lo = (float)(rest - (double)r);
+        float sn, co;
+        sincosf(r, &sn, &co);
+        cs[tid] = make_float2(fmaf(-sn, lo, co) * rope.mscale, fmaf(co, lo, sn) * rope.mscale);
     }
     const bool page_ok = (unsigned)id < (unsigned)a.n_pages;
     if (!page_ok && tid == 0) paged_flag(a.status);
@@ -735,7 +740,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
         }
         if (!whole && u0 == 0 && tid == 0) {  // the blocks after this one hold the rest of the tile
             const long long tile_end = at + nu;
-            A.meta[blockIdx.x] = make_int4((int)((tile_end - 1) / share) - blockIdx.x, seq, kvh, rt);
+            A.meta[blockIdx.x] = make_int4(((int)((tile_end - 1) / share) - blockIdx.x) | n_rows << 16, sq.q0, kvh, r0);
         }
         __syncthreads();
         at += A.whole ? 1 : n_it;
@@ -743,15 +748,12 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
 }
 
 // Joins the records of the row tiles that the split cut. Block (b, y) takes rows of the tile that block b of the
-// attention began and left to the blocks after it (meta: how many, sequence, kv head, row tile): with ONE one row, its
-// records dealt over the block (a long context is cut often), else a row to each group of hd / 4 threads.
+// attention began and left to the blocks after it (meta: how many, with the tile's rows above bit 16; output row of the
+// sequence's first token; kv head; the tile's first row): with ONE one row, its records dealt over the block (a long context is cut often), else a row to each
+// group of hd / 4 threads. cap: rows of a record, o [cap][hd], m [cap], sum [cap].
 constexpr int PM_NT = 256;
-struct MergeShape {
-    int tile_rows;  // rows from one row tile to the next
-    int cap;        // rows of a record: o [cap][hd], m [cap], sum [cap]
-};
 template <int HD, bool ONE>
-__global__ void __launch_bounds__(PM_NT) k_paged_merge(PagedAttnArgs A, MergeShape ms) {
+__global__ void __launch_bounds__(PM_NT) k_paged_merge(PagedAttnArgs A, int cap) {
     constexpr int LN = HD / 4, G = PM_NT / LN;
     __shared__ __align__(16) float so[ONE ? G : 1][HD];
     __shared__ float sm[G], sl[G];
@@ -761,28 +763,39 @@ __global__ void __launch_bounds__(PM_NT) k_paged_merge(PagedAttnArgs A, MergeSha
     pdl_trigger();
     const int4 me = A.meta[b];
     if (me.x == 0) return;
-    const Seq sq = paged_seq(A.c, me.y, false);
-    const int rr = me.w * ms.tile_rows + r;
-    if (r >= ms.tile_rows || rr >= sq.q * A.c.grp) return;
+    const int follow = me.x & 0xffff;
+    if (r >= me.x >> 16) return;
+    const int rr = me.w + r;
     float m = -INFINITY, l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int j = ONE ? grp : 0; j <= me.x; j += step) {
-        const float* rec = A.part + ((size_t)(b + j) * 2 + (j == 0 ? 1 : 0)) * ((size_t)ms.cap * (HD + 2));
-        const float mj = rec[ms.cap * HD + r], lj = rec[ms.cap * HD + ms.cap + r];
-        const float4 f = reinterpret_cast<const float4*>(rec)[r * LN + lane];
-        const float mn = fmaxf(m, mj);
-        if (mn == -INFINITY) {  // nothing seen so far (a NaN sum stays one)
-            l += lj;
-            continue;
+    constexpr int N = 4;  // records in flight
+    for (int j0 = ONE ? grp : 0; j0 <= follow; j0 += N * step) {
+        float mj[N], lj[N];
+        float4 f[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int j = j0 + i * step;
+            const float* rec = A.part + ((size_t)(b + min(j, follow)) * 2 + (j == 0 ? 1 : 0)) * ((size_t)cap * (HD + 2));
+            mj[i] = rec[cap * HD + r];
+            lj[i] = rec[cap * HD + cap + r];
+            f[i] = reinterpret_cast<const float4*>(rec)[r * LN + lane];
         }
-        const float ea = exp2f(m - mn), eb_ = exp2f(mj - mn);
-        m = mn;
-        l = fmaf(l, ea, lj * eb_);
-        o.x = fmaf(o.x, ea, f.x * eb_);
-        o.y = fmaf(o.y, ea, f.y * eb_);
-        o.z = fmaf(o.z, ea, f.z * eb_);
-        o.w = fmaf(o.w, ea, f.w * eb_);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (j0 + i * step > follow) break;
+            const float mn = fmaxf(m, mj[i]);
+            if (mn == -INFINITY) {  // nothing seen so far (a NaN sum stays one)
+                l += lj[i];
+                continue;
+            }
+            const float ea = ex2(m - mn), eb_ = ex2(mj[i] - mn);
+            m = mn;
+            l = fmaf(l, ea, lj[i] * eb_);
+            o.x = fmaf(o.x, ea, f[i].x * eb_);
+            o.y = fmaf(o.y, ea, f[i].y * eb_);
+            o.z = fmaf(o.z, ea, f[i].z * eb_);
+            o.w = fmaf(o.w, ea, f[i].w * eb_);
+        }
     }
     float L = l;
     if (ONE) {
@@ -811,7 +824,7 @@ __global__ void __launch_bounds__(PM_NT) k_paged_merge(PagedAttnArgs A, MergeSha
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const int tok = rr / A.c.grp;
-    *reinterpret_cast<float4*>(A.out + (size_t)(sq.q0 + tok) * A.ldo + (size_t)(me.z * A.c.grp + rr - tok * A.c.grp) * HD +
+    *reinterpret_cast<float4*>(A.out + (size_t)(me.y + tok) * A.ldo + (size_t)(me.z * A.c.grp + rr - tok * A.c.grp) * HD +
                                4 * lane) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
@@ -837,8 +850,8 @@ cudaError_t attn_go(PagedAttnArgs A, int max_kv, cudaStream_t st) {
     if (e != cudaSuccess || A.whole) return e;
     // few tiles are cut often: their records dealt over blocks; many tiles, each cut once or twice: a row to a group
     if ((long long)A.c.n_seq * A.c.n_kv * 8 <= A.grid)
-        return launch_pdl(k_paged_merge<HD, true>, dim3(A.grid, RT), dim3(PM_NT), 0, st, A, MergeShape{RT, 16});
-    return launch_pdl(k_paged_merge<HD, false>, dim3(A.grid, (RT * HD / 4 + PM_NT - 1) / PM_NT), dim3(PM_NT), 0, st, A, MergeShape{RT, 16});
+        return launch_pdl(k_paged_merge<HD, true>, dim3(A.grid, RT), dim3(PM_NT), 0, st, A, 16);
+    return launch_pdl(k_paged_merge<HD, false>, dim3(A.grid, (RT * HD / 4 + PM_NT - 1) / PM_NT), dim3(PM_NT), 0, st, A, 16);
 }
 template <typename T, int HD>
 cudaError_t attn_rows(const PagedAttnArgs& A, bool stack, int max_kv, cudaStream_t st) {
@@ -877,9 +890,8 @@ cudaError_t launch_paged_attention(int type, int hd, int max_q, int max_kv, Page
         carve(A, paged_tc_grid(), static_cast<uint8_t*>(ws) + step_ws_bytes(hd));
         cudaError_t e = launch_paged_attn_tc(hd, A, st);
         if (e != cudaSuccess) return e;
-        const MergeShape ms{2 * (128 / A.c.grp) * A.c.grp, 256};
-        e = hd == 128 ? launch_pdl(k_paged_merge<128, false>, dim3(A.grid, 256 / (PM_NT / 32)), dim3(PM_NT), 0, st, A, ms)
-                      : launch_pdl(k_paged_merge<64, false>, dim3(A.grid, 256 / (PM_NT / 16)), dim3(PM_NT), 0, st, A, ms);
+        e = hd == 128 ? launch_pdl(k_paged_merge<128, false>, dim3(A.grid, 256 / (PM_NT / 32)), dim3(PM_NT), 0, st, A, 256)
+                      : launch_pdl(k_paged_merge<64, false>, dim3(A.grid, 256 / (PM_NT / 16)), dim3(PM_NT), 0, st, A, 256);
         if (e != cudaSuccess || A.c.n_seq == 1) return e;
     }
     carve(A, step_grid_max(), ws);

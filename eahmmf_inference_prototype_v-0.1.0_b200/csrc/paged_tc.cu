@@ -510,7 +510,8 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
             const bool whole = w.u0 == 0 && w.n_it == w.nu;
             if (!whole && w.u0 == 0 && tid == 0) {
                 const long long tile_end = w.at + (w.nu - w.n_it);
-                A.meta[blockIdx.x] = make_int4((int)((tile_end - 1) / share) - blockIdx.x, w.seq, w.kvh, w.pair);
+                A.meta[blockIdx.x] = make_int4(((int)((tile_end - 1) / share) - blockIdx.x) | (w.pr.t1 - w.pr.t0) * a.grp << 16, w.sq.q0, w.kvh,
+                                                w.pr.t0 * a.grp);
             }
             // ---- the warp's rows through shared memory (their q is read), so that a row leaves as one run: to the output, or to
             // this block's record (rows in (token, head) order: the two tiles' rows follow each other)
