@@ -865,7 +865,7 @@ size_t step_ws_bytes(int hd) {
 size_t tc_ws_bytes(int hd) {
     return align256((size_t)paged_tc_grid() * sizeof(int4)) + (size_t)paged_tc_grid() * 2 * 256 * (hd + 2) * sizeof(float);
 }
-bool tc_call(int type, int grp, int max_q) { return type == T_F16 && max_q * grp > STEP_ROWS; }
+bool tc_call(int grp, int max_q) { return (long long)max_q * grp > STEP_ROWS; }
 
 void carve(PagedAttnArgs& A, int grid, void* ws) {
     A.grid = grid;
@@ -875,11 +875,11 @@ void carve(PagedAttnArgs& A, int grid, void* ws) {
 }  // namespace
 
 size_t paged_attn_ws_bytes(int type, int hd, int grp, int max_q) {
-    return step_ws_bytes(hd) + (tc_call(type, grp, max_q) ? tc_ws_bytes(hd) : 0);
+    return step_ws_bytes(hd) + (tc_call(grp, max_q) ? tc_ws_bytes(hd) : 0);
 }
 
 cudaError_t launch_paged_attention(int type, int hd, int max_q, int max_kv, PagedAttnArgs A, void* ws, cudaStream_t st) {
-    const bool tc = tc_call(type, A.c.grp, max_q);
+    const bool tc = tc_call(A.c.grp, max_q);
     A.rows_min = 0;
     A.rows_max = 0x7fffffff;
     if (tc) {
@@ -888,7 +888,7 @@ cudaError_t launch_paged_attention(int type, int hd, int max_q, int max_kv, Page
         A.rows_max = A.rows_min;
         A.min_units = 1;
         carve(A, paged_tc_grid(), static_cast<uint8_t*>(ws) + step_ws_bytes(hd));
-        cudaError_t e = launch_paged_attn_tc(hd, A, st);
+        cudaError_t e = launch_paged_attn_tc(type, hd, A, st);
         if (e != cudaSuccess) return e;
         e = hd == 128 ? launch_pdl(k_paged_merge<128, false>, dim3(A.grid, 256 / (PM_NT / 32)), dim3(PM_NT), 0, st, A, 256)
                       : launch_pdl(k_paged_merge<64, false>, dim3(A.grid, 256 / (PM_NT / 16)), dim3(PM_NT), 0, st, A, 256);

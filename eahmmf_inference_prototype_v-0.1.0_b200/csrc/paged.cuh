@@ -71,7 +71,7 @@ size_t paged_attn_ws_bytes(int type, int hd, int grp, int max_q);
 cudaError_t launch_paged_attention(int type, int hd, int max_q, int max_kv, PagedAttnArgs a, void* ws, cudaStream_t st);
 
 int paged_tc_grid();  // blocks of the chunk kernel
-cudaError_t launch_paged_attn_tc(int hd, const PagedAttnArgs& A, cudaStream_t st);
+cudaError_t launch_paged_attn_tc(int type, int hd, const PagedAttnArgs& A, cudaStream_t st);
 
 // Raises a kernel's dynamic shared-memory limit, once on each device; Tag: a type of the kernel's own.
 template <typename Tag, typename Kern>

@@ -28,35 +28,42 @@
 namespace eb {
 namespace {
 
-constexpr int TC_NT = 384;
-// Registers: 384 threads are launched with 168 each; a softmax thread holds its row's hd sums beside its scores. Shares
-// after the split: 2 x 128 x 208 + 128 x 88 = 384 x 168, the launch's own total (checked before the launch).
-constexpr int REGS_LAUNCH = 168;
-#define EB_REGS_MORE() asm volatile("setmaxnreg.inc.sync.aligned.u32 208;")
-#define EB_REGS_LESS() asm volatile("setmaxnreg.dec.sync.aligned.u32 88;")
 constexpr int UNIT = 128;  // positions of a unit
 constexpr int MROWS = 128;
 constexpr int VALID_RING = 8;
 
-template <int HD>
+// Registers: all threads are launched with REGS; a softmax thread holds its row's hd sums beside its scores, so its warps
+// take registers over from the others: 16-bit pools 2 x 128 x 208 + 128 x 88 = 384 x 168, 32-bit pools 128 x 208 + 256 x 104 +
+// 128 x 96 = 512 x 128, the launch's own totals (checked before the launch).
+template <int HD, bool F32>
 struct Tc {
+    static constexpr int NM = F32 ? 1 : 2;               // row tiles that share the k and v tiles
+    static constexpr int PARTS = F32 ? 2 : 1;            // 11-bit parts of a pool element
     static constexpr int HALVES = HD / 64;               // 128-byte column blocks of an operand tile
     static constexpr int BLK = 128 * 128;                // bytes of a column block of 128 rows
     static constexpr int TILE = HALVES * BLK;            // bytes of a 128 x hd operand tile
-    static constexpr int NST = HD == 128 ? 3 : 8;        // tiles of k and v in flight
-    static constexpr int Q_BYTES = 2 * 2 * TILE;         // two row tiles, two parts
-    static constexpr int SMEM = 1024 + Q_BYTES + NST * TILE + 512;
+    static constexpr int STAGE = PARTS * TILE;           // of a k or v tile in all its parts: hi, lo
+    static constexpr int NST = F32 ? 2 : HD == 128 ? 3 : 8;  // tiles of k and v in flight
+    static constexpr int Q_BYTES = NM * 2 * TILE;
+    static constexpr int SMEM = 1024 + Q_BYTES + NST * STAGE + 1024;
     static constexpr uint32_t O_COL = 384;               // tensor memory: three S, one O
     static constexpr uint32_t COLS = 512;
+    static constexpr int W_LOAD = 4 * NM, N_LOAD = F32 ? 8 : 1;  // first warp that brings k and v, how many do
+    static constexpr int W_QK = F32 ? 12 : 9, W_PV = W_QK + 1;
+    static constexpr int NT = F32 ? 512 : 384;
+    static constexpr int REGS = F32 ? 128 : 168, REGS_SOFTMAX = 208, REGS_LOAD = F32 ? 104 : 88, REGS_ISSUE = F32 ? 96 : 88;
 };
+static_assert(128 * (2 * 208 + 88) == 384 * 168 && 128 * (208 + 2 * 104 + 96) == 512 * 128, "register shares");
 struct Bars {
     uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2], p_full[2], pv_done[2], s_free[3], o_free;
-    uint32_t valid[VALID_RING];  // by unit: which boxes lie in pages of the pool
+    uint32_t valid[VALID_RING];                     // by unit: which boxes lie in pages of the pool
+    float k_back[VALID_RING], v_back[VALID_RING];   // 32-bit pools, by unit: what undoes the scale of the k (v) tile
+    float wmax[2][8];
     uint32_t tmem;
     int seq;
-    long long start, scan[TC_NT / 32];
+    long long start, scan[16];
 };
-static_assert(sizeof(Bars) <= 512, "");
+static_assert(sizeof(Bars) <= 1024, "");
 
 // Bounded wait, as mbar_wait_bounded, without its suspend hint: these waits last a few hundred cycles.
 __device__ __forceinline__ bool bar_try(uint64_t* bar, uint32_t parity) {
@@ -183,16 +190,16 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 
 // ticks: one for a unit and TILE_TICKS for a pair's q and output.
 constexpr int TILE_TICKS = 3;
 struct Pair {
-    int t0, t1;                   // tokens of the pair
+    int t0, t1;                   // tokens of the pair (32-bit pools: of one row tile)
     int low_min, lim_max;         // positions that some row sees: [low_min, lim_max] and the first n_sink
     int us, uw, ue;               // their units
     __device__ __forceinline__ int n() const { return max(1, us + ue - uw); }
     __device__ __forceinline__ int unit(int i) const { return i < us ? i : uw + (i - us); }
 };
-__device__ __forceinline__ Pair pair_of(const PagedAttnArgs& A, const Seq& sq, int pair, int tpt) {
+__device__ __forceinline__ Pair pair_of(const PagedAttnArgs& A, const Seq& sq, int pair, int tok) {
     Pair p;
-    p.t0 = pair * 2 * tpt;
-    p.t1 = min(sq.q, p.t0 + 2 * tpt);
+    p.t0 = pair * tok;
+    p.t1 = min(sq.q, p.t0 + tok);
     const int first = sq.kv - sq.q + p.t0;
     p.lim_max = sq.kv - sq.q + p.t1 - 1;
     p.low_min = A.window > 0 ? first - A.window + 1 : 0;
@@ -205,25 +212,25 @@ __device__ __forceinline__ bool tc_takes(const PagedAttnArgs& A, const Seq& sq) 
 
 struct Walk {
     const PagedAttnArgs& A;
-    int tpt, seq, pair = 0;
+    int tok, seq, pair = 0;  // tok: tokens of a pair
     long long at, end, base;
     Seq sq;
     Pair pr;
     int kvh, u0, n_it, nu;
-    __device__ Walk(const PagedAttnArgs& A_, int tpt_, int seq_, long long base_, long long at_, long long end_)
-        : A(A_), tpt(tpt_), seq(seq_), at(at_), end(end_), base(base_) {
+    __device__ Walk(const PagedAttnArgs& A_, int tok_, int seq_, long long base_, long long at_, long long end_)
+        : A(A_), tok(tok_), seq(seq_), at(at_), end(end_), base(base_) {
         sq.q = 0;
     }
     __device__ bool next() {
         while (at < end) {
             if (seq >= A.c.n_seq) return false;
             sq = paged_seq(A.c, seq, false);
-            if (!tc_takes(A, sq) || pair * 2 * tpt >= sq.q) {
+            if (!tc_takes(A, sq) || pair * tok >= sq.q) {
                 seq++;
                 pair = 0;
                 continue;
             }
-            pr = pair_of(A, sq, pair, tpt);
+            pr = pair_of(A, sq, pair, tok);
             nu = pr.n();
             const int ticks = nu + TILE_TICKS;
             const long long w = (long long)ticks * A.c.n_kv;
@@ -244,34 +251,44 @@ struct Walk {
     }
 };
 
-template <int HD>
-__global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, const __grid_constant__ CUtensorMap kmap,
-                                                            const __grid_constant__ CUtensorMap vmap, int box) {
-    using C = Tc<HD>;
+template <int N>
+__device__ __forceinline__ void regs_more() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_less() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+template <int HD, bool F32>
+__global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnArgs A, const __grid_constant__ CUtensorMap kmap,
+                                                                      const __grid_constant__ CUtensorMap vmap, int box) {
+    using C = Tc<HD, F32>;
+    constexpr int TC_NT = C::NT;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sq_ = sm;                      // q: [tile][lo, hi][column block][128 rows][128 bytes]
     uint8_t* skv = sm + C::Q_BYTES;         // k, v tiles
-    Bars& B = *reinterpret_cast<Bars*>(skv + C::NST * C::TILE);
+    Bars& B = *reinterpret_cast<Bars*>(skv + C::NST * C::STAGE);
     const PagedArgs& a = A.c;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int tpt = MROWS / a.grp;  // tokens of a row tile
     if (tid == 0) {
         for (int i = 0; i < C::NST; i++) {
-            mbar_init(&B.kv_full[i], 1);
+            mbar_init(&B.kv_full[i], F32 ? 32 * C::N_LOAD : 1);
             mbar_init(&B.kv_empty[i], 1);
         }
         for (int m = 0; m < 2; m++) {
             mbar_init(&B.q_full[m], MROWS);
             mbar_init(&B.s_full[m], 2);
             mbar_init(&B.p_full[m], MROWS);
-            mbar_init(&B.pv_done[m], 1);
+            mbar_init(&B.pv_done[m], 2);
         }
         mbar_init(&B.o_free, MROWS);
         for (int b = 0; b < 3; b++) mbar_init(&B.s_free[b], 1);
         mbar_fence_init();
     }
-    if (warp == 8) tc_alloc(&B.tmem, C::COLS);
+    if (warp == C::W_LOAD) tc_alloc(&B.tmem, C::COLS);
     pdl_wait();
     pdl_trigger();
     // ---- this block's share
@@ -279,7 +296,7 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
         const Seq sq = paged_seq(a, s, flag);
         if (!tc_takes(A, sq)) return 0;
         long long n = 0;
-        for (int p = 0; p * 2 * tpt < sq.q; p++) n += pair_of(A, sq, p, tpt).n() + TILE_TICKS;
+        for (int p = 0; p * C::NM * tpt < sq.q; p++) n += pair_of(A, sq, p, C::NM * tpt).n() + TILE_TICKS;
         return n * a.n_kv;
     };
     long long total = 0, mine = 0;
@@ -326,11 +343,13 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = B.tmem;
-    Walk w(A, tpt, B.seq, B.start, begin, end);
+    Walk w(A, C::NM * tpt, B.seq, B.start, begin, end);
+    uint32_t ok_all = 1;
+    (void)ok_all;
     bool ok = true;  // a bounded wait that gives up ends the walk; the other warps' own waits then give up too
 
-    if (warp < 8) {
-        EB_REGS_MORE();
+    if (warp < 4 * C::NM) {
+        regs_more<C::REGS_SOFTMAX>();
         // ---------------------------------------------------------------- softmax and sums of row tile mt
         const int mt = warp >> 2, r = tid & 127;
         uint8_t* q_lo = sq_ + mt * 2 * C::TILE;
@@ -341,7 +360,7 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
         uint32_t n_s = 0, n_pv = 0, n_valid = 0, n_buf = 0;  // uses of the barriers, units and score buffers so far
         while (ok && w.next()) {
             const int tok = w.pr.t0 + mt * tpt + r / a.grp;
-            const int n_m = w.pr.t0 + tpt < w.pr.t1 ? 2 : 1;
+            const int n_m = !F32 && w.pr.t0 + tpt < w.pr.t1 ? 2 : 1;
             if (mt >= n_m) {  // the pair has one row tile
                 n_valid += w.n_it;
                 n_buf += w.n_it;
@@ -418,14 +437,17 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
                     ok = bar_wait(&B.pv_done[mt], n_pv++ & 1);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t al = f2(alpha, alpha);
+                    const float vb = F32 ? B.v_back[(n_valid - 1) % VALID_RING] : 1.f;
+                    const uint64_t al = f2(alpha, alpha), vb2 = f2(vb, vb);
 #pragma unroll
                     for (int c = 0; c < HD; c += 32) {
                         uint32_t o[32];
                         tm_ld32(o_tm + c, o);
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2)
-                            acc[(c + j) / 2] = fma2(acc[(c + j) / 2], al, f2(__uint_as_float(o[j]), __uint_as_float(o[j + 1])));
+                        for (int j = 0; j < 32; j += 2) {
+                            const uint64_t u = f2(__uint_as_float(o[j]), __uint_as_float(o[j + 1]));
+                            acc[(c + j) / 2] = F32 ? fma2(u, vb2, fma2(acc[(c + j) / 2], al, 0)) : fma2(acc[(c + j) / 2], al, u);
+                        }
                     }
                     tc_fence_before();
                     mbar_arrive(&B.o_free);
@@ -436,6 +458,7 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t s_tm = tmem + lanes + (n_buf % 3) * UNIT, valid = B.valid[n_valid % VALID_RING];
+                const float csu = F32 ? fminf(fmaxf(cs * B.k_back[n_valid % VALID_RING], 1e-37f), 1e37f) : cs;
                 n_valid++;
                 n_buf += n_m;
                 const bool all = p0 + UNIT - 1 <= lim && (p0 >= low || p0 + UNIT <= A.n_sink) && valid == (1u << n_box) - 1;
@@ -471,11 +494,11 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
                     }
                     mx = fmaxf(mx, m2);
                 }
-                const float mn = mx == -INFINITY ? m : fmaxf(m, mx * cs);
+                const float mn = mx == -INFINITY ? m : fmaxf(m, mx * csu);
                 alpha = mn == -INFINITY ? 1.f : ex2(m - mn);
                 m = mn;
                 const float mo = mn == -INFINITY ? 0.f : mn - 15.f;
-                const uint64_t cs2 = f2(cs, cs), mo2 = f2(-mo, -mo);
+                const uint64_t cs2 = f2(csu, csu), mo2 = f2(-mo, -mo);
                 uint64_t ls2 = 0;
 #pragma unroll 1
                 for (int c = 0; c < UNIT; c += 32) {
@@ -547,9 +570,112 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
             }
             __syncwarp();
         }
+    } else if (F32 && warp < C::W_LOAD + C::N_LOAD) {
+        regs_less<C::REGS_LOAD>();
+        // ---------------------------------------------------------------- k and v tiles of 32-bit pools
+        // Eight warps, 16 positions each (of one page): read, scaled by the power of two that brings the tile's largest element to
+        // [2^14, 2^15), split in two 11-bit parts. What the parts leave out is 2^-39 of the tile's largest element, or 2^-22 of the
+        // element itself, whichever is more: an absolute error of a score or an output far below that of 32 bits. Positions that
+        // no row sees are not read: their rows are zero.
+        constexpr int LPR = HD / 4, RPP = 32 / LPR, N = 16 / RPP;
+        const int cw = warp - C::W_LOAD, el = lane % LPR, sub = lane / LPR;
+        uint32_t n = 0, n_valid = 0;
+        auto any = [&](int p) { return p <= w.pr.lim_max && (p >= w.pr.low_min || p < A.n_sink); };
+        auto page_id = [&](int i) {  // lanes 0 .. 7: the pages of the unit's eight groups of 16 positions; -1: none that is seen
+            const int p = w.pr.unit(w.u0 + i) * UNIT + 16 * (lane & 7);
+            int id = -1;
+            if (i < w.n_it && p <= w.pr.lim_max && (p + 15 >= w.pr.low_min || p < A.n_sink)) {
+                id = a.table[(size_t)w.seq * a.table_ld + p / a.page];
+                if ((unsigned)id >= (unsigned)a.n_pages) {
+                    if (cw == 0 && lane < 8) paged_flag(a.status);
+                    id = -2;
+                }
+            }
+            return id;
+        };
+        while (ok && w.next()) {
+            int ids = page_id(0);
+            for (int i = 0; i < w.n_it && ok; i++) {
+                const uint32_t valid = __ballot_sync(0xffffffffu, ids != -2) & 0xff;
+                const int id = __shfl_sync(0xffffffffu, ids, cw), p = w.pr.unit(w.u0 + i) * UNIT + 16 * cw;
+                const size_t at = (size_t)(id >= 0 ? id : 0) * a.page_stride + ((size_t)w.kvh * a.page + p % a.page) * HD + 4 * lane;
+                const float* src[2] = {static_cast<const float*>(a.k) + at, static_cast<const float*>(a.v) + at};
+                const bool full = id >= 0 && p + 15 <= w.pr.lim_max && (p >= w.pr.low_min || p + 16 <= A.n_sink);
+                if (id >= 0)  // v's lines on their way while k is split
+#pragma unroll
+                    for (int r = 0; r < 16; r += 8)
+                        asm volatile("prefetch.global.L2 [%0];" ::"l"(src[1] - 4 * lane + ((r + (lane >> 2)) * HD + (lane & 3) * (HD / 4))));
+                ids = page_id(i + 1);
+#pragma unroll 1
+                for (int kv = 0; kv < 2 && ok; kv++, n++) {
+                    float4 f[N];
+#pragma unroll
+                    for (int j = 0; j < N; j++) {
+                        f[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (full || (id >= 0 && any(p + j * RPP + sub)))
+                            f[j] = __ldg(reinterpret_cast<const float4*>(src[kv] + (size_t)j * 128));
+                    }
+                    if (kv == 1) {  // and the next unit's k
+                        const int idn = __shfl_sync(0xffffffffu, ids, cw);
+                        if (idn >= 0) {
+                            const int pn = w.pr.unit(w.u0 + i + 1) * UNIT + 16 * cw;
+                            const float* s = static_cast<const float*>(a.k) + (size_t)idn * a.page_stride +
+                                             ((size_t)w.kvh * a.page + pn % a.page) * HD;
+#pragma unroll
+                            for (int r = 0; r < 16; r += 8)
+                                asm volatile("prefetch.global.L2 [%0];" ::"l"(s + (r + (lane >> 2)) * HD + (lane & 3) * (HD / 4)));
+                        }
+                    }
+                    float mx = 0.f;
+#pragma unroll
+                    for (int j = 0; j < N; j++) {
+                        const float v = fmaxf(fmaxf(fabsf(f[j].x), fabsf(f[j].y)), fmaxf(fabsf(f[j].z), fabsf(f[j].w)));
+                        if (v < INFINITY) mx = fmaxf(mx, v);
+                    }
+#pragma unroll
+                    for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    if (lane == 0) B.wmax[n & 1][cw] = mx;
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+#pragma unroll
+                    for (int j = 0; j < 8; j++) mx = fmaxf(mx, B.wmax[n & 1][j]);
+                    const int ex = (int)((__float_as_uint(mx) >> 23) & 255) - 127, e = min(max(14 - ex, -100), 100);
+                    const float sc = mx > 0.f ? pow2f(e) : 1.f;
+                    const uint32_t st = n % C::NST, use = n / C::NST;
+                    if (use > 0) ok = bar_wait(&B.kv_empty[st], (use - 1) & 1);
+                    // a wait that gave up is taken by all eight warps alike: the barrier above counts on them
+                    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                                 : "=r"(ok_all)
+                                 : "r"((uint32_t)ok)
+                                 : "memory");
+                    ok = ok_all != 0;
+                    if (!ok) break;
+                    if (cw == 0 && lane == 0) {
+                        (kv ? B.v_back : B.k_back)[n_valid % VALID_RING] = mx > 0.f ? pow2f(-e) : 1.f;
+                        if (kv == 0) B.valid[n_valid % VALID_RING] = valid;
+                    }
+                    uint8_t* hi = skv + st * C::STAGE;
+#pragma unroll
+                    for (int j = 0; j < N; j++) {
+                        const int row = 16 * cw + j * RPP + sub, ch = el >> 1;
+                        const __half2 h0 = __floats2half2_rn(f[j].x * sc, f[j].y * sc), h1 = __floats2half2_rn(f[j].z * sc, f[j].w * sc);
+                        const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+                        const __half2 l0 = __floats2half2_rn(fmaf(f[j].x, sc, -b0.x), fmaf(f[j].y, sc, -b0.y)),
+                                      l1 = __floats2half2_rn(fmaf(f[j].z, sc, -b1.x), fmaf(f[j].w, sc, -b1.y));
+                        const int to = (ch >> 3) * C::BLK + row * 128 + (((ch & 7) ^ (row & 7)) << 4) + (el & 1) * 8;
+                        *reinterpret_cast<uint2*>(hi + to) =
+                            make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+                        *reinterpret_cast<uint2*>(hi + C::TILE + to) =
+                            make_uint2(*reinterpret_cast<const uint32_t*>(&l0), *reinterpret_cast<const uint32_t*>(&l1));
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    mbar_arrive(&B.kv_full[st]);
+                }
+                n_valid++;
+            }
+        }
     } else {
-        EB_REGS_LESS();
-        if (warp == 8) {
+        regs_less<C::REGS_ISSUE>();
+        if (!F32 && warp == C::W_LOAD) {
         // ---------------------------------------------------------------- k and v tiles
         uint32_t n = 0, n_valid = 0;
         const int n_box = UNIT / box;
@@ -574,12 +700,12 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
                     const uint32_t st = n % C::NST, use = n / C::NST;
                     if (use > 0) ok = bar_wait(&B.kv_empty[st], (use - 1) & 1);
                     if (!ok) break;
-                    if (lane == 0) mbar_expect_tx(&B.kv_full[st], C::TILE);
+                    if (lane == 0) mbar_expect_tx(&B.kv_full[st], C::STAGE);
                     __syncwarp();
                     if (lane < n_box) {
 #pragma unroll
                         for (int h = 0; h < C::HALVES; h++)
-                            tma_box(kv ? &vmap : &kmap, skv + st * C::TILE + h * C::BLK + lane * box * 128, &B.kv_full[st], 64 * h,
+                            tma_box(kv ? &vmap : &kmap, skv + st * C::STAGE + h * C::BLK + lane * box * 128, &B.kv_full[st], 64 * h,
                                     p % a.page, w.kvh, id);
                     }
                 }
@@ -587,7 +713,7 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
         }
         // copies in flight land before the block ends
         for (uint32_t k = n > (uint32_t)C::NST ? n - C::NST : 0; k < n; k++) bar_wait(&B.kv_full[k % C::NST], (k / C::NST) & 1);
-        } else if (warp == 9) {
+        } else if (warp == C::W_QK) {
         // ---------------------------------------------------------------- products q k
         // Scores rotate through three buffers, so that new ones wait for the product p v that read their buffer, two
         // products before, and not for the last one of their own tile.
@@ -596,7 +722,7 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
         const uint32_t q_addr = __shfl_sync(0xffffffffu, smem_u32(sq_), 0), kv_addr = __shfl_sync(0xffffffffu, smem_u32(skv), 0);
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
         while (ok && w.next()) {
-            const bool two = w.pr.t0 + tpt < w.pr.t1;
+            const bool two = !F32 && w.pr.t0 + tpt < w.pr.t1;
             ok = bar_wait(&B.q_full[0], n_q0++ & 1);
             if (ok && two) ok = bar_wait(&B.q_full[1], n_q1++ & 1);
 #pragma unroll 1
@@ -611,14 +737,15 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
                     n_buf++;
                     tc_fence_after();
                     const uint32_t d = tm + b * UNIT;
-                    const uint32_t qd = desc_lo(q_addr + mt * 2 * C::TILE, 0), kd = desc_lo(kv_addr + st * C::TILE, 0);
+                    const uint32_t qd = desc_lo(q_addr + mt * 2 * C::TILE, 0), kd = desc_lo(kv_addr + st * C::STAGE, 0);
                     if (elect()) {
 #pragma unroll
-                        for (int part = 0; part < 2; part++)  // low parts first
+                        for (int part = 0; part < C::PARTS + 1; part++)  // q_lo k_hi, (q_hi k_lo,) q_hi k_hi: low parts first
 #pragma unroll
                             for (int k = 0; k < HD / 16; k++) {
                                 const uint32_t off = ((k >> 2) * C::BLK + (k & 3) * 32) >> 4;
-                                mma_smem_a(d, qd + ((part * C::TILE) >> 4) + off, kd + off, ID_S, part | k);
+                                mma_smem_a(d, qd + (part ? C::TILE >> 4 : 0) + off, kd + (F32 && part == 1 ? C::TILE >> 4 : 0) + off, ID_S,
+                                           part | k);
                             }
                         tc_commit(&B.s_full[mt]);
                         mbar_arrive(&B.s_full[mt]);  // what this warp saw of the loads (B.valid) is passed on
@@ -630,23 +757,23 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
         }
         // whatever was issued is done before the tensor memory goes back: the last k tile's release follows its products
         if (n > 0) bar_wait(&B.kv_empty[(n - 2) % C::NST], ((n - 2) / C::NST) & 1);
-        } else if (warp == 10) {
+        } else if (warp == C::W_PV) {
         // ---------------------------------------------------------------- products p v
         // O is one buffer, read by the tile's softmax warps while the other products run.
         constexpr uint32_t ID_O = tc_idesc_f16(128, HD) | (1u << 16);
         uint32_t n = 1, n_p0 = 0, n_p1 = 0, n_buf = 0;
         const uint32_t kv_addr = __shfl_sync(0xffffffffu, smem_u32(skv), 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
         while (ok && w.next()) {
-            const bool two = w.pr.t0 + tpt < w.pr.t1;
+            const bool two = !F32 && w.pr.t0 + tpt < w.pr.t1;
 #pragma unroll 1
             for (int i = 0; i < w.n_it && ok; i++, n += 2) {
                 const uint32_t st = n % C::NST;
                 ok = bar_wait(&B.kv_full[st], (n / C::NST) & 1);
                 if (!ok) break;
                 const int p0 = w.pr.unit(w.u0 + i) * UNIT;
-                if (p0 + UNIT - 1 > w.pr.lim_max || (p0 < w.pr.low_min && p0 + UNIT > A.n_sink)) {
+                if (!F32 && (p0 + UNIT - 1 > w.pr.lim_max || (p0 < w.pr.low_min && p0 + UNIT > A.n_sink))) {
                     // positions that no row sees may hold anything: their v rows become zero, as their p are
-                    uint8_t* vt = skv + st * C::TILE;
+                    uint8_t* vt = skv + st * C::STAGE;
 #pragma unroll 4
                     for (int j = lane >> 3; j < UNIT; j += 4) {  // 8 lanes a row
                         const int p = p0 + j;
@@ -665,15 +792,16 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
                     if (!ok) break;
                     const uint32_t b = n_buf++ % 3;
                     tc_fence_after();
-                    const uint32_t vd = desc_lo(kv_addr + st * C::TILE, C::BLK), p = tm + b * UNIT;
+                    const uint32_t vd = desc_lo(kv_addr + st * C::STAGE, C::BLK), p = tm + b * UNIT;
                     if (elect()) {
 #pragma unroll
-                        for (int part = 0; part < 2; part++)  // low parts first
+                        for (int part = 0; part < C::PARTS + 1; part++)
 #pragma unroll
                             for (int k = 0; k < UNIT / 16; k++)
                                 mma_tmem_a(tm + C::O_COL, p + 32 * (k >> 1) + (part ? 0 : 16) + 8 * (k & 1),
-                                           vd + ((k * 2048) >> 4), ID_O, part | k);
+                                           vd + ((k * 2048) >> 4) + (F32 && part == 1 ? C::TILE >> 4 : 0), ID_O, part | k);
                         tc_commit(&B.pv_done[mt]);
+                        mbar_arrive(&B.pv_done[mt]);  // passes on what this warp saw (B.v_back)
                         tc_commit(&B.s_free[b]);
                         if (mt == 1 || !two) tc_commit(&B.kv_empty[st]);
                     }
@@ -688,7 +816,7 @@ __global__ void __launch_bounds__(TC_NT, 1) k_paged_attn_tc(PagedAttnArgs A, con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 8) tc_dealloc(tmem, C::COLS);
+    if (warp == C::W_LOAD) tc_dealloc(tmem, C::COLS);
 }
 
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -717,24 +845,26 @@ bool pool_map(CUtensorMap* m, const PagedArgs& a, const void* base, int hd, int 
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int HD>
+template <int HD, bool F32>
 cudaError_t tc_go(const PagedAttnArgs& A, cudaStream_t st) {
-    int box = UNIT;
+    using C = Tc<HD, F32>;
+    int box = F32 ? 16 : UNIT;
     while (A.c.page % box) box /= 2;  // gcd(page, 128): at least 16
-    CUtensorMap km, vm;
-    if (!pool_map(&km, A.c, A.c.k, HD, box) || !pool_map(&vm, A.c, A.c.v, HD, box)) return cudaErrorInvalidValue;
+    CUtensorMap km{}, vm{};
+    if (!F32 && (!pool_map(&km, A.c, A.c.k, HD, box) || !pool_map(&vm, A.c, A.c.v, HD, box))) return cudaErrorInvalidValue;
     cudaFuncAttributes at;
-    cudaError_t e = cudaFuncGetAttributes(&at, k_paged_attn_tc<HD>);
-    if (e != cudaSuccess || at.numRegs != REGS_LAUNCH) return e != cudaSuccess ? e : cudaErrorInvalidConfiguration;
-    e = smem_limit<Tc<HD>>(k_paged_attn_tc<HD>, Tc<HD>::SMEM);
+    cudaError_t e = cudaFuncGetAttributes(&at, k_paged_attn_tc<HD, F32>);
+    if (e != cudaSuccess || at.numRegs != C::REGS) return e != cudaSuccess ? e : cudaErrorInvalidConfiguration;
+    e = smem_limit<C>(k_paged_attn_tc<HD, F32>, C::SMEM);
     if (e != cudaSuccess) return e;
-    return launch_pdl(k_paged_attn_tc<HD>, dim3(A.grid), dim3(TC_NT), Tc<HD>::SMEM, st, A, km, vm, box);
+    return launch_pdl(k_paged_attn_tc<HD, F32>, dim3(A.grid), dim3(C::NT), C::SMEM, st, A, km, vm, box);
 }
 }  // namespace
 
 int paged_tc_grid() { return sm_count(); }
-cudaError_t launch_paged_attn_tc(int hd, const PagedAttnArgs& A, cudaStream_t st) {
-    return hd == 128 ? tc_go<128>(A, st) : tc_go<64>(A, st);
+cudaError_t launch_paged_attn_tc(int type, int hd, const PagedAttnArgs& A, cudaStream_t st) {
+    if (type == T_F16) return hd == 128 ? tc_go<128, false>(A, st) : tc_go<64, false>(A, st);
+    return hd == 128 ? tc_go<128, true>(A, st) : tc_go<64, true>(A, st);
 }
 
 }  // namespace eb
