@@ -61,7 +61,7 @@ struct Bars {
     float wmax[2][8];
     uint32_t tmem;
     int seq;
-    long long start, scan[16];
+    long long start, scan_u[16], scan_p[16];
 };
 static_assert(sizeof(Bars) <= 1024, "");
 
@@ -187,8 +187,9 @@ __device__ __forceinline__ bool elect() {  // one lane of a converged warp
 __device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; }
 
 // The walk of a block through its share: work in (sequence, pair of row tiles, kv head, unit) order. Shares are even in
-// ticks: one for a unit and TILE_TICKS for a pair's q and output.
-constexpr int TILE_TICKS = 3;
+// ticks: one for a unit and TILE_TICKS for a pair's q and output; where there are fewer than CUT_UNITS units for each block, pairs
+// are cut into so many shares that every block pays for q and output, and only units count.
+constexpr int TILE_TICKS = 3, CUT_UNITS = 8;
 struct Pair {
     int t0, t1;                   // tokens of the pair (32-bit pools: of one row tile)
     int low_min, lim_max;         // positions that some row sees: [low_min, lim_max] and the first n_sink
@@ -212,13 +213,13 @@ __device__ __forceinline__ bool tc_takes(const PagedAttnArgs& A, const Seq& sq) 
 
 struct Walk {
     const PagedAttnArgs& A;
-    int tok, seq, pair = 0;  // tok: tokens of a pair
+    int tok, extra, seq, pair = 0;  // tok: tokens of a pair; extra: its ticks beside its units'
     long long at, end, base;
     Seq sq;
     Pair pr;
     int kvh, u0, n_it, nu;
-    __device__ Walk(const PagedAttnArgs& A_, int tok_, int seq_, long long base_, long long at_, long long end_)
-        : A(A_), tok(tok_), seq(seq_), at(at_), end(end_), base(base_) {
+    __device__ Walk(const PagedAttnArgs& A_, int tok_, int extra_, int seq_, long long base_, long long at_, long long end_)
+        : A(A_), tok(tok_), extra(extra_), seq(seq_), at(at_), end(end_), base(base_) {
         sq.q = 0;
     }
     __device__ bool next() {
@@ -232,7 +233,7 @@ struct Walk {
             }
             pr = pair_of(A, sq, pair, tok);
             nu = pr.n();
-            const int ticks = nu + TILE_TICKS;
+            const int ticks = nu + extra;
             const long long w = (long long)ticks * A.c.n_kv;
             if (at >= base + w) {
                 base += w;
@@ -243,8 +244,8 @@ struct Walk {
             kvh = idx / ticks;
             const int t0 = idx - kvh * ticks, t1 = (int)min((long long)ticks, t0 + (end - at));
             at += t1 - t0;
-            u0 = max(0, t0 - TILE_TICKS);
-            n_it = max(0, t1 - TILE_TICKS) - u0;
+            u0 = max(0, t0 - extra);
+            n_it = max(0, t1 - extra) - u0;
             if (n_it > 0) return true;  // else this block's share ends before the tile's first unit
         }
         return false;
@@ -291,59 +292,69 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
     if (warp == C::W_LOAD) tc_alloc(&B.tmem, C::COLS);
     pdl_wait();
     pdl_trigger();
-    // ---- this block's share
-    auto weight = [&](int s, bool flag) -> long long {
-        const Seq sq = paged_seq(a, s, flag);
-        if (!tc_takes(A, sq)) return 0;
-        long long n = 0;
-        for (int p = 0; p * C::NM * tpt < sq.q; p++) n += pair_of(A, sq, p, C::NM * tpt).n() + TILE_TICKS;
-        return n * a.n_kv;
-    };
-    long long total = 0, mine = 0;
-    for (int s0 = 0; s0 < a.n_seq; s0 += TC_NT) {
-        mine = s0 + tid < a.n_seq ? weight(s0 + tid, blockIdx.x == 0) : 0;
-        long long v = mine;
+    // ---- this block's share: sums over the sequences of their units and pairs
+    long long units = 0, pairs = 0, mine_u = 0, mine_p = 0, upto_u = 0, upto_p = 0;  // of sequence s0 + tid; with all before it
+    auto scan = [&](int s0, bool flag) {
+        mine_u = mine_p = 0;
+        if (s0 + tid < a.n_seq) {
+            const Seq sq = paged_seq(a, s0 + tid, flag);
+            if (tc_takes(A, sq))
+                for (int p = 0; p * C::NM * tpt < sq.q; p++, mine_p++) mine_u += pair_of(A, sq, p, C::NM * tpt).n();
+        }
+        upto_u = mine_u;
+        upto_p = mine_p;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-        if (lane == 0) B.scan[warp] = v;
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, upto_u, o), p = __shfl_up_sync(0xffffffffu, upto_p, o);
+            if (lane >= o) {
+                upto_u += u;
+                upto_p += p;
+            }
+        }
+        __syncthreads();  // the sums of the round before are read
+        if (lane == 31) {
+            B.scan_u[warp] = upto_u;
+            B.scan_p[warp] = upto_p;
+        }
         __syncthreads();
-        for (int w = 0; w < TC_NT / 32; w++) total += B.scan[w];
-        __syncthreads();
-    }
-    const long long share = max((total + gridDim.x - 1) / gridDim.x, (long long)A.min_units);
-    const long long begin = share * blockIdx.x, end = min(total, begin + share);
+        upto_u += units;
+        upto_p += pairs;
+        for (int w = 0; w < TC_NT / 32; w++) {
+            if (w < warp) {
+                upto_u += B.scan_u[w];
+                upto_p += B.scan_p[w];
+            }
+            units += B.scan_u[w];
+            pairs += B.scan_p[w];
+        }
+    };
     if (tid == 0) {
         A.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
         B.seq = a.n_seq;
         B.start = 0;
     }
-    __syncthreads();
-    long long run = 0;
-    for (int s0 = 0; s0 < a.n_seq && begin < total; s0 += TC_NT) {
-        if (a.n_seq > TC_NT) mine = s0 + tid < a.n_seq ? weight(s0 + tid, false) : 0;
-        long long v = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long n = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += n;
-        }
-        if (lane == 31) B.scan[warp] = v;
-        __syncthreads();
-        for (int w = 0; w < warp; w++) v += B.scan[w];
-        v += run;
-        if (mine > 0 && v - mine <= begin && begin < v) {
+    for (int s0 = 0; s0 < a.n_seq; s0 += TC_NT) scan(s0, blockIdx.x == 0);
+    const int extra = units * a.n_kv >= (long long)CUT_UNITS * gridDim.x ? TILE_TICKS : 0;
+    const long long total = (units + extra * pairs) * a.n_kv;
+    const long long share = max((total + gridDim.x - 1) / gridDim.x, (long long)A.min_units);
+    const long long begin = share * blockIdx.x, end = min(total, begin + share);
+    units = pairs = 0;
+    for (int s0 = 0; s0 < a.n_seq && begin < total && (units + extra * pairs) * a.n_kv <= begin; s0 += TC_NT) {
+        if (a.n_seq > TC_NT)
+            scan(s0, false);
+        else
+            units = total;  // scanned already: one round
+        const long long to = (upto_u + extra * upto_p) * a.n_kv, from = to - (mine_u + extra * mine_p) * a.n_kv;
+        if (from <= begin && begin < to) {
             B.seq = s0 + tid;
-            B.start = v - mine;
+            B.start = from;
         }
-        for (int w = 0; w < TC_NT / 32; w++) run += B.scan[w];
-        __syncthreads();
-        if (run > begin) break;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = B.tmem;
-    Walk w(A, C::NM * tpt, B.seq, B.start, begin, end);
+    Walk w(A, C::NM * tpt, extra, B.seq, B.start, begin, end);
     uint32_t ok_all = 1;
     (void)ok_all;
     bool ok = true;  // a bounded wait that gives up ends the walk; the other warps' own waits then give up too
@@ -385,16 +396,13 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
                     asm volatile("ld.global.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "l"(src + 4 * el));
                 };
                 float mx = 0.f;
-#pragma unroll 1
-                for (int i0 = 0; i0 < 32; i0 += 16) {
-                    float4 f[16 / RPP];
+                float4 f[32 / RPP];  // all of the warp's rows in flight at once (the sums are not live yet)
 #pragma unroll
-                    for (int i = 0; i < 16 / RPP; i++) load(i0 + i * RPP, f[i]);
+                for (int i = 0; i < 32 / RPP; i++) load(i * RPP, f[i]);
 #pragma unroll
-                    for (int i = 0; i < 16 / RPP; i++) {
-                        const float v = fmaxf(fmaxf(fabsf(f[i].x), fabsf(f[i].y)), fmaxf(fabsf(f[i].z), fabsf(f[i].w)));
-                        if (v < INFINITY) mx = fmaxf(mx, v);  // a row that is not finite does not disturb the others
-                    }
+                for (int i = 0; i < 32 / RPP; i++) {
+                    const float v = fmaxf(fmaxf(fabsf(f[i].x), fabsf(f[i].y)), fmaxf(fabsf(f[i].z), fabsf(f[i].w)));
+                    if (v < INFINITY) mx = fmaxf(mx, v);  // a row that is not finite does not disturb the others
                 }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -402,26 +410,20 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
                 float sc = mx > 0.f ? pow2f(min(max(14 - ex, -100), 100)) : 1.f;
                 cs = fmaxf(fabsf(A.scale) * 1.4426950408889634f / sc, 1e-37f);  // never zero: c times -infinity
                 if (A.scale <= 0.f) sc = A.scale < 0.f ? -sc : 0.f;             // the running maximum is that of +c S
-#pragma unroll 1
-                for (int i0 = 0; i0 < 32; i0 += 8) {
-                    float4 f[8 / RPP];
 #pragma unroll
-                    for (int i = 0; i < 8 / RPP; i++) load(i0 + i * RPP, f[i]);
-#pragma unroll
-                    for (int i = 0; i < 8 / RPP; i++) {
-                        const int ro = i0 + i * RPP + sub, row = 32 * (warp & 3) + ro;
-                        if (!((rows_ok >> ro) & 1)) f[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        const __half2 h0 = __floats2half2_rn(f[i].x * sc, f[i].y * sc), h1 = __floats2half2_rn(f[i].z * sc, f[i].w * sc);
-                        const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
-                        const __half2 l0 = __floats2half2_rn(f[i].x * sc - b0.x, f[i].y * sc - b0.y),
-                                      l1 = __floats2half2_rn(f[i].z * sc - b1.x, f[i].w * sc - b1.y);
-                        const int ch = el >> 1;  // 16-byte chunk
-                        const int at = (ch >> 3) * C::BLK + row * 128 + (((ch & 7) ^ (row & 7)) << 4) + (el & 1) * 8;
-                        *reinterpret_cast<uint2*>(q_hi + at) =
-                            make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
-                        *reinterpret_cast<uint2*>(q_lo + at) =
-                            make_uint2(*reinterpret_cast<const uint32_t*>(&l0), *reinterpret_cast<const uint32_t*>(&l1));
-                    }
+                for (int i = 0; i < 32 / RPP; i++) {
+                    const int ro = i * RPP + sub, row = 32 * (warp & 3) + ro;
+                    if (!((rows_ok >> ro) & 1)) f[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    const __half2 h0 = __floats2half2_rn(f[i].x * sc, f[i].y * sc), h1 = __floats2half2_rn(f[i].z * sc, f[i].w * sc);
+                    const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
+                    const __half2 l0 = __floats2half2_rn(fmaf(f[i].x, sc, -b0.x), fmaf(f[i].y, sc, -b0.y)),
+                                  l1 = __floats2half2_rn(fmaf(f[i].z, sc, -b1.x), fmaf(f[i].w, sc, -b1.y));
+                    const int ch = el >> 1;  // 16-byte chunk
+                    const int at = (ch >> 3) * C::BLK + row * 128 + (((ch & 7) ^ (row & 7)) << 4) + (el & 1) * 8;
+                    *reinterpret_cast<uint2*>(q_hi + at) =
+                        make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
+                    *reinterpret_cast<uint2*>(q_lo + at) =
+                        make_uint2(*reinterpret_cast<const uint32_t*>(&l0), *reinterpret_cast<const uint32_t*>(&l1));
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(&B.q_full[mt]);
