@@ -6,6 +6,10 @@ and its generate loop feeds one token per forward call, :1294-1310). Here reques
 slot is free the next request's prompt is prefilled into it, and every step runs one token of every
 active sequence as a single forward pass. A sequence leaves when it has its tokens, and its slot takes
 the next request at once. Greedy selection; per-sequence tokens equal that sequence decoded alone.
+
+With `pages` the slots share a paged cache (eahmmf_engine_set_paged): a request is admitted when the pages
+for its prompt and all of its tokens are free beside those that the running ones will still take, and its
+pages go back when it leaves.
 """
 from __future__ import annotations
 
@@ -25,23 +29,36 @@ class Request:
 class ContinuousBatcher:
     """Run requests through an engine with `n_slots` sequence slots, at most `max_rows` (<= 64) per step."""
 
-    def __init__(self, engine, n_slots: int, max_rows: int = 64, n_batch: int = 64):
-        if engine.set_slots(n_slots):
+    def __init__(self, engine, n_slots: int, max_rows: int = 64, n_batch: int = 64, pages: int = 0, page: int = 64,
+                 dtype: str = "f16"):
+        if pages:
+            if engine.set_paged(n_slots, pages, page, dtype):
+                raise RuntimeError("eahmmf_engine_set_paged failed")
+        elif engine.set_slots(n_slots):
             raise RuntimeError("eahmmf_engine_set_slots failed")
+        self.pages, self.page = pages, page
         self.e, self.n_slots, self.max_rows, self.n_batch = engine, n_slots, min(max_rows, 64), n_batch
         self.queue: deque = deque()
         self.active: dict = {}  # slot -> Request
         self.steps = 0
         self.rows = 0  # sequence-tokens decoded by steps (throughput accounting)
 
+    def _need(self, r: Request) -> int:
+        """Pages of a request's positions: its prompt and every token but the last, which is not fed."""
+        return -(-(len(r.prompt) + r.n_gen - 1) // self.page)
+
     def submit(self, prompt, n_gen: int) -> Request:
         r = Request(list(map(int, prompt)), int(n_gen))
+        if self.pages and self._need(r) > self.pages:
+            raise ValueError(f"the request needs {self._need(r)} pages, the cache has {self.pages}")
         self.queue.append(r)
         return r
 
     def _admit(self):
         free = [s for s in range(self.n_slots) if s not in self.active]
         while free and self.queue and len(self.active) < self.max_rows:
+            if self.pages and sum(map(self._need, self.active.values())) + self._need(self.queue[0]) > self.pages:
+                break
             r = self.queue.popleft()
             r.slot = free.pop(0)
             rc, first = self.e.prefill_slot(r.slot, r.prompt, self.n_batch)
@@ -51,6 +68,8 @@ class ContinuousBatcher:
             r.pos = len(r.prompt)
             if len(r.tokens) < r.n_gen:
                 self.active[r.slot] = r
+            elif self.pages:
+                self.e.free_slot(r.slot)
 
     def step(self) -> bool:
         """Admit what fits, then one token of every active sequence. False when nothing is left."""
@@ -68,6 +87,8 @@ class ContinuousBatcher:
             r.pos += 1
             if len(r.tokens) >= r.n_gen:
                 del self.active[r.slot]
+                if self.pages:
+                    self.e.free_slot(r.slot)
         return True
 
     def run(self):

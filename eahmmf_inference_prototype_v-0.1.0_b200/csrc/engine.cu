@@ -25,6 +25,7 @@
 #include <cstring>
 #include <map>
 #include <memory>
+#include <new>
 #include <string>
 #include <thread>
 #include <vector>
@@ -342,6 +343,20 @@ struct EahmmfEngine {
     int* d_btok = nullptr;          // [MAXB] their input tokens, then their argmax
     int* h_b = nullptr;             // pinned staging [3 * MAXB]
     float* logits_b = nullptr;      // [MAXB x n_vocab] logits of every row of a multi-sequence step
+    // paged slots: one cache of pages for all of them instead of n_ctx positions each; `pass` is the sequences of the
+    // forward pass in progress (n_seq 0: a pass over the contiguous cache)
+    struct Paged {
+        EahmmfPagedKv kv{};
+        EahmmfPages* pages = nullptr;
+        int n_slots = 0, max_pages = 0;
+        void* ws = nullptr;
+        size_t ws_bytes = 0;
+        int* dev = nullptr;   // [MAXB + 1] first rows, [MAXB] lengths, [MAXB x max_pages] page ids
+        int* host = nullptr;  // pinned staging of the same
+        std::vector<int> len, pairs, table;  // host: positions of each slot, copies of a step, every slot's pages
+    };
+    std::unique_ptr<Paged> paged;
+    EahmmfPagedSeqs pass{};
     int graph_nodes = 0;
     bool trace = false;
     std::vector<int> trace_ids;
@@ -373,6 +388,7 @@ struct EahmmfEngine {
             else if (C.pinned && C.file) cudaHostUnregister(const_cast<uint8_t*>(C.file->map));
             cache.reset();  // unmaps the file
         }
+        drop_paged();
         for (cudaEvent_t v : pev) cudaEventDestroy(v);
         if (step_graph) cudaGraphExecDestroy(step_graph);
         if (u_host) cudaFreeHost(u_host);
@@ -948,7 +964,8 @@ struct EahmmfEngine {
         const int nsplit = nsplit_for(nb);
         const float scale = 1.0f / sqrtf((float)hd);
         if (!mark(0)) return ST_CUDA;
-        if (launch_rope_table(fst, inv_freq, hd / 2, nb, rope_cs, st) != cudaSuccess) return ST_CUDA;
+        const bool pg = pass.n_seq > 0;
+        if (!pg && launch_rope_table(fst, inv_freq, hd / 2, nb, rope_cs, st) != cudaSuccess) return ST_CUDA;
         if (launch_embed(embd, embd_type, embd_rb, D, n_embd_rows, tok, nb, x, status, st) != cudaSuccess)
             return ST_CUDA;
         if (!mark(0)) return ST_CUDA;
@@ -1000,7 +1017,7 @@ struct EahmmfEngine {
             const size_t lo = ((size_t)l * n_slots + (batch ? 0 : slot_cur)) * n_ctx * KD;
             float* lk = kc + lo;
             float* lv = vc + lo;
-            if (nb == 1 && !batch && fused_step_ok(L)) {  // single-token step: 6 launches per layer
+            if (nb == 1 && !batch && !pg && fused_step_ok(L)) {  // single-token step: 6 launches per layer
                 const int rc = layer_step1(L, lk, lv, scale, nsplit, pending);
                 if (rc != ST_OK) return rc;
                 continue;
@@ -1031,7 +1048,12 @@ struct EahmmfEngine {
             }
             if (rc != ST_OK || !mark(2)) return rc != ST_OK ? rc : ST_CUDA;
             RopeFuse rf{};
-            if (nb == 1 && !batch) {  // single-token step: norms, rotation and KV append inside the attention kernel
+            const XF xf_o = xf_carve(xf_att, MAXB, QD);
+            if (pg) {
+                if (!mark(3)) return ST_CUDA;
+                rc = paged_attention(L, l, nb, scale, xf_o);
+                if (rc != ST_OK || !mark(4)) return rc != ST_OK ? rc : ST_CUDA;
+            } else if (nb == 1 && !batch) {  // single-token step: norms, rotation and KV append inside the attention kernel
                 rf.qkv = qkv;
                 rf.qn = L.q_norm;
                 rf.kn = L.k_norm;
@@ -1043,11 +1065,11 @@ struct EahmmfEngine {
                        !mark(3)) {
                 return ST_CUDA;
             }
-            const XF xf_o = xf_carve(xf_att, MAXB, QD);
-            if (launch_attention(hd, q, lk, lv, n_head, n_kv, scale, fst, nb, nsplit, attn_part, att, xf_o, rf, pos_host,
+            if (!pg &&
+                (launch_attention(hd, q, lk, lv, n_head, n_kv, scale, fst, nb, nsplit, attn_part, att, xf_o, rf, pos_host,
                                  st) !=
-                    cudaSuccess ||
-                !mark(4))
+                     cudaSuccess ||
+                 !mark(4)))
                 return ST_CUDA;
             {  // o-projection accumulated into the residual, over the merged rows in fragment form
                 const QMat W{L.wo, L.wo_type, QD, D, L.wo_rb};
@@ -1145,6 +1167,126 @@ struct EahmmfEngine {
             hpos += nb;
         }
         return ST_OK;
+    }
+
+    // ---- paged slots ---------------------------------------------------------------------------------
+    static void release(std::unique_ptr<Paged>& p) {
+        if (!p) return;
+        for (void* b : {p->kv.d_k, p->kv.d_v, p->ws, (void*)p->dev})
+            if (b) cudaFree(b);
+        if (p->host) cudaFreeHost(p->host);
+        if (p->pages) eahmmf_pages_destroy(p->pages);
+        p.reset();
+    }
+    void drop_paged() { release(paged); }
+    // A new paged cache in the place of the present one, which stays where there is not enough memory.
+    int set_paged(int n_slots_, int n_pages, int page, int type) {
+        if (cudaStreamSynchronize(st) != cudaSuccess) return ST_CUDA;
+        std::unique_ptr<Paged> made;
+        bool ok = false;
+        try {
+            made.reset(new Paged());
+            Paged& P = *made;
+            P.n_slots = n_slots_;
+            P.max_pages = (n_ctx + page - 1) / page;
+            P.len.assign(n_slots_, 0);
+            P.pairs.resize(2 * (size_t)n_pages);
+            P.table.resize((size_t)n_slots_ * P.max_pages);
+            P.pages = eahmmf_pages_create(n_pages, page, n_slots_, P.max_pages);
+            const size_t own = (size_t)n_kv * page * hd, bytes = own * n_pages * n_layer * (type == T_F16 ? 2 : 4);
+            const size_t ints = 2 * MAXB + 1 + (size_t)MAXB * P.max_pages;
+            P.kv.type = type;
+            P.kv.n_layer = n_layer;
+            P.kv.n_pages = n_pages;
+            P.kv.n_kv = n_kv;
+            P.kv.page = page;
+            P.kv.hd = hd;
+            P.kv.page_stride = own;
+            P.kv.layer_stride = own * n_pages;
+            ok = P.pages && cudaMalloc(&P.kv.d_k, bytes) == cudaSuccess && cudaMalloc(&P.kv.d_v, bytes) == cudaSuccess &&
+                 cudaMalloc((void**)&P.dev, ints * 4) == cudaSuccess &&
+                 cudaHostAlloc((void**)&P.host, ints * 4, cudaHostAllocDefault) == cudaSuccess;
+            if (ok) {
+                EahmmfPagedSeqs s{};
+                s.n_tok = s.max_q = MAXB;
+                P.ws_bytes = eahmmf_cuda_paged_attention_workspace_bytes(&P.kv, &s, n_head);
+                ok = P.ws_bytes && cudaMalloc(&P.ws, P.ws_bytes) == cudaSuccess;
+            }
+        } catch (const std::bad_alloc&) {
+            ok = false;
+        }
+        if (!ok) {
+            cudaGetLastError();
+            release(made);
+            return ST_CAPACITY;
+        }
+        drop_paged();
+        paged = std::move(made);
+        return ST_OK;
+    }
+    // The sequences of a pass: n slots with rows q[i] (their last positions) on the device, after the copies that their pages
+    // need. The staging is free: the caller has waited for the stream.
+    int paged_begin(const int* slots, const int* rows, int n) {
+        Paged& P = *paged;
+        const int n_copy = eahmmf_pages_take_copies(P.pages, P.pairs.data(), (int)P.pairs.size() / 2);
+        const int rc = eahmmf_cuda_pages_copy(&P.kv, P.pairs.data(), n_copy, st);
+        if (rc != ST_OK) return rc;
+        if (eahmmf_pages_table(P.pages, P.table.data(), P.max_pages, nullptr) != ST_OK) return ST_CAPACITY;
+        int ld = 1, max_q = 0, max_kv = 0;
+        for (int i = 0; i < n; i++) {
+            ld = std::max(ld, (P.len[slots[i]] + P.kv.page - 1) / P.kv.page);
+            max_q = std::max(max_q, rows[i]);
+            max_kv = std::max(max_kv, P.len[slots[i]]);
+        }
+        int *cu = P.host, *len = cu + MAXB + 1, *tab = len + MAXB;
+        cu[0] = 0;
+        for (int i = 0; i < n; i++) {
+            cu[i + 1] = cu[i] + rows[i];
+            len[i] = P.len[slots[i]];
+            memcpy(tab + (size_t)i * ld, P.table.data() + (size_t)slots[i] * P.max_pages, (size_t)ld * 4);
+        }
+        const size_t ints = 2 * MAXB + 1 + (size_t)n * ld;
+        if (cudaMemcpyAsync(P.dev, P.host, ints * 4, cudaMemcpyHostToDevice, st) != cudaSuccess) return ST_CUDA;
+        pass = EahmmfPagedSeqs{n, cu[n], max_q, max_kv, P.dev, P.dev + MAXB + 1, P.dev + 2 * MAXB + 1, ld};
+        return ST_OK;
+    }
+    // A layer's attention of a paged pass: q|k|v rows -> pages and q, attention over the pages, the merged rows in fragment form.
+    int paged_attention(const Layer& L, int layer, int nb, float scale, const XF& xf_o) {
+        const Paged& P = *paged;
+        const EahmmfRope rope{EAHMMF_ROPE_HALF, hd, 1.0f, inv_freq};
+        int rc = eahmmf_cuda_rope_append(&P.kv, layer, &pass, &rope, n_head, qkv, QD + 2 * KD, L.q_norm, L.k_norm, eps, q, QD, st,
+                                         status);
+        if (rc == ST_OK)
+            rc = eahmmf_cuda_paged_attention(&P.kv, layer, &pass, n_head, q, QD, scale, 0, 0, att, QD, P.ws, P.ws_bytes, st, status);
+        if (rc == ST_OK && launch_prep_x(att, QD, nb, QD, xf_o, st) != cudaSuccess) rc = ST_CUDA;
+        return rc;
+    }
+    // n tokens behind those of `slot`, in passes of n_batch; the last token's logits in `logits`. A failure takes the slot back
+    // to its length of before.
+    int paged_extend(int slot, const int* htoks, int n, int n_batch) {
+        Paged& P = *paged;
+        const int p0 = P.len[slot];
+        int rc = eahmmf_pages_extend(P.pages, slot, p0 + n);
+        if (rc != ST_OK) return rc;
+        if (cudaMemsetAsync(status, 0, 4, st) != cudaSuccess) rc = ST_CUDA;
+        for (int i = 0; i < n && rc == ST_OK; i += n_batch) {
+            const int nb = std::min(n_batch, n - i);
+            if (cudaStreamSynchronize(st) != cudaSuccess) {  // the staging is free
+                rc = ST_CUDA;
+                break;
+            }
+            memcpy(h_toks, htoks + i, (size_t)nb * 4);
+            P.len[slot] = p0 + i + nb;
+            if (cudaMemcpyAsync(toks, h_toks, (size_t)nb * 4, cudaMemcpyHostToDevice, st) != cudaSuccess) rc = ST_CUDA;
+            if (rc == ST_OK) rc = paged_begin(&slot, &nb, 1);
+            if (rc == ST_OK) rc = forward(toks, nb, i + nb == n);
+            pass.n_seq = 0;
+        }
+        if (rc != ST_OK) {
+            P.len[slot] = p0;
+            eahmmf_pages_truncate(P.pages, slot, p0);
+        }
+        return rc;
     }
 
     // KV caches for n sequence slots of n_ctx positions each (zeroed); the previous caches are freed.
@@ -1418,13 +1560,74 @@ extern "C" int eahmmf_engine_step(EahmmfEngine* e, int token, int* next) {
 
 extern "C" int eahmmf_engine_set_slots(EahmmfEngine* e, int n_slots) {
     if (!e || n_slots < 1 || n_slots > 4096) return ST_BAD_ARG;
-    return e->set_slots(n_slots) ? ST_OK : ST_CUDA;
+    if (!e->set_slots(n_slots)) return ST_CUDA;
+    e->drop_paged();
+    return ST_OK;
 }
 
-extern "C" int eahmmf_engine_prefill_slot(EahmmfEngine* e, int slot, const int* prompt, int n, int n_batch, int* first) {
-    if (!e || !prompt || !first || slot < 0 || slot >= e->n_slots || n < 1 || n >= e->n_ctx || n_batch < 1 ||
-        n_batch > MAXB)
+extern "C" int eahmmf_engine_set_paged(EahmmfEngine* e, int n_slots, int n_pages, int page, int type) {
+    if (!e || n_slots < 1 || n_slots > 4096 || n_pages < 1 || page < 16 || page > 1024 || page % 16) return ST_BAD_ARG;
+    if (type != T_F32 && type != T_F16) return ST_BAD_TYPE;
+    const int rc = e->set_paged(n_slots, n_pages, page, type);
+    if (rc != ST_OK) return rc;
+    if (e->n_slots > 1 && !e->set_slots(1)) return ST_CUDA;  // the contiguous cache keeps the single-sequence calls' slot
+    return ST_OK;
+}
+
+namespace {
+bool paged_slot(const EahmmfEngine* e, int slot) { return e && e->paged && slot >= 0 && slot < e->paged->n_slots; }
+bool tokens_ok(const EahmmfEngine* e, const int* toks, int n) {
+    for (int i = 0; i < n; i++)
+        if (toks[i] < 0 || toks[i] >= e->n_embd_rows) return false;
+    return true;
+}
+// n tokens behind those of a paged slot and the first maximum of the last one's logits.
+int extend_slot(EahmmfEngine* e, int slot, const int* toks, int n, int n_batch, int* next) {
+    if (!tokens_ok(e, toks, n)) return ST_BAD_ARG;
+    if ((long long)e->paged->len[slot] + n > e->n_ctx) return ST_BAD_ARG;
+    int rc = e->paged_extend(slot, toks, n, n_batch);
+    if (rc != ST_OK) return rc;
+    if (launch_argmax_rows(e->logits, e->n_vocab, e->n_vocab, 1, e->d_btok, e->st) != cudaSuccess ||
+        cudaMemcpyAsync(e->h_b, e->d_btok, 4, cudaMemcpyDeviceToHost, e->st) != cudaSuccess)
+        return ST_CUDA;
+    rc = e->read_status();
+    *next = e->h_b[0];
+    return rc;
+}
+}  // namespace
+
+extern "C" int eahmmf_engine_extend_slot(EahmmfEngine* e, int slot, const int* toks, int n, int n_batch, int* next) {
+    if (!paged_slot(e, slot) || !toks || !next || n < 1 || n_batch < 1 || n_batch > MAXB) return ST_BAD_ARG;
+    return extend_slot(e, slot, toks, n, n_batch, next);
+}
+
+extern "C" int eahmmf_engine_fork_slot(EahmmfEngine* e, int src, int dst, int len) {
+    if (!paged_slot(e, src) || !paged_slot(e, dst) || src == dst || len < 0 || len > e->paged->len[src] || e->paged->len[dst])
         return ST_BAD_ARG;
+    int rc = eahmmf_pages_fork(e->paged->pages, src, dst);
+    if (rc == ST_OK) rc = eahmmf_pages_truncate(e->paged->pages, dst, len);
+    if (rc == ST_OK) e->paged->len[dst] = len;
+    return rc;
+}
+
+extern "C" int eahmmf_engine_free_slot(EahmmfEngine* e, int slot) {
+    if (!paged_slot(e, slot)) return ST_BAD_ARG;
+    e->paged->len[slot] = 0;
+    return eahmmf_pages_truncate(e->paged->pages, slot, 0);
+}
+
+extern "C" int eahmmf_engine_slot_len(EahmmfEngine* e, int slot) { return paged_slot(e, slot) ? e->paged->len[slot] : -1; }
+extern "C" int eahmmf_engine_free_pages(EahmmfEngine* e) { return e && e->paged ? eahmmf_pages_free_count(e->paged->pages) : -1; }
+
+extern "C" int eahmmf_engine_prefill_slot(EahmmfEngine* e, int slot, const int* prompt, int n, int n_batch, int* first) {
+    if (!e || !prompt || !first || slot < 0 || slot >= (e->paged ? e->paged->n_slots : e->n_slots) || n < 1 || n >= e->n_ctx ||
+        n_batch < 1 || n_batch > MAXB)
+        return ST_BAD_ARG;
+    if (e->paged) {
+        if (!tokens_ok(e, prompt, n)) return ST_BAD_ARG;
+        const int rc = eahmmf_engine_free_slot(e, slot);
+        return rc != ST_OK ? rc : extend_slot(e, slot, prompt, n, n_batch, first);
+    }
     e->slot_cur = slot;
     int rc = e->eval_dev(prompt, n, 0, n_batch);
     e->slot_cur = 0;
@@ -1441,8 +1644,8 @@ extern "C" int eahmmf_engine_step_slots(EahmmfEngine* e, int n, const int* slots
                                         int* next) {
     if (!e || !slots || !pos || !toks || !next || n < 1 || n > MAXB) return ST_BAD_ARG;
     for (int i = 0; i < n; i++) {
-        if (slots[i] < 0 || slots[i] >= e->n_slots || pos[i] < 0 || pos[i] >= e->n_ctx || toks[i] < 0 ||
-            toks[i] >= e->n_embd_rows)
+        if (slots[i] < 0 || slots[i] >= (e->paged ? e->paged->n_slots : e->n_slots) || pos[i] < 0 || pos[i] >= e->n_ctx ||
+            toks[i] < 0 || toks[i] >= e->n_embd_rows || (e->paged && pos[i] != e->paged->len[slots[i]]))
             return ST_BAD_ARG;
         for (int j = 0; j < i; j++)
             if (slots[j] == slots[i]) return ST_BAD_ARG;  // one row per sequence per step
@@ -1458,7 +1661,29 @@ extern "C" int eahmmf_engine_step_slots(EahmmfEngine* e, int n, const int* slots
         cudaMemcpyAsync(e->d_tslot, h + 2 * MAXB, (size_t)n * 4, cudaMemcpyHostToDevice, e->st) != cudaSuccess)
         return ST_CUDA;
     e->pn = 0;
-    int rc = e->forward(e->d_btok, n, true, true);
+    int rc = ST_OK;
+    if (e->paged) {
+        auto& P = *e->paged;
+        int got = 0;
+        while (got < n && (rc = eahmmf_pages_extend(P.pages, slots[got], pos[got] + 1)) == ST_OK) got++;
+        if (got == n) {
+            int ones[MAXB];
+            for (int i = 0; i < n; i++) {
+                P.len[slots[i]] = pos[i] + 1;
+                ones[i] = 1;
+            }
+            rc = e->paged_begin(slots, ones, n);
+        }
+        if (rc != ST_OK) {  // no row is taken: the slots keep their lengths
+            for (int i = 0; i < got; i++) {
+                P.len[slots[i]] = pos[i];
+                eahmmf_pages_truncate(P.pages, slots[i], pos[i]);
+            }
+            return rc;
+        }
+    }
+    rc = e->forward(e->d_btok, n, true, true);
+    e->pass.n_seq = 0;
     if (rc != ST_OK) return rc;
     if (launch_argmax_rows(e->logits_b, e->n_vocab, e->n_vocab, n, e->d_btok, e->st) != cudaSuccess ||
         cudaMemcpyAsync(h, e->d_btok, (size_t)n * 4, cudaMemcpyDeviceToHost, e->st) != cudaSuccess)

@@ -124,6 +124,12 @@ EXPORTS = {
                                      C.c_void_p, C.c_size_t, C.c_void_p]),
     "eahmmf_engine_verify": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "eahmmf_engine_set_slots": (C.c_int, [C.c_void_p, C.c_int]),
+    "eahmmf_engine_set_paged": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "eahmmf_engine_extend_slot": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "eahmmf_engine_fork_slot": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int]),
+    "eahmmf_engine_free_slot": (C.c_int, [C.c_void_p, C.c_int]),
+    "eahmmf_engine_slot_len": (C.c_int, [C.c_void_p, C.c_int]),
+    "eahmmf_engine_free_pages": (C.c_int, [C.c_void_p]),
     "eahmmf_engine_load_budget": (C.c_void_p, [C.c_char_p, C.c_int, C.c_size_t, C.c_char_p, C.c_size_t]),
     "eahmmf_engine_cache_stats": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int]),
     "eahmmf_engine_prefill_slot": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
@@ -384,6 +390,30 @@ class Engine:
     def set_slots(self, n: int) -> int:
         """eahmmf_engine_set_slots: KV caches for n sequences."""
         return lib().eahmmf_engine_set_slots(self._h, n)
+
+    def set_paged(self, n_slots: int, n_pages: int, page: int = 64, dtype: str = "f16") -> int:
+        """eahmmf_engine_set_paged: the slots share a cache of n_pages pages ("f16" or "f32")."""
+        return lib().eahmmf_engine_set_paged(self._h, n_slots, n_pages, page, {"f32": 0, "f16": 1}[dtype])
+
+    def extend_slot(self, slot: int, toks, n_batch: int = 64):
+        """Tokens behind those of a paged slot: (rc, next token)."""
+        t = np.ascontiguousarray(toks, np.int32)
+        nxt = C.c_int(0)
+        rc = lib().eahmmf_engine_extend_slot(self._h, slot, t.ctypes.data, len(t), n_batch, C.byref(nxt))
+        return rc, int(nxt.value)
+
+    def fork_slot(self, src: int, dst: int, length: int) -> int:
+        """eahmmf_engine_fork_slot: dst shares the first `length` positions of src."""
+        return lib().eahmmf_engine_fork_slot(self._h, src, dst, length)
+
+    def free_slot(self, slot: int) -> int:
+        return lib().eahmmf_engine_free_slot(self._h, slot)
+
+    def slot_len(self, slot: int) -> int:
+        return lib().eahmmf_engine_slot_len(self._h, slot)
+
+    def free_pages(self) -> int:
+        return lib().eahmmf_engine_free_pages(self._h)
 
     def prefill_slot(self, slot: int, prompt, n_batch: int = 64):
         """A new sequence in `slot`: (rc, first token)."""

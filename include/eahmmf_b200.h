@@ -417,6 +417,24 @@ int eahmmf_engine_step(EahmmfEngine* e, int token, int* next);
 int eahmmf_engine_set_slots(EahmmfEngine* e, int n_slots);
 int eahmmf_engine_prefill_slot(EahmmfEngine* e, int slot, const int* prompt, int n, int n_batch, int* first);
 int eahmmf_engine_step_slots(EahmmfEngine* e, int n, const int* slots, const int* pos, const int* toks, int* next);
+/* The slots of the calls above over a paged cache (eahmmf_cuda_paged_attention's; no counterpart in the reference): n_pages
+ * pages of `page` positions (a multiple of 16 up to 1024) of type 0 F32 or 1 F16 in every layer, taken by the sequences as
+ * they grow, up to n_ctx positions each; the single-sequence calls keep the contiguous cache. EAHMMF_ST_CAPACITY: not enough
+ * memory, nothing changed. eahmmf_engine_set_slots goes back to contiguous slots.
+ *  - prefill_slot then frees the slot's pages first; step_slots wants each row at its slot's length, and returns
+ *    EAHMMF_ST_CAPACITY without taking any row when there are not enough pages;
+ *  - extend_slot: n tokens behind those of the slot (a further turn, or the rest of a prompt behind a shared start), the first
+ *    maximum of the last one's logits into *next; EAHMMF_ST_CAPACITY leaves the slot as it was;
+ *  - fork_slot: the empty slot dst takes the first len positions of src and shares their pages; the one that grows into a
+ *    shared part-filled page gets a copy of it in its next step;
+ *  - free_slot: the slot's pages are given back; slot_len: its positions (-1: no such paged slot); free_pages: pages that
+ *    nobody holds (-1: no paged cache). */
+int eahmmf_engine_set_paged(EahmmfEngine* e, int n_slots, int n_pages, int page, int type);
+int eahmmf_engine_extend_slot(EahmmfEngine* e, int slot, const int* toks, int n, int n_batch, int* next);
+int eahmmf_engine_fork_slot(EahmmfEngine* e, int src, int dst, int len);
+int eahmmf_engine_free_slot(EahmmfEngine* e, int slot);
+int eahmmf_engine_slot_len(EahmmfEngine* e, int slot);
+int eahmmf_engine_free_pages(EahmmfEngine* e);
 /* The residency layer's --verify contract (Config::verify, eahmmf.h:203-214: every copy checksummed
  * against its GGUF source with hash64, eahmmf.h:64-76, :940, :1014) for the engine's HBM copy: the hash64
  * of every expert component (layers x experts x gate/up/down) computed on the device in one launch, the

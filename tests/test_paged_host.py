@@ -318,3 +318,47 @@ def test_random_calls_keep_every_sequence_its_positions(seed):
                     held[int(x)] = held.get(int(x), 0) + 1
         assert all(p.refs(x) == held.get(x, 0) for x in range(n_pages))
         assert p.free == n_pages - len(held)
+
+
+# ---- the scheduler over a paged cache ----------------------------------------------------------------
+class PagedEngine:
+    """Counts pages as the engine does: a sequence of n positions holds ceil(n / page) of them."""
+
+    def set_paged(self, n_slots, n_pages, page, dtype):
+        self.n_slots, self.n_pages, self.page, self.len = n_slots, n_pages, page, {}
+        return 0
+
+    def used(self):
+        return sum(-(-n // self.page) for n in self.len.values())
+
+    def prefill_slot(self, slot, prompt, n_batch):
+        assert slot not in self.len
+        self.len[slot] = len(prompt)
+        assert self.used() <= self.n_pages
+        return 0, 1
+
+    def step_slots(self, slots, pos, toks):
+        for s, p in zip(slots, pos):
+            assert self.len[s] == p
+            self.len[s] += 1
+        assert self.used() <= self.n_pages  # an admitted request never runs out of pages
+        return 0, [1] * len(slots)
+
+    def free_slot(self, slot):
+        del self.len[slot]
+        return 0
+
+
+def test_scheduler_admits_what_the_pages_hold():
+    import batching
+    rng = random.Random(1)
+    e = PagedEngine()
+    b = batching.ContinuousBatcher(e, n_slots=6, pages=10, page=16)
+    reqs = [b.submit([1] * rng.randint(1, 90), rng.randint(1, 60)) for _ in range(40)]
+    b.run()
+    assert all(len(r.tokens) == r.n_gen for r in reqs)
+    assert not e.len
+    with pytest.raises(ValueError):
+        b.submit([1] * 150, 12)  # 161 positions fed: 11 pages
+    b.submit([1] * 150, 11)
+    b.run()
