@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(CP_NT) k_pages_copy(uint4* __restrict__ k, uin
 // Up to 8 rows (STACK) the two parts of a row lie in rows g and g + 8 of one instruction: no extra work, and the
 // thread that holds row g holds row g + 8 too. 16 rows take an instruction for each part.
 constexpr int PA_NW = 4, PA_NT = 32 * PA_NW;
+constexpr int STEP_BLOCKS = 3;  // blocks an SM holds, by registers and by the rings' shared memory: all run at once
 constexpr float P_SHIFT = 15.f;
 
 template <typename T>
@@ -238,10 +239,10 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
     hi = h2(hx, hy);
     lo = h2(__float2half_rn(x - __half2float(hx)), __float2half_rn(y - __half2float(hy)));
 }
-// x as two parts of 11 bits, both cut (the conversion instruction that rounds runs at a quarter of the rate): 2^-21 of x at
-// most is left out. An infinity or NaN keeps its kind in hi.
+// x as two parts of 11 bits, hi rounded and lo cut, in integer instructions (the conversion instruction runs at a quarter of
+// their rate): at most 2^-21 of x is left out, with either sign. An infinity or a NaN gives a NaN.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-    hi = __float_as_uint(x) & 0xffffe000u;
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 __device__ __forceinline__ float ex2(float v) {  // 2 units of 32 bits; results below 2^-126 are zero, as weights of them may be
@@ -296,8 +297,54 @@ struct AttnSmem {
 // A partial record: o [16][hd], m [16], sum [16].
 __host__ __device__ constexpr int part_floats(int hd) { return 16 * hd + 32; }
 
+// Parts of a row joined by their maxima and sums.
+struct Joined {
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    __device__ __forceinline__ void add(float mj, float lj, const float4& f) {
+        const float mn = fmaxf(m, mj);
+        if (mn == -INFINITY) {  // nothing seen so far (a NaN sum stays one)
+            l += lj;
+            return;
+        }
+        const float a = ex2(m - mn), b = ex2(mj - mn);
+        m = mn;
+        l = fmaf(l, a, lj * b);
+        o.x = fmaf(o.x, a, f.x * b);
+        o.y = fmaf(o.y, a, f.y * b);
+        o.z = fmaf(o.z, a, f.z * b);
+        o.w = fmaf(o.w, a, f.w * b);
+    }
+};
+// Four elements of row r from the records of block b and the `follow` blocks after it, from record j0 on by `step`. A record:
+// o [cap][hd], m [cap], sum [cap]; block b's is its second (begun and not finished), the others' their first.
+__device__ __forceinline__ void join_records(Joined& j, const float* part, int cap, int hd, int r, int c4, int b, int follow, int j0,
+                                             int step) {
+    constexpr int N = 4;  // in flight
+    for (; j0 <= follow; j0 += N * step) {
+        float mj[N], lj[N];
+        float4 f[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const int k = min(j0 + i * step, follow);
+            const float* rec = part + ((size_t)(b + k) * 2 + (k == 0 ? 1 : 0)) * ((size_t)cap * (hd + 2));
+            mj[i] = __ldcg(rec + cap * hd + r);
+            lj[i] = __ldcg(rec + cap * hd + cap + r);
+            f[i] = __ldcg(reinterpret_cast<const float4*>(rec) + r * (hd / 4) + c4);
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (j0 + i * step <= follow) j.add(mj[i], lj[i], f[i]);
+    }
+}
+__device__ __forceinline__ void store_joined(const PagedAttnArgs& A, const Joined& j, int q0, int kvh, int row, int hd, int c4) {
+    const float inv = j.l == 0.f ? 0.f : 1.f / j.l;
+    const int tok = row / A.c.grp;
+    *reinterpret_cast<float4*>(A.out + (size_t)(q0 + tok) * A.ldo + (size_t)(kvh * A.c.grp + row - tok * A.c.grp) * hd + 4 * c4) =
+        make_float4(j.o.x * inv, j.o.y * inv, j.o.z * inv, j.o.w * inv);
+}
 template <typename T, int HD, bool STACK>
-__global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
+__global__ void __launch_bounds__(PA_NT, STEP_BLOCKS) k_paged_attn(PagedAttnArgs A) {
     constexpr bool H16 = sizeof(T) == 2;
     constexpr int STEP = pos_step<T>(), UNIT = STEP * PA_NW, RT = STACK ? 8 : 16, NR = STACK ? 1 : 2;
     constexpr int KS = AttnSmem<T, HD, STACK>::KS;  // k steps of q k
@@ -531,7 +578,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
             const int p_cur = un.unit(u0 + it) * UNIT + warp * STEP;
             const bool on = (live >> (it & 31)) & 1;
             if (!on) continue;  // warp-uniform: no row sees any of the step's positions
-            float sacc[JT][4], slow[JT][4];  // the high parts' product and the rest, joined once at the end
+            float sacc[JT][4], slow[JT][4];  // the high parts' product and the rest (32-bit pools: and every other high one's)
 #pragma unroll
             for (int j = 0; j < JT; j++)
 #pragma unroll
@@ -564,7 +611,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                             uint32_t h0, l0, h1, l1;
                             split_tf32(__uint_as_float(b0), h0, l0);
                             split_tf32(__uint_as_float(b1), h1, l1);
-                            mma_tf32(sacc[j], ah, h0, h1);
+                            mma_tf32(h ? slow[j] : sacc[j], ah, h0, h1);
                             mma_tf32(slow[j], ah, l0, l1);
                             if (!STACK) mma_tf32(slow[j], al, h0, h1);
                         }
@@ -581,7 +628,7 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                 for (int j = 0; j < PT; j++) {
                     const int e = (j & 1) + 2 * i;
                     float raw = H16 && STACK ? sacc[j >> 1][e] : sacc[j >> 1][e] + slow[j >> 1][e];
-                    if (STACK) raw += sacc[j >> 1][e + 2];
+                    if (STACK) raw += H16 ? sacc[j >> 1][e + 2] : sacc[j >> 1][e + 2] + slow[j >> 1][e + 2];
                     sv[i][j] = raw * cs[i];
                 }
             if (!plain) {
@@ -738,118 +785,64 @@ __global__ void __launch_bounds__(PA_NT) k_paged_attn(PagedAttnArgs A) {
                 }
             }
         }
-        if (!whole && u0 == 0 && tid == 0) {  // the blocks after this one hold the rest of the tile
-            const long long tile_end = at + nu;
-            A.meta[blockIdx.x] = make_int4(((int)((tile_end - 1) / share) - blockIdx.x) | n_rows << 16, sq.q0, kvh, r0);
-        }
+        if (!whole && u0 == 0 && tid == 0)  // the blocks after this one hold the rest of the tile
+            A.meta[blockIdx.x] = make_int4(((int)((at + nu - 1) / share) - blockIdx.x) | n_rows << 16, sq.q0, kvh, r0);
         __syncthreads();
         at += A.whole ? 1 : n_it;
     }
 }
 
-// Joins the records of the row tiles that the split cut. Block (b, y) takes rows of the tile that block b of the
-// attention began and left to the blocks after it (meta: how many, with the tile's rows above bit 16; output row of the
-// sequence's first token; kv head; the tile's first row): with ONE one row, its records dealt over the block (a long context is cut often), else a row to each
-// group of hd / 4 threads. cap: rows of a record, o [cap][hd], m [cap], sum [cap].
+// Joins the records of the row tiles that the split cut: block (b, y) takes rows of the tile
+// that block b of the attention began and left to the blocks after it (meta: how many, with the tile's rows above bit 16;
+// output row of the sequence's first token; kv head; the tile's first row). With ONE one row, its records dealt over the
+// block (a long context is cut often), else a row to each group of hd / 4 threads.
 constexpr int PM_NT = 256;
 template <int HD, bool ONE>
 __global__ void __launch_bounds__(PM_NT) k_paged_merge(PagedAttnArgs A, int cap) {
     constexpr int LN = HD / 4, G = PM_NT / LN;
-    __shared__ __align__(16) float so[ONE ? G : 1][HD];
+    __shared__ __align__(16) float4 so[ONE ? G : 1][LN];
     __shared__ float sm[G], sl[G];
     const int b = blockIdx.x, lane = threadIdx.x % LN, grp = threadIdx.x / LN;
-    const int r = ONE ? blockIdx.y : blockIdx.y * G + grp, step = ONE ? G : 1;
+    const int r = ONE ? blockIdx.y : blockIdx.y * G + grp;
     pdl_wait();
     pdl_trigger();
     const int4 me = A.meta[b];
-    if (me.x == 0) return;
-    const int follow = me.x & 0xffff;
-    if (r >= me.x >> 16) return;
-    const int rr = me.w + r;
-    float m = -INFINITY, l = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int N = 4;  // records in flight
-    for (int j0 = ONE ? grp : 0; j0 <= follow; j0 += N * step) {
-        float mj[N], lj[N];
-        float4 f[N];
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            const int j = j0 + i * step;
-            const float* rec = A.part + ((size_t)(b + min(j, follow)) * 2 + (j == 0 ? 1 : 0)) * ((size_t)cap * (HD + 2));
-            mj[i] = rec[cap * HD + r];
-            lj[i] = rec[cap * HD + cap + r];
-            f[i] = reinterpret_cast<const float4*>(rec)[r * LN + lane];
-        }
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            if (j0 + i * step > follow) break;
-            const float mn = fmaxf(m, mj[i]);
-            if (mn == -INFINITY) {  // nothing seen so far (a NaN sum stays one)
-                l += lj[i];
-                continue;
-            }
-            const float ea = ex2(m - mn), eb_ = ex2(mj[i] - mn);
-            m = mn;
-            l = fmaf(l, ea, lj[i] * eb_);
-            o.x = fmaf(o.x, ea, f[i].x * eb_);
-            o.y = fmaf(o.y, ea, f[i].y * eb_);
-            o.z = fmaf(o.z, ea, f[i].z * eb_);
-            o.w = fmaf(o.w, ea, f[i].w * eb_);
-        }
-    }
-    float L = l;
+    if (me.x == 0 || r >= me.x >> 16) return;
+    Joined j;
+    join_records(j, A.part, cap, HD, r, lane, b, me.x & 0xffff, ONE ? grp : 0, ONE ? G : 1);
     if (ONE) {
-        reinterpret_cast<float4*>(so[grp])[lane] = o;
+        so[grp][lane] = j.o;
         if (lane == 0) {
-            sm[grp] = m;
-            sl[grp] = l;
+            sm[grp] = j.m;
+            sl[grp] = j.l;
         }
         __syncthreads();
         if (grp) return;
-        float M = -INFINITY;
-        L = 0.f;
+        j = Joined();
 #pragma unroll
-        for (int j = 0; j < G; j++) M = fmaxf(M, sm[j]);
-        o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int j = 0; j < G; j++) {
-            const float e = sm[j] == -INFINITY ? 0.f : exp2f(sm[j] - M);
-            const float4 f = reinterpret_cast<const float4*>(so[j])[lane];
-            L = sm[j] == -INFINITY ? L + sl[j] : fmaf(sl[j], e, L);
-            o.x = fmaf(f.x, e, o.x);
-            o.y = fmaf(f.y, e, o.y);
-            o.z = fmaf(f.z, e, o.z);
-            o.w = fmaf(f.w, e, o.w);
-        }
+        for (int i = 0; i < G; i++) j.add(sm[i], sl[i], so[i][lane]);
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    const int tok = rr / A.c.grp;
-    *reinterpret_cast<float4*>(A.out + (size_t)(me.y + tok) * A.ldo + (size_t)(me.z * A.c.grp + rr - tok * A.c.grp) * HD +
-                               4 * lane) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    store_joined(A, j, me.y, me.z, me.w + r, HD, lane);
 }
 
-// Up to this many positions a row tile is one block's work: cutting it would save less than the joining launch costs.
+// Up to this many positions a row tile is one block's work: cutting it would save less than joining it costs.
 constexpr int WHOLE_KV = 512;
-// Blocks of the step kernel that an SM holds: by registers and by the rings' shared memory.
-template <typename T, int HD, bool STACK>
-constexpr int step_blocks() {
-    return sizeof(T) == 2 ? 3 : 2;
-}
-constexpr int STEP_BLOCKS_MAX = 3;
-int step_grid_max() { return STEP_BLOCKS_MAX * sm_count(); }
+int step_grid() { return STEP_BLOCKS * sm_count(); }
 
 template <typename T, int HD, bool STACK>
 cudaError_t attn_go(PagedAttnArgs A, int max_kv, cudaStream_t st) {
     constexpr int RT = STACK ? 8 : 16;
     cudaError_t e = smem_limit<AttnSmem<T, HD, STACK>>(k_paged_attn<T, HD, STACK>, sizeof(AttnSmem<T, HD, STACK>));
     if (e != cudaSuccess) return e;
-    A.grid = step_blocks<T, HD, STACK>() * sm_count();
+    A.grid = step_grid();
     A.whole = max_kv <= WHOLE_KV;
     A.min_units = A.whole ? 1 : 4;
     e = launch_pdl(k_paged_attn<T, HD, STACK>, dim3(A.grid), dim3(PA_NT), sizeof(AttnSmem<T, HD, STACK>), st, A);
     if (e != cudaSuccess || A.whole) return e;
-    // few tiles are cut often: their records dealt over blocks; many tiles, each cut once or twice: a row to a group
-    if ((long long)A.c.n_seq * A.c.n_kv * 8 <= A.grid)
+    // A launch of its own joins the pieces: few tiles, each in many, with a row's pieces dealt over a block; many tiles, each in
+    // two or three, with a row to each group. (The block that ends last joining them within the launch took 36.3 instead of
+    // 34.7 us for 32 sequences of 300 to 4,500 positions: the fences of every piece cost more than the launch.)
+    if ((long long)A.c.n_seq * A.c.n_kv * 16 <= A.grid)
         return launch_pdl(k_paged_merge<HD, true>, dim3(A.grid, RT), dim3(PM_NT), 0, st, A, 16);
     return launch_pdl(k_paged_merge<HD, false>, dim3(A.grid, (RT * HD / 4 + PM_NT - 1) / PM_NT), dim3(PM_NT), 0, st, A, 16);
 }
@@ -860,7 +853,7 @@ cudaError_t attn_rows(const PagedAttnArgs& A, bool stack, int max_kv, cudaStream
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 size_t step_ws_bytes(int hd) {
-    return align256((size_t)step_grid_max() * sizeof(int4)) + align256((size_t)step_grid_max() * 2 * part_floats(hd) * sizeof(float));
+    return align256((size_t)step_grid() * sizeof(int4)) + align256((size_t)step_grid() * 2 * part_floats(hd) * sizeof(float));
 }
 size_t tc_ws_bytes(int hd) {
     return align256((size_t)paged_tc_grid() * sizeof(int4)) + (size_t)paged_tc_grid() * 2 * 256 * (hd + 2) * sizeof(float);
@@ -894,7 +887,7 @@ cudaError_t launch_paged_attention(int type, int hd, int max_q, int max_kv, Page
                       : launch_pdl(k_paged_merge<64, false>, dim3(A.grid, 256 / (PM_NT / 16)), dim3(PM_NT), 0, st, A, 256);
         if (e != cudaSuccess || A.c.n_seq == 1) return e;
     }
-    carve(A, step_grid_max(), ws);
+    carve(A, step_grid(), ws);
     const bool stack = max_q * A.c.grp <= 8;
     if (type == T_F16) return hd == 128 ? attn_rows<__half, 128>(A, stack, max_kv, st) : attn_rows<__half, 64>(A, stack, max_kv, st);
     return hd == 128 ? attn_rows<float, 128>(A, stack, max_kv, st) : attn_rows<float, 64>(A, stack, max_kv, st);

@@ -614,22 +614,30 @@ class PagedCache:
                                   page, hd, k.stride(0), k.stride(1))
         self._ref = C.addressof(self.desc)
         self._lib = lib()
+        # what a call of a few microseconds looks up, once
+        self._append, self._attention = self._lib.eahmmf_cuda_rope_append, self._lib.eahmmf_cuda_paged_attention
+        self._f32, self._idx = torch.float32, k.device.index
+        self._device_now, self._stream_now = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
     def _go(self, stream):
-        idx = self.device.index
-        if self._torch.cuda.current_device() != idx:
+        idx = self._idx
+        if self._device_now() != idx:
             raise ValueError(f"the cache lives on {self.device}: make it the current device")
-        return self._torch._C._cuda_getCurrentRawStream(idx) if stream is None else _stream(stream)
+        return self._stream_now(idx) if stream is None else _stream(stream)
 
     def _rows(self, x, name: str, batch, width: int):
-        if (x.dtype is not self._torch.float32 or x.device != self.device or x.dim() != 2 or x.shape[0] < batch.n_tok
-                or x.shape[1] != width or (x.stride(1) != 1 and width > 1)):
+        shape, stride = x.shape, x.stride()
+        if (x.dtype is not self._f32 or x.get_device() != self._idx or len(shape) != 2 or shape[0] < batch.n_tok
+                or shape[1] != width or stride[1] != 1):
             raise ValueError(f"{name}: float32 rows [{batch.n_tok} x {width}] on {self.device} are needed")
-        return x.data_ptr(), x.stride(0) if x.shape[0] > 1 else width
+        return x.data_ptr(), stride[0] if shape[0] > 1 else width
 
-    def _check(self, rc: int, what: str):
-        if rc:
-            raise RuntimeError(f"{what} returned {rc}")
+    def _norm(self, w, name: str):
+        if w is None:
+            return None
+        if w.dtype is not self._f32 or w.get_device() != self._idx or w.numel() != self.hd or not w.is_contiguous():
+            raise ValueError(f"{name}: {self.hd} contiguous float32 weights on {self.device} are needed")
+        return w.data_ptr()
 
     def append(self, layer: int, batch: PagedBatch, qkv, n_head: int, rope: Rope, q_out, q_norm=None, k_norm=None,
                eps: float = 1e-6, stream=None, d_status=None) -> None:
@@ -638,14 +646,10 @@ class PagedCache:
         st = self._go(stream)
         x, ld = self._rows(qkv, "qkv", batch, (n_head + 2 * self.n_kv) * self.hd)
         q, ldq = self._rows(q_out, "q_out", batch, n_head * self.hd)
-        for w, n in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-            if w is not None:
-                _dev_tensor(w, n, "float32", self.device)
-                if w.numel() != self.hd:
-                    raise ValueError(f"{n}: {self.hd} weights are needed")
-        self._check(self._lib.eahmmf_cuda_rope_append(self._ref, layer, batch._ref, rope._ref, n_head, x, ld, _ptr(q_norm),
-                                                      _ptr(k_norm), eps, q, ldq, st, _ptr(d_status)),
-                    "eahmmf_cuda_rope_append")
+        rc = self._append(self._ref, layer, batch._ref, rope._ref, n_head, x, ld, self._norm(q_norm, "q_norm"),
+                          self._norm(k_norm, "k_norm"), eps, q, ldq, st, None if d_status is None else d_status.data_ptr())
+        if rc:
+            raise RuntimeError(f"eahmmf_cuda_rope_append returned {rc}")
 
     def attention_workspace(self, batch: PagedBatch, n_head: int):
         """A device workspace for attention() of this batch (torch uint8 tensor); one per call in flight."""
@@ -660,10 +664,11 @@ class PagedCache:
         y, ldo = self._rows(out, "out", batch, n_head * self.hd)
         if ws is None:
             ws = self.attention_workspace(batch, n_head)
-        self._check(self._lib.eahmmf_cuda_paged_attention(self._ref, layer, batch._ref, n_head, x, ldq,
-                                                          self.hd ** -0.5 if scale is None else scale, window, n_sink, y,
-                                                          ldo, ws.data_ptr(), ws.numel(), st, _ptr(d_status)),
-                    "eahmmf_cuda_paged_attention")
+        rc = self._attention(self._ref, layer, batch._ref, n_head, x, ldq, self.hd ** -0.5 if scale is None else scale, window,
+                             n_sink, y, ldo, ws.data_ptr(), ws.numel() * ws.element_size(), st,
+                             None if d_status is None else d_status.data_ptr())
+        if rc:
+            raise RuntimeError(f"eahmmf_cuda_paged_attention returned {rc}")
 
     def copy_pages(self, pairs, stream=None) -> None:
         """eahmmf_cuda_pages_copy: pairs (from, to) [n x 2] on the host, every layer, k and v."""
@@ -671,7 +676,9 @@ class PagedCache:
         p = np.ascontiguousarray(pairs, np.int32)
         if p.size % 2:
             raise ValueError("pairs: [n x 2] page ids are needed")
-        self._check(self._lib.eahmmf_cuda_pages_copy(self._ref, p.ctypes.data, p.size // 2, st), "eahmmf_cuda_pages_copy")
+        rc = self._lib.eahmmf_cuda_pages_copy(self._ref, p.ctypes.data, p.size // 2, st)
+        if rc:
+            raise RuntimeError(f"eahmmf_cuda_pages_copy returned {rc}")
 
 
 class Pages:
