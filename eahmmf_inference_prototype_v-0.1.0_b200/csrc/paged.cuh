@@ -32,6 +32,10 @@ __device__ __forceinline__ void paged_flag(int* status) {
     if (status) atomicOr(status, (int)ST_BAD_INDEX);
 }
 
+// a / b of non-negative values: nearly always both fit 32 bits, whose division is several times shorter
+__device__ __forceinline__ long long div64(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
 // Sequence s of a call: its activation rows [q0, q0 + q) and kv cached positions. Lengths that do not fit the
 // buffers (rows past n_tok, more positions than the table row names) are cut to what does and flagged.
 struct Seq {

@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
     for (int s0 = 0; s0 < a.n_seq; s0 += TC_NT) scan(s0, blockIdx.x == 0);
     const int extra = units * a.n_kv >= (long long)CUT_UNITS * gridDim.x ? TILE_TICKS : 0;
     const long long total = (units + extra * pairs) * a.n_kv;
-    const long long share = max((total + gridDim.x - 1) / gridDim.x, (long long)A.min_units);
+    const long long share = max(div64(total + gridDim.x - 1, gridDim.x), (long long)A.min_units);
     const long long begin = share * blockIdx.x, end = min(total, begin + share);
     units = pairs = 0;
     for (int s0 = 0; s0 < a.n_seq && begin < total && (units + extra * pairs) * a.n_kv <= begin; s0 += TC_NT) {
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
             const bool row_ok = r < tpt * a.grp && tok < w.pr.t1;
             const int head = w.kvh * a.grp + r % a.grp;
             const int lim = row_ok ? w.sq.kv - w.sq.q + tok : -1;
-            const int low = A.window > 0 ? lim - A.window + 1 : 0;
+            const int low = A.window > 0 ? max(0, lim - A.window + 1) : 0;
             // ---- q: a warp's rows scaled by the power of two that brings their largest to [2^14, 2^15), then split. The low
             // parts are exact to 2^-25 of that, 2^-39 of the largest row: in a score an absolute error of 2^-39 of the
             // warp's largest, far below that of 32 bits. Rows come one (hd 128) or two (hd 64) to a load instruction.
@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
             const bool whole = w.u0 == 0 && w.n_it == w.nu;
             if (!whole && w.u0 == 0 && tid == 0) {
                 const long long tile_end = w.at + (w.nu - w.n_it);
-                A.meta[blockIdx.x] = make_int4(((int)((tile_end - 1) / share) - blockIdx.x) | (w.pr.t1 - w.pr.t0) * a.grp << 16, w.sq.q0, w.kvh,
+                A.meta[blockIdx.x] = make_int4(((int)div64(tile_end - 1, share) - blockIdx.x) | (w.pr.t1 - w.pr.t0) * a.grp << 16, w.sq.q0, w.kvh,
                                                 w.pr.t0 * a.grp);
             }
             // ---- the warp's rows through shared memory (their q is read), so that a row leaves as one run: to the output, or to

@@ -585,7 +585,7 @@ class PagedBatch:
         for t, n in ((table, "table"), (cu_q, "cu_q"), (kv_len, "kv_len")):
             _dev_tensor(t, n, "int32", kv_len.device)
         n_seq = kv_len.numel()
-        if cu_q.numel() != n_seq + 1 or table.dim() != 2 or table.shape[0] != n_seq:
+        if cu_q.numel() != n_seq + 1 or table.dim() != 2 or table.shape[0] != n_seq or (n_seq and table.shape[1] < 1):
             raise ValueError("table [n_seq x ld], cu_q [n_seq + 1] and kv_len [n_seq] are needed")
         self._keep = (table, cu_q, kv_len)
         self.n_tok, self.device = n_tok, kv_len.device
@@ -619,8 +619,10 @@ class PagedCache:
         self._f32, self._idx = torch.float32, k.device.index
         self._device_now, self._stream_now = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
-    def _go(self, stream):
+    def _go(self, batch, stream):
         idx = self._idx
+        if batch is not None and batch.device.index != idx:
+            raise ValueError(f"the batch lives on {batch.device}, the cache on {self.device}")
         if self._device_now() != idx:
             raise ValueError(f"the cache lives on {self.device}: make it the current device")
         return self._stream_now(idx) if stream is None else _stream(stream)
@@ -643,7 +645,7 @@ class PagedCache:
                eps: float = 1e-6, stream=None, d_status=None) -> None:
         """eahmmf_cuda_rope_append: rows qkv [n_tok x (n_head + 2 n_kv) hd] normalised (where weights are given) and
         rotated; q into q_out [n_tok x n_head hd], k and v into the pages of their positions."""
-        st = self._go(stream)
+        st = self._go(batch, stream)
         x, ld = self._rows(qkv, "qkv", batch, (n_head + 2 * self.n_kv) * self.hd)
         q, ldq = self._rows(q_out, "q_out", batch, n_head * self.hd)
         rc = self._append(self._ref, layer, batch._ref, rope._ref, n_head, x, ld, self._norm(q_norm, "q_norm"),
@@ -659,11 +661,15 @@ class PagedCache:
     def attention(self, layer: int, batch: PagedBatch, q, n_head: int, out, scale: float | None = None, window: int = 0,
                   n_sink: int = 0, ws=None, stream=None, d_status=None) -> None:
         """eahmmf_cuda_paged_attention: out [n_tok x n_head hd] from the rows q (scale: 1 / sqrt(hd))."""
-        st = self._go(stream)
+        st = self._go(batch, stream)
         x, ldq = self._rows(q, "q", batch, n_head * self.hd)
         y, ldo = self._rows(out, "out", batch, n_head * self.hd)
         if ws is None:
+            if stream is not None:
+                raise ValueError("ws: a workspace is needed with a stream of the caller's")
             ws = self.attention_workspace(batch, n_head)
+        elif ws.get_device() != self._idx:
+            raise ValueError(f"ws: a workspace on {self.device} is needed")
         rc = self._attention(self._ref, layer, batch._ref, n_head, x, ldq, self.hd ** -0.5 if scale is None else scale, window,
                              n_sink, y, ldo, ws.data_ptr(), ws.numel() * ws.element_size(), st,
                              None if d_status is None else d_status.data_ptr())
@@ -672,10 +678,11 @@ class PagedCache:
 
     def copy_pages(self, pairs, stream=None) -> None:
         """eahmmf_cuda_pages_copy: pairs (from, to) [n x 2] on the host, every layer, k and v."""
-        st = self._go(stream)
-        p = np.ascontiguousarray(pairs, np.int32)
-        if p.size % 2:
-            raise ValueError("pairs: [n x 2] page ids are needed")
+        st = self._go(None, stream)
+        p = np.asarray(pairs)
+        if p.size % 2 or (p.size and (p.dtype.kind not in "iu" or p.min() < 0 or p.max() >= self.desc.n_pages)):
+            raise ValueError(f"pairs: [n x 2] page ids below {self.desc.n_pages} are needed")
+        p = np.ascontiguousarray(p, np.int32)
         rc = self._lib.eahmmf_cuda_pages_copy(self._ref, p.ctypes.data, p.size // 2, st)
         if rc:
             raise RuntimeError(f"eahmmf_cuda_pages_copy returned {rc}")

@@ -241,8 +241,8 @@ typedef struct EahmmfPagedSeqs {
 } EahmmfPagedSeqs;
 
 /* Rotary positions: pair i < n_rot / 2 of a head, (x[i], x[i + n_rot/2]) or (x[2i], x[2i + 1]), is turned by the angle
- * position * d_inv_freq[i] (product, sine and cosine in 64 bits) and multiplied by mscale; the rest of the head
- * stays as it is. */
+ * position * d_inv_freq[i] (the angle in 64 bits, its sine and cosine to 2^-23) and multiplied by mscale; the rest of the
+ * head stays as it is. */
 #define EAHMMF_ROPE_HALF 0
 #define EAHMMF_ROPE_INTERLEAVED 1
 typedef struct EahmmfRope {
@@ -271,7 +271,7 @@ int eahmmf_rope_inv_freq(int scaling, int n_rot, double base, double factor, int
  * x / sqrt(mean x^2 + eps) * w where d_qnorm (d_knorm) [hd] is given, then its rotation; q goes to d_q (row stride ldq,
  * 32 bits), k and v to their positions' pages, rounded once to the pool's type. Row buffers and weights 16-byte
  * aligned, strides multiples of 4. A row at a negative position (fewer cached positions than rows) gets a zero q row
- * and appends nothing. Two rows of a call must not share a position of a page. Asynchronous. */
+ * and appends nothing. Two rows of a call must not share a position of a page, d_q must not overlap d_qkv. Asynchronous. */
 int eahmmf_cuda_rope_append(const EahmmfPagedKv* kv, int layer, const EahmmfPagedSeqs* seqs, const EahmmfRope* rope,
                             int n_head, const float* d_qkv, int ld, const float* d_qnorm, const float* d_knorm,
                             float eps, float* d_q, int ldq, void* stream, int* d_status);

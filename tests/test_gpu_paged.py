@@ -10,6 +10,9 @@ Tolerances are worst-case bounds of the arithmetic, per element, formed from the
              step of the pool's type (2^-11 relative, 2^-25 below the normal range of 16 bits)
 """
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -254,6 +257,67 @@ def test_bad_pages_and_lengths_are_skipped_and_flagged(torch):
         c.cu[0], c.cu[1] = 5, 1
         c.out.fill_(7.5)
         assert (c.attention() == 7.5).all() and int(c.status.item()) == eb.ST_BAD_INDEX
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("lens", [((1, 1), (40, 700)), ((5, 1, 40), (40, 700, 90))])
+@pytest.mark.parametrize("max_q,max_kv", [(0, 0), (1, 1 << 30), (1 << 30, 0), (1 << 30, 1 << 30)])
+def test_bounds_of_the_lengths_do_not_matter(torch, type, lens, max_q, max_kv):
+    c = Call(torch, type, 128, 2, 8, 16, *lens, seed=14)
+    c.batch = eb.PagedBatch(c.table, c.cu, c.len, c.n_tok, max_q, max_kv)
+    c.check()
+    c.check(window=(1 << 31) - 1, n_sink=(1 << 31) - 1)
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("q", [(1,), (0, 1, 3, 20, 1, 0)])
+def test_many_sequences(torch, type, q):
+    n = 900
+    qs = tuple(q[i % len(q)] for i in range(n))
+    Call(torch, type, 64, 1, 2, 16, qs, tuple(m + (7 * i) % 61 for i, m in enumerate(qs)), seed=15).check()
+
+
+def test_the_first_call_of_a_process_may_be_captured(torch):
+    code = """
+import sys; sys.path[:0] = [%r, %r]
+import torch, test_gpu_paged as t
+for q in ((1,), (40,)):
+    for type in ("f16", "f32"):
+        c = t.Call(torch, type, 128, 2, 8, 16, q, (900,), seed=16)
+        ws = c.cache.attention_workspace(c.batch, c.n_head)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.cache.attention(0, c.batch, c.q, c.n_head, c.out, ws=ws, d_status=c.status)
+        g.replay(); torch.cuda.synchronize()
+        want, tol = c.want()
+        assert (abs(c.out.cpu().numpy() - want) <= tol).all()
+""" % (os.path.dirname(eb.__file__), os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=200)
+    assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_calls_check_their_tensors(torch):
+    c = Call(torch, "f16", 64, 2, 2, 16, (2,), (20,), seed=17)
+    for bad in (c.q.double(), c.q[:1], c.q[:, :-4], c.q.cpu(), c.q.t()):
+        with pytest.raises(ValueError):
+            c.cache.attention(0, c.batch, bad, c.n_head, c.out)
+    with pytest.raises(ValueError):
+        c.cache.attention(0, c.batch, c.q, c.n_head, c.out, stream=torch.cuda.Stream())  # no workspace of its own
+    with pytest.raises(RuntimeError):
+        c.cache.attention(1, c.batch, c.q, c.n_head, c.out)
+    for bad in ([[0, 1 << 32]], [[0, -1]], [[0.0, 1.0]], [[0, 1, 2]]):
+        with pytest.raises(ValueError):
+            c.cache.copy_pages(bad)
+    with pytest.raises(RuntimeError):
+        c.cache.copy_pages([[0, 0]])
+    with pytest.raises(ValueError):
+        eb.PagedCache(c.k, c.v.float())
+    with pytest.raises(ValueError):
+        eb.PagedCache(c.k[..., ::2], c.v[..., ::2])
+    with pytest.raises(ValueError):
+        eb.PagedBatch(c.table.long(), c.cu, c.len, 2, 1, 1)
+    with pytest.raises(ValueError):
+        eb.PagedBatch(c.table, c.cu[:-1], c.len, 2, 1, 1)
 
 
 @pytest.mark.parametrize("lens", [((1, 1, 1), (30, 700, 64)), ((30, 1), (30, 700))])
