@@ -246,6 +246,17 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
     hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
+// the same of the adjacent values x, y: one subtraction for both
+__device__ __forceinline__ void split2_tf32(uint32_t x, uint32_t y, uint32_t (&hi)[2], uint32_t (&lo)[2]) {
+    hi[0] = (x + 0x1000u) & 0xffffe000u;
+    hi[1] = (y + 0x1000u) & 0xffffe000u;
+    asm("{\n\t.reg .b64 a, b, c;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %6};\n\t"
+        "fma.rn.f32x2 a, b, c, a;\n\tmov.b64 {%0, %1}, a;\n\t}"
+        : "=r"(lo[0]), "=r"(lo[1])
+        : "r"(x), "r"(y), "r"(hi[0]), "r"(hi[1]), "r"(0xbf800000u));  // x - hi
+    lo[0] &= 0xffffe000u;
+    lo[1] &= 0xffffe000u;
+}
 __device__ __forceinline__ float ex2(float v) {  // 2 units of 32 bits; results below 2^-126 are zero, as weights of them may be
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
@@ -609,12 +620,11 @@ __global__ void __launch_bounds__(PA_NT, STEP_BLOCKS) k_paged_attn(PagedAttnArgs
                             mma_f16(sacc[j], ah, b0, b1);
                             if (!STACK) mma_f16(slow[j], al, b0, b1);
                         } else {
-                            uint32_t h0, l0, h1, l1;
-                            split_tf32(__uint_as_float(b0), h0, l0);
-                            split_tf32(__uint_as_float(b1), h1, l1);
-                            mma_tf32(h ? slow[j] : sacc[j], ah, h0, h1);
-                            mma_tf32(slow[j], ah, l0, l1);
-                            if (!STACK) mma_tf32(slow[j], al, h0, h1);
+                            uint32_t hi[2], lo[2];
+                            split2_tf32(b0, b1, hi, lo);
+                            mma_tf32(h ? slow[j] : sacc[j], ah, hi[0], hi[1]);
+                            mma_tf32(slow[j], ah, lo[0], lo[1]);
+                            if (!STACK) mma_tf32(slow[j], al, hi[0], hi[1]);
                         }
                     }
                 }
@@ -711,20 +721,22 @@ __global__ void __launch_bounds__(PA_NT, STEP_BLOCKS) k_paged_attn(PagedAttnArgs
             } else {
 #pragma unroll
                 for (int c = 0; c < NB; c++) {
-                    uint4 vr[2];  // rows 2t and 2t + 1: chunk g of the block
+                    uint32_t hi[2][4], lo[2][4];  // rows 2t and 2t + 1: chunk g of the block
 #pragma unroll
-                    for (int j = 0; j < 2; j++)
-                        vr[j] = *reinterpret_cast<const uint4*>(vt + c * BLK + (2 * t + j) * 128 + ((g ^ (2 * t + j)) << 4));
+                    for (int j = 0; j < 2; j++) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(vt + c * BLK + (2 * t + j) * 128 + ((g ^ (2 * t + j)) << 4));
+                        uint32_t h0[2], l0[2], h1[2], l1[2];
+                        split2_tf32(w.x, w.y, h0, l0);
+                        split2_tf32(w.z, w.w, h1, l1);
+                        hi[j][0] = h0[0], hi[j][1] = h0[1], hi[j][2] = h1[0], hi[j][3] = h1[1];
+                        lo[j][0] = l0[0], lo[j][1] = l0[1], lo[j][2] = l1[0], lo[j][3] = l1[1];
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        auto word = [&](const uint4& w) { return e == 0 ? w.x : e == 1 ? w.y : e == 2 ? w.z : w.w; };
                         float s[4] = {0.f, 0.f, 0.f, 0.f};
-                        uint32_t h0, l0, h1, l1;
-                        split_tf32(__uint_as_float(word(vr[0])), h0, l0);
-                        split_tf32(__uint_as_float(word(vr[1])), h1, l1);
-                        if (!STACK) mma_tf32(s, pl, h0, h1);
-                        mma_tf32(s, ph, l0, l1);
-                        mma_tf32(s, ph, h0, h1);
+                        if (!STACK) mma_tf32(s, pl, hi[0][e], hi[1][e]);
+                        mma_tf32(s, ph, lo[0][e], lo[1][e]);
+                        mma_tf32(s, ph, hi[0][e], hi[1][e]);
                         join(4 * c + e, s);
                     }
                 }
