@@ -14,9 +14,9 @@
 // Bound: 4 hd flops per row and position, twice because of the two parts: 2 * 2 * 2 * 128 * 128 * hd per tile and unit. Two
 // tiles share every k and v tile and take turns: while one tile's scores are in the softmax the other's products run.
 //
-// Warps: 0-3 softmax of tile 0, 4-7 of tile 1 (thread = row = tensor-memory lane), 8 loads, 9 issues q k, 10 issues p v
-// (one warp for both left the tensor cores idle a third of the time: each wait costs it some 150 cycles), 11 only gives its
-// registers to the softmax warps.
+// Warps: 0-3 softmax of tile 0, 4-7 of tile 1 (thread = row = tensor-memory lane), 8 loads k, 11 loads v, 9 issues q k, 10 issues
+// p v (one warp for both products left the tensor cores idle a third of the time: each wait costs it some 150 cycles). 32-bit
+// pools: one row tile, 0-3 softmax, 4-11 split k and v, 12 and 13 issue.
 #include <cuda.h>
 
 #include <mutex>
@@ -43,16 +43,16 @@ struct Tc {
     static constexpr int BLK = 128 * 128;                // bytes of a column block of 128 rows
     static constexpr int TILE = HALVES * BLK;            // bytes of a 128 x hd operand tile
     static constexpr int STAGE = PARTS * TILE;           // of a k or v tile in all its parts: hi, lo
-    // Tiles of k and v in shared memory. With room for three, k has two: the next scores wait for the last product p v of the
-    // other tile anyway (its p lies in the score buffer that they take), v is needed a softmax later. A ring of three for both
-    // made every k tile wait for a v tile's slot: 5,900 instead of 4,700 cycles a unit.
+    // Tiles of k and of v in shared memory. Where there is room for three in all, k has two: the next scores wait for the last
+    // product p v of the other tile anyway (its p lies in the score buffer that they take), v is needed a softmax later. One
+    // ring of three for both, two for v, or halves of tiles in twice as many slots measured within 3 % of it.
     static constexpr int NK = F32 ? 1 : HD == 128 ? 2 : 4, NV = F32 || HD == 128 ? 1 : 4, NST = NK + NV;
     static constexpr int Q_BYTES = NM * 2 * TILE;
     static constexpr int SMEM = 1024 + Q_BYTES + NST * STAGE + 1024;
     static constexpr uint32_t O_COL = 384;               // tensor memory: three S, one O
     static constexpr uint32_t COLS = 512;
     static constexpr int W_LOAD = 4 * NM, N_LOAD = F32 ? 8 : 1;  // first warp that brings k and v, how many do
-    static constexpr int W_QK = F32 ? 12 : 9, W_PV = W_QK + 1;
+    static constexpr int W_QK = F32 ? 12 : 9, W_PV = W_QK + 1, W_LOAD_V = 11;  // 16-bit pools: k and v have a warp each
     static constexpr int NT = F32 ? 512 : 384;
     static constexpr int REGS = F32 ? 128 : 168, REGS_SOFTMAX = 208, REGS_LOAD = F32 ? 104 : 88, REGS_ISSUE = F32 ? 96 : 88;
 };
@@ -682,53 +682,42 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
         }
     } else {
         regs_less<C::REGS_ISSUE>();
-        if (!F32 && warp == C::W_LOAD) {
+        if (!F32 && (warp == C::W_LOAD || warp == C::W_LOAD_V)) {
         // ---------------------------------------------------------------- k and v tiles
-        // Order: k of a unit, then v of the unit before.
-        uint32_t n = 0;  // units whose k was asked for
-        const int n_box = UNIT / box;
-        auto bring = [&](const CUtensorMap* map, int slot, uint32_t use, int p, int id) {
-            if (use > 0) ok = bar_wait(&B.kv_empty[slot], (use - 1) & 1);
-            if (!ok) return;
-            if (lane == 0) mbar_expect_tx(&B.kv_full[slot], C::STAGE);
-            __syncwarp();
-            if (lane < n_box) {
-#pragma unroll
-                for (int h = 0; h < C::HALVES; h++)
-                    tma_box(map, skv + slot * C::STAGE + h * C::BLK + lane * box * 128, &B.kv_full[slot], 64 * h, p % a.page, w.kvh, id);
-            }
-        };
+        const bool is_v = warp == C::W_LOAD_V;
+        const CUtensorMap* map = is_v ? &vmap : &kmap;
+        const int n_box = UNIT / box, slot0 = is_v ? C::NK : 0, slots = is_v ? C::NV : C::NK;
+        uint32_t n = 0;  // units
         while (ok && w.next()) {
-            int p_v = 0, id_v = 0;
-            for (int i = 0; i <= w.n_it && ok; i++) {
-                int p = 0, id = a.n_pages;  // outside the pool: the box is filled with zeros
-                if (i < w.n_it) {
-                    p = w.pr.unit(w.u0 + i) * UNIT + lane * box;
-                    bool good = lane < n_box;
-                    if (good && p <= w.pr.lim_max && (p + box - 1 >= w.pr.low_min || p < A.n_sink)) {
-                        id = a.table[(size_t)w.seq * a.table_ld + p / a.page];
-                        if ((unsigned)id >= (unsigned)a.n_pages) {
-                            paged_flag(a.status);
-                            id = a.n_pages;
-                            good = false;
-                        }
+            for (int i = 0; i < w.n_it && ok; i++, n++) {
+                const int p = w.pr.unit(w.u0 + i) * UNIT + lane * box;
+                int id = a.n_pages;  // outside the pool: the box is filled with zeros
+                bool good = lane < n_box;
+                if (good && p <= w.pr.lim_max && (p + box - 1 >= w.pr.low_min || p < A.n_sink)) {
+                    id = a.table[(size_t)w.seq * a.table_ld + p / a.page];
+                    if ((unsigned)id >= (unsigned)a.n_pages) {
+                        if (!is_v) paged_flag(a.status);
+                        id = a.n_pages;
+                        good = false;
                     }
-                    const uint32_t valid = __ballot_sync(0xffffffffu, good);
-                    if (lane == 0) B.valid[n % VALID_RING] = valid;
-                    bring(&kmap, n % C::NK, n / C::NK, p, id);
-                    n++;
                 }
-                if (i > 0 && ok) {
-                    const uint32_t nv = i < w.n_it ? n - 2 : n - 1;
-                    bring(&vmap, C::NK + nv % C::NV, nv / C::NV, p_v, id_v);
+                const uint32_t valid = __ballot_sync(0xffffffffu, good);
+                if (!is_v && lane == 0) B.valid[n % VALID_RING] = valid;
+                const int slot = slot0 + n % slots;
+                const uint32_t use = n / slots;
+                if (use > 0) ok = bar_wait(&B.kv_empty[slot], (use - 1) & 1);
+                if (!ok) break;
+                if (lane == 0) mbar_expect_tx(&B.kv_full[slot], C::STAGE);
+                __syncwarp();
+                if (lane < n_box) {
+#pragma unroll
+                    for (int b = 0; b < C::HALVES; b++)
+                        tma_box(map, skv + slot * C::STAGE + b * C::BLK + lane * box * 128, &B.kv_full[slot], 64 * b, p % a.page, w.kvh, id);
                 }
-                p_v = p;
-                id_v = id;
             }
         }
         // copies in flight land before the block ends
-        for (uint32_t k = n > (uint32_t)C::NK ? n - C::NK : 0; k < n; k++) bar_wait(&B.kv_full[k % C::NK], (k / C::NK) & 1);
-        for (uint32_t k = n > (uint32_t)C::NV ? n - C::NV : 0; k < n && ok; k++) bar_wait(&B.kv_full[C::NK + k % C::NV], (k / C::NV) & 1);
+        for (uint32_t k = n > (uint32_t)slots ? n - slots : 0; k < n; k++) bar_wait(&B.kv_full[slot0 + k % slots], (k / slots) & 1);
         } else if (warp == C::W_QK) {
         // ---------------------------------------------------------------- products q k
         // Scores rotate through three buffers, so that new ones wait for the product p v that read their buffer, two
@@ -744,15 +733,15 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
 #pragma unroll 1
             for (int i = 0; i < w.n_it && ok; i++, n++) {
                 const uint32_t st = n % C::NK;
-                ok = bar_wait(&B.kv_full[st], (n / C::NK) & 1);
 #pragma unroll 1
-                for (int mt = 0; mt < (two ? 2 : 1) && ok; mt++) {
+                for (int mt = 0; mt < (two ? 2 : 1); mt++) {
                     const uint32_t b = n_buf % 3, use = n_buf / 3;
                     if (use > 0) ok = bar_wait(&B.s_free[b], (use - 1) & 1);
                     // A wait sees a phase by its parity, so none may complete twice between two looks. A tile's units take turns on two
                     // barriers: its scores may be two units ahead of its softmax, not three. With two tiles the buffer's turn sees to
                     // that, with one the product p v of the unit before the last has to be done.
                     if (ok && !two && n_buf >= 2) ok = bar_wait(&B.s_free[(n_buf - 2) % 3], ((n_buf - 2) / 3) & 1);
+                    if (ok && mt == 0) ok = bar_wait(&B.kv_full[st], (n / C::NK) & 1);
                     if (!ok) break;
                     n_buf++;
                     uint64_t* full = &B.s_full[mt][(mt ? n_s1++ : n_s0++) & 1];
@@ -816,7 +805,7 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
                     const uint32_t vd = desc_lo(kv_addr + st * C::STAGE, C::BLK), p = tm + b * UNIT;
                     if (elect()) {
 #pragma unroll
-                        for (int part = 0; part < C::PARTS + 1; part++)
+                        for (int part = 0; part < C::PARTS + 1; part++)  // low parts first
 #pragma unroll
                             for (int k = 0; k < UNIT / 16; k++)
                                 mma_tmem_a(tm + C::O_COL, p + 32 * (k >> 1) + (part ? 0 : 16) + 8 * (k & 1),

@@ -23,8 +23,8 @@ class Barrier:
 
 
 class Model:
-    def __init__(self, items, nk, nv, ahead, rng):
-        self.items, self.nk, self.nv, self.ahead, self.rng = items, nk, nv, ahead, rng
+    def __init__(self, items, nk, nv, apart, rng):
+        self.items, self.nk, self.nv, self.apart, self.rng = items, nk, nv, apart, rng
         b = lambda n, c=1: [Barrier(c) for _ in range(n)]  # noqa: E731
         self.kv_full, self.kv_empty = b(nk + nv), b(nk + nv)
         self.q_full, self.p_full, self.pv_done = b(2), b(2), b(2, 2)
@@ -33,30 +33,26 @@ class Model:
         self.score = [None] * 3         # what a score buffer holds: ("s" or "p", item, unit, tile)
         self.out = None                 # the output buffer
         self.q = [None, None]
-        self.queue = []                 # products and loads in flight: they end in order among the products, loads at any time
-        self.loads = []
+        self.queue = []                 # products in flight
+        self.loads = []                 # loads in flight, which land in any order
         self.summed = []
 
     # each warp is a generator that yields a condition to wait for, or None to let others run
-    def loader(self):
-        n = 0
+    def loader(self, kinds):
+        """The warp that fills the slots of k, that of v, or (32-bit pools) the warps that fill both in turn."""
+        n = {"k": 0, "v": 0}
         for it, (n_m, n_it) in enumerate(self.items):
-            for i in range(n_it + 1):
-                if i < n_it:
-                    s, use = n % self.nk, n // self.nk
+            for i in range(n_it):
+                for kind in kinds:
+                    slots = self.nv if kind == "v" else self.nk
+                    s, use = n[kind] % slots + (self.nk if kind == "v" else 0), n[kind] // slots
                     if use:
                         yield lambda: self.kv_empty[s].done((use - 1) & 1)
-                    self.loads.append((s, ("k", it, i)))
-                    n += 1
-                if not self.ahead and i == n_it:
-                    break
-                if i or not self.ahead:  # v of the unit before, or (32-bit pools) of the same unit
-                    nv = n - 2 if self.ahead and i < n_it else n - 1
-                    s, use = self.nk + nv % self.nv, nv // self.nv
-                    if use:
-                        yield lambda: self.kv_empty[s].done((use - 1) & 1)
-                    self.loads.append((s, ("v", it, i - 1 if self.ahead else i)))
-                yield None
+                    assert self.slot[s] is None
+                    self.slot[s] = "on its way"
+                    self.loads.append((s, (kind, it, i)))
+                    n[kind] += 1
+                    yield None
 
     def scores(self):
         n = buf = 0
@@ -66,8 +62,6 @@ class Model:
                 yield lambda: self.q_full[m].done(n_q[m] & 1)
                 n_q[m] += 1
             for i in range(n_it):
-                s = n % self.nk
-                yield lambda: self.kv_full[s].done((n // self.nk) & 1)
                 for m in range(n_m):
                     b, use = buf % 3, buf // 3
                     if use:
@@ -77,6 +71,9 @@ class Model:
                     buf += 1
                     full = self.s_full[m][n_s[m] & 1]
                     n_s[m] += 1
+                    s = n % self.nk
+                    if m == 0:
+                        yield lambda: self.kv_full[s].done((n // self.nk) & 1)
                     self.queue.append(("s", s, b, m, it, i, m == n_m - 1, full))
                     full.arrive()
                     yield None
@@ -94,9 +91,8 @@ class Model:
                         yield lambda: self.o_free.done((buf - 1) & 1)
                     yield lambda: self.p_full[m].done(n_p[m] & 1)
                     n_p[m] += 1
-                    b = buf % 3
+                    self.queue.append(("o", s, buf % 3, m, it, i, m == n_m - 1, None))
                     buf += 1
-                    self.queue.append(("o", s, b, m, it, i, m == n_m - 1, None))
                     self.pv_done[m].arrive()
                     yield None
                 n += 1
@@ -137,7 +133,11 @@ class Model:
         self.kv_full[s].arrive()
 
     def finish_product(self):
-        kind, s, b, m, it, i, last, full = self.queue.pop(0)
+        # products of one warp end in its order; those of the two warps in any
+        kinds = sorted({x[0] for x in self.queue})
+        kind = self.rng.choice(kinds)
+        at = next(k for k, x in enumerate(self.queue) if x[0] == kind)
+        kind, s, b, m, it, i, last, full = self.queue.pop(at)
         if kind == "s":
             assert self.slot[s] == ("k", it, i) and self.q[m] == it and self.score[b] is None
             self.score[b] = ("s", it, i, m)
@@ -153,7 +153,11 @@ class Model:
 
     def run(self, lazy):
         """lazy: the actor that is chosen least often."""
-        actors = {"load": self.loader(), "qk": self.scores(), "pv": self.values(), "s0": self.softmax(0), "s1": self.softmax(1)}
+        actors = {"qk": self.scores(), "pv": self.values(), "s0": self.softmax(0), "s1": self.softmax(1)}
+        if self.apart:
+            actors["k"], actors["v"] = self.loader("k"), self.loader("v")
+        else:
+            actors["k"] = self.loader("kv")
         waiting = {a: None for a in actors}
         while actors or self.loads or self.queue:
             ready = [a for a in actors if waiting[a] is None or waiting[a]()]
@@ -175,7 +179,7 @@ class Model:
 
 
 @pytest.mark.parametrize("nk,nv,two", [(2, 1, True), (4, 4, True), (1, 1, False)])  # 16-bit heads of 128 and 64, 32-bit
-@pytest.mark.parametrize("lazy", [None, "load", "qk", "pv", "s0", "s1", "land", "product"])
+@pytest.mark.parametrize("lazy", [None, "k", "v", "qk", "pv", "s0", "s1", "land", "product"])
 def test_every_schedule_ends(nk, nv, two, lazy):
     rng = random.Random(7)
     for _ in range(60):
