@@ -680,8 +680,11 @@ class PagedCache:
         """eahmmf_cuda_pages_copy: pairs (from, to) [n x 2] on the host, every layer, k and v."""
         st = self._go(None, stream)
         p = np.asarray(pairs)
-        if p.size % 2 or (p.size and (p.dtype.kind not in "iu" or p.min() < 0 or p.max() >= self.desc.n_pages)):
-            raise ValueError(f"pairs: [n x 2] page ids below {self.desc.n_pages} are needed")
+        if p.size % 2:
+            raise ValueError("pairs: [n x 2] page ids are needed")
+        if p.dtype != np.int32 and p.size:  # what another type holds has to survive the conversion
+            if p.dtype.kind not in "iu" or p.min() < 0 or p.max() >= self.desc.n_pages:
+                raise ValueError(f"pairs: [n x 2] page ids below {self.desc.n_pages} are needed")
         p = np.ascontiguousarray(p, np.int32)
         rc = self._lib.eahmmf_cuda_pages_copy(self._ref, p.ctypes.data, p.size // 2, st)
         if rc:
