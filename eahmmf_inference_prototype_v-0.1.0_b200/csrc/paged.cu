@@ -10,6 +10,8 @@
 //   k_pages_copy    page copies of a list of pairs, every layer, both pools
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
+#include <utility>
 
 #include "kernels.cuh"
 #include "paged.cuh"
@@ -25,10 +27,11 @@ namespace {
 //   (a, b) <- (a cos - b sin, a sin + b cos),  (a, b) = (x[i], x[i + n_rot/2]) or (x[2i], x[2i + 1]).
 // The angle and what is left of it after whole turns are in 64 bits (at p = 1e5 a 32-bit product is off by 4e-3 rad), its
 // sine and cosine in 32 bits, with the part of the remainder that 32 bits lose added to first order: within 2^-23. A
-// sincos in 64 bits cost 1.1 us of a step's 8 us and a seventh of a prompt's rate.
-// Bytes: 4 hd (n_head + 2 n_kv) in, 4 hd n_head + 2 hd n_kv es out per row; nothing is read twice.
+// sincos in 64 bits cost 1.1 us of the 8 us that a step's call took then, and a seventh of a prompt's rate.
+// Bytes: 4 hd (n_head + 2 n_kv) in, 4 hd n_head + 2 hd n_kv es out per row; nothing is read twice. Bound by them: 4,273 rows of 32
+// q and 4 kv heads of 128, 32-bit pages: 175 MB in 29.4 us (5.96 TB/s); 32 rows 4.8 us, a chain of dependent loads.
 constexpr int AP_NT = 256;
-constexpr int AP_PF = 5;  // head vectors a thread loads before it needs the row's sequence: 4,096 rows of 40 heads took 33.4 us with 4
+constexpr int AP_PF = 5;  // head vectors a thread loads before it needs the row's sequence: 4,273 rows of 40 heads took 33.4 us with 4
                           // and 32.8 with 6 (registers for one block fewer), 29.4 with 5
 
 __device__ __forceinline__ void store4(float* p, const float (&v)[4]) {
@@ -156,7 +159,8 @@ __global__ void __launch_bounds__(AP_NT) k_rope_append(PagedArgs a, EahmmfRope r
 // page copies
 // ------------------------------------------------------------------------------------------------
 // The pairs travel as a kernel argument: the list is in host memory, checked there, and the call neither
-// copies nor keeps anything. Bytes: each page read once and written once, in every layer, both pools.
+// copies nor keeps anything. Bytes: each page read once and written once, in every layer, both pools: 501 pages of 64 KB in 8
+// layers, 1.05 GB, in 164 us (6.4 TB/s).
 constexpr int CP_NT = 256, CP_VEC = 4;  // 16-byte vectors a thread has in flight
 constexpr int CP_PAIRS = 480;           // 3840 bytes of the 4 KB that every kernel's arguments may take
 struct CopyList {
@@ -189,7 +193,9 @@ __global__ void __launch_bounds__(CP_NT) k_pages_copy(uint4* __restrict__ k, uin
 // joined by their (m, sum, o).
 //
 // A step reads 2 hd es bytes per position and kv head and does 4 hd flops per q head with them: it is bound by
-// the reads. Every warp has its own positions and its own ring of tiles in shared memory, which it fills ahead by
+// the reads. 2 sequences of 131,000 positions, 4 kv heads of 128, 16-bit pages: 533 MB in 88 us (6.0 TB/s), with the joining
+// launch 92; 32 sequences of 300 to 4,500: 138 MB in 35 us, of which 5 before the first reads and 5 joining. 32-bit pages wait
+// for the splitting below: 32 sequences of 200 to 2,050, 101 MB in 31 us. Every warp has its own positions and its own ring of tiles in shared memory, which it fills ahead by
 // asynchronous 16-byte copies: no barrier between warps. A tile keeps rows of 128 bytes with exchanged 16-byte chunks
 // (chunk c of row r at c ^ (r mod 8)); the sums run over hd and over positions, whose order is free, and so is the order of
 // the output's columns, so a thread's operands of several instructions are one 16-byte load without bank conflicts.
@@ -240,8 +246,7 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
     hi = h2(hx, hy);
     lo = h2(__float2half_rn(x - __half2float(hx)), __float2half_rn(y - __half2float(hy)));
 }
-// x as two parts of 11 bits, hi rounded and lo cut, in integer instructions (the conversion instruction runs at a quarter of
-// their rate): at most 2^-21 of x is left out, with either sign. An infinity or a NaN gives a NaN.
+// x as two parts of 11 bits, hi rounded and lo cut, in integer instructions: at most 2^-21 of x is left out, with either sign. An infinity or a NaN gives a NaN.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
     hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
@@ -355,7 +360,7 @@ __device__ __forceinline__ void store_joined(const PagedAttnArgs& A, const Joine
     *reinterpret_cast<float4*>(A.out + (size_t)(q0 + tok) * A.ldo + (size_t)(kvh * A.c.grp + row - tok * A.c.grp) * hd + 4 * c4) =
         make_float4(j.o.x * inv, j.o.y * inv, j.o.z * inv, j.o.w * inv);
 }
-template <typename T, int HD, bool STACK>
+template <typename T, int HD, bool STACK, bool WHOLE>
 __global__ void __launch_bounds__(PA_NT, STEP_BLOCKS) k_paged_attn(PagedAttnArgs A) {
     constexpr bool H16 = sizeof(T) == 2;
     constexpr int STEP = pos_step<T>(), UNIT = STEP * PA_NW, RT = STACK ? 8 : 16, NR = STACK ? 1 : 2;
@@ -377,68 +382,88 @@ __global__ void __launch_bounds__(PA_NT, STEP_BLOCKS) k_paged_attn(PagedAttnArgs
     pdl_wait();
     pdl_trigger();
 
-    // ---- this block's share of the call: work items in (sequence, kv head, row tile, unit) order, or whole row tiles
-    auto weight = [&](int s, bool flag) -> long long {
-        const Seq sq = paged_seq(a, s, flag);
-        if (!step_takes(A, sq)) return 0;
-        const int n = A.whole ? 1 : units_of(sq, A.window, A.n_sink, UNIT).n();
-        return (long long)n * a.n_kv * ((sq.q * a.grp + RT - 1) / RT);
-    };
-    long long total = 0, mine = 0, upto = 0;  // of thread's sequence s0 + tid: its weight, and the sum with it
-    auto scan = [&](int s0, bool flag) {
-        mine = s0 + tid < a.n_seq ? weight(s0 + tid, flag) : 0;
-        upto = mine;
+    // ---- this block's share of the call: work items in (sequence, kv head, row tile, unit) order; or, where tiles stay whole,
+    // every gridDim-th (sequence, kv head) with its row tiles, which needs no sums over the sequences (a kernel of its own: as a
+    // branch it took registers that the other needs, 31.1 instead of 29.7 us for 32 sequences over 32-bit pages)
+    long long share = 0, begin = 0, end = 0;
+    if constexpr (!WHOLE) {
+        auto weight = [&](int s, bool flag) -> long long {
+            const Seq sq = paged_seq(a, s, flag);
+            if (!step_takes(A, sq)) return 0;
+            return (long long)units_of(sq, A.window, A.n_sink, UNIT).n() * a.n_kv * ((sq.q * a.grp + RT - 1) / RT);
+        };
+        long long total = 0, mine = 0, upto = 0;  // of thread's sequence s0 + tid: its weight, and the sum with it
+        auto scan = [&](int s0, bool flag) {
+            mine = s0 + tid < a.n_seq ? weight(s0 + tid, flag) : 0;
+            upto = mine;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long n = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += n;
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long n = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += n;
+            }
+            __syncthreads();  // s_scan is read
+            if (lane == 31) s_scan[warp] = upto;
+            __syncthreads();
+            upto += total;
+            for (int w = 0; w < PA_NW; w++) {
+                if (w < warp) upto += s_scan[w];
+                total += s_scan[w];
+            }
+        };
+        for (int s0 = 0; s0 < a.n_seq; s0 += PA_NT) scan(s0, blockIdx.x == 0);
+        const long long all = total;
+        share = max(div64(all + gridDim.x - 1, gridDim.x), (long long)(A.min_units));
+        begin = share * blockIdx.x;
+        end = min(all, begin + share);
+        if (tid == 0) A.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+        if (begin >= all) return;
+        total = 0;
+        for (int s0 = 0; s0 < a.n_seq && total <= begin; s0 += PA_NT) {  // the sequence that holds `begin`
+            if (a.n_seq > PA_NT)
+                scan(s0, false);
+            else
+                total = all;
+            if (mine > 0 && upto - mine <= begin && begin < upto) {
+                s_seq = s0 + tid;
+                s_start = upto - mine;
+            }
         }
-        __syncthreads();  // s_scan is read
-        if (lane == 31) s_scan[warp] = upto;
         __syncthreads();
-        upto += total;
-        for (int w = 0; w < PA_NW; w++) {
-            if (w < warp) upto += s_scan[w];
-            total += s_scan[w];
-        }
-    };
-    for (int s0 = 0; s0 < a.n_seq; s0 += PA_NT) scan(s0, blockIdx.x == 0);
-    const long long all = total, share = max(div64(all + gridDim.x - 1, gridDim.x), (long long)(A.min_units));
-    const long long begin = share * blockIdx.x, end = min(all, begin + share);
-    if (tid == 0) A.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-    if (begin >= all) return;
-    total = 0;
-    for (int s0 = 0; s0 < a.n_seq && total <= begin; s0 += PA_NT) {  // the sequence that holds `begin`
-        if (a.n_seq > PA_NT)
-            scan(s0, false);
-        else
-            total = all;
-        if (mine > 0 && upto - mine <= begin && begin < upto) {
-            s_seq = s0 + tid;
-            s_start = upto - mine;
-        }
     }
-    __syncthreads();
-    int seq = s_seq;
-    long long seq_at = s_start;
+    long long seq_at = WHOLE ? 0 : s_start, at = begin;
+    long long pick = blockIdx.x;  // whole tiles: sequence * n_kv + kv head, and the row tile
+    int seq = WHOLE ? (int)div64(pick, a.n_kv) : s_seq, kvh = (int)(pick - (long long)seq * a.n_kv), rt = 0;
     const T* kp = static_cast<const T*>(a.k);
     const T* vp = static_cast<const T*>(a.v);
 
-    for (long long at = begin; at < end && seq < a.n_seq;) {
-        const Seq sq = paged_seq(a, seq, false);
+    while ((WHOLE || at < end) && seq < a.n_seq) {
+        const Seq sq = paged_seq(a, seq, WHOLE && kvh == 0 && rt == 0 && tid == 0);
         const Units un = units_of(sq, A.window, A.n_sink, UNIT);
-        const int nu = un.n(), ticks = A.whole ? 1 : nu, nrt = (sq.q * a.grp + RT - 1) / RT;
-        const long long here = (long long)ticks * nrt * a.n_kv;
-        const bool takes = step_takes(A, sq);
-        if (!takes || at >= seq_at + here) {
-            if (takes) seq_at += here;
-            seq++;
-            continue;
+        const int nu = un.n(), nrt = (sq.q * a.grp + RT - 1) / RT;
+        int u0 = 0, n_it = nu;
+        if constexpr (WHOLE) {
+            if (rt >= nrt || !step_takes(A, sq)) {
+                pick += gridDim.x;
+                seq = (int)div64(pick, a.n_kv);
+                kvh = (int)(pick - (long long)seq * a.n_kv);
+                rt = 0;
+                continue;
+            }
+        } else {
+            const long long here = (long long)nu * nrt * a.n_kv;
+            const bool takes = step_takes(A, sq);
+            if (!takes || at >= seq_at + here) {
+                if (takes) seq_at += here;
+                seq++;
+                continue;
+            }
+            const long long idx = at - seq_at;
+            const int item = (int)div64(idx, nu);
+            u0 = (int)(idx - (long long)item * nu);
+            kvh = item / nrt;
+            rt = item - kvh * nrt;
+            n_it = (int)min((long long)(nu - u0), end - at);
         }
-        const long long idx = at - seq_at;
-        const int item = (int)div64(idx, ticks), u0 = (int)(idx - (long long)item * ticks);
-        const int kvh = item / nrt, rt = item - kvh * nrt;
-        const int n_it = A.whole ? nu : (int)min((long long)(nu - u0), end - at);
         // ---- the row tile: rows r0 .. of (token, q head of the group)
         const int r0 = rt * RT, n_rows = min(RT, sq.q * a.grp - r0), p_first = sq.kv - sq.q;
         const int lim_max = p_first + (r0 + n_rows - 1) / a.grp, first_pos = p_first + r0 / a.grp;
@@ -764,7 +789,7 @@ __global__ void __launch_bounds__(PA_NT, STEP_BLOCKS) k_paged_attn(PagedAttnArgs
             }
         }
         __syncthreads();
-        const bool whole = u0 == 0 && n_it == nu;
+        const bool whole = WHOLE || (u0 == 0 && n_it == nu);
         float* rec = A.part + ((size_t)blockIdx.x * 2 + (u0 == 0 ? 1 : 0)) * part_floats(HD);
         for (int i = tid; i < n_rows * (HD / 4); i += PA_NT) {
             const int r = i / (HD / 4), c4 = i - r * (HD / 4);
@@ -801,7 +826,10 @@ __global__ void __launch_bounds__(PA_NT, STEP_BLOCKS) k_paged_attn(PagedAttnArgs
         if (!whole && u0 == 0 && tid == 0)  // the blocks after this one hold the rest of the tile
             A.meta[blockIdx.x] = make_int4(((int)div64(at + nu - 1, share) - blockIdx.x) | n_rows << 16, sq.q0, kvh, r0);
         __syncthreads();
-        at += A.whole ? 1 : n_it;
+        if constexpr (WHOLE)
+            rt++;
+        else
+            at += n_it;
     }
 }
 
@@ -838,20 +866,31 @@ __global__ void __launch_bounds__(PM_NT) k_paged_merge(PagedAttnArgs A, int cap)
     store_joined(A, j, me.y, me.z, me.w + r, HD, lane);
 }
 
-// Up to this many positions a row tile is one block's work: cutting it would save less than joining it costs.
-constexpr int WHOLE_KV = 512;
+// Up to this many positions a row tile is one block's work: cutting it would save less than joining it costs. Heads of 128, 4
+// kv heads, whole and cut: one sequence over 16-bit pages 11.6 and 15.6 us at 700 positions, 13.9 and 15.4 at 900, 14.8 and 12.7
+// at 1,000; over 32-bit pages 14.5 and 16.4 at 320, 17.0 and 14.5 at 380. With more tiles than blocks some blocks take two, and
+// a cut pays sooner: 128 sequences over 16-bit pages 26.7 and 30.0 at 400, 33.7 and 31.6 at 500; over 32-bit pages 31.3 and
+// 33.4 at 200, 39.5 and 34.9 at 256.
+int whole_kv(int es, bool block_each) { return es == 2 ? (block_each ? 896 : 448) : (block_each ? 352 : 224); }
 int step_grid() { return STEP_BLOCKS * sm_count(); }
 
+template <typename T, int HD, bool STACK, bool WHOLE>
+cudaError_t attn_launch(const PagedAttnArgs& A, int blocks, cudaStream_t st) {
+    using Smem = AttnSmem<T, HD, STACK>;
+    using Tag = std::pair<Smem, std::bool_constant<WHOLE>>;
+    cudaError_t e = smem_limit<Tag>(k_paged_attn<T, HD, STACK, WHOLE>, sizeof(Smem));
+    return e == cudaSuccess ? launch_pdl(k_paged_attn<T, HD, STACK, WHOLE>, dim3(blocks), dim3(PA_NT), sizeof(Smem), st, A) : e;
+}
 template <typename T, int HD, bool STACK>
 cudaError_t attn_go(PagedAttnArgs A, int max_kv, cudaStream_t st) {
     constexpr int RT = STACK ? 8 : 16;
-    cudaError_t e = smem_limit<AttnSmem<T, HD, STACK>>(k_paged_attn<T, HD, STACK>, sizeof(AttnSmem<T, HD, STACK>));
-    if (e != cudaSuccess) return e;
     A.grid = step_grid();
-    A.whole = max_kv <= WHOLE_KV;
-    A.min_units = A.whole ? 1 : 4;
-    e = launch_pdl(k_paged_attn<T, HD, STACK>, dim3(A.grid), dim3(PA_NT), sizeof(AttnSmem<T, HD, STACK>), st, A);
-    if (e != cudaSuccess || A.whole) return e;
+    A.min_units = 4;
+    const long long heads = (long long)A.c.n_seq * A.c.n_kv;
+    if (max_kv <= whole_kv((int)sizeof(T), heads <= A.grid))
+        return attn_launch<T, HD, STACK, true>(A, (int)std::min<long long>(heads, A.grid), st);
+    cudaError_t e = attn_launch<T, HD, STACK, false>(A, A.grid, st);
+    if (e != cudaSuccess) return e;
     // A launch of its own joins the pieces: few tiles, each in many, with a row's pieces dealt over a block; many tiles, each in
     // two or three, with a row to each group. (The block that ends last joining them within the launch took 36.3 instead of
     // 34.7 us for 32 sequences of 300 to 4,500 positions: the fences of every piece cost more than the launch.)

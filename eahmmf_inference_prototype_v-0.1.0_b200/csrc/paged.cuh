@@ -43,7 +43,7 @@ struct Seq {
 };
 __device__ __forceinline__ Seq paged_seq(const PagedArgs& a, int s, bool flag) {
     const int c0 = a.cu_q[s], c1 = a.cu_q[s + 1], n = a.kv_len[s];
-    const long long cap = (long long)a.table_ld * a.page;
+    const long long cap = min((long long)a.table_ld * a.page, 0x7fff0000ll);
     Seq r;
     r.q0 = min(max(c0, 0), a.n_tok);
     r.q = min(max(c1, r.q0), a.n_tok) - r.q0;
@@ -64,7 +64,6 @@ struct PagedAttnArgs {
     int window, n_sink;  // window 0: every earlier position is visible
     int grid;            // blocks of the split launch, also the records of `part`
     int min_units;       // least share of a block
-    bool whole;          // step kernel: row tiles are not cut
     int rows_min, rows_max;  // sequences of more rows (tokens x q heads of a kv head) than rows_min go to the chunk
                              // kernel, of at most rows_max to the step kernel
     float* part;         // [grid][2] partial results

@@ -277,6 +277,14 @@ def test_many_sequences(torch, type, q):
     Call(torch, type, 64, 1, 2, 16, qs, tuple(m + (7 * i) % 61 for i, m in enumerate(qs)), seed=15).check()
 
 
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("n_kv,grp,longest", [(1, 2, 1500), (1, 16, 1100), (3, 5, 300), (2, 8, 700)])
+def test_many_sequences_with_a_few_long_ones(torch, type, n_kv, grp, longest):  # tiles cut, or whole with several a block
+    lens = tuple(longest - i % 13 if i % 61 == 60 else 1 + (11 * i) % 47 for i in range(300))
+    qs = tuple((0 if i % 7 == 3 else 1) for i in range(300))
+    Call(torch, type, 64, n_kv, grp, 16, qs, lens, seed=18).check()
+
+
 def test_the_first_call_of_a_process_may_be_captured(torch):
     code = """
 import sys; sys.path[:0] = [%r, %r]
