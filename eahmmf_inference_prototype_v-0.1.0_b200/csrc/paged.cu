@@ -467,8 +467,8 @@ __global__ void __launch_bounds__(PA_NT, STEP_BLOCKS) k_paged_attn(PagedAttnArgs
         // ---- the row tile: rows r0 .. of (token, q head of the group)
         const int r0 = rt * RT, n_rows = min(RT, sq.q * a.grp - r0), p_first = sq.kv - sq.q;
         const int lim_max = p_first + (r0 + n_rows - 1) / a.grp, first_pos = p_first + r0 / a.grp;
-        const int low_min = A.window > 0 ? first_pos - A.window + 1 : 0;
-        const int lim_min = first_pos, low_max = A.window > 0 ? lim_max - A.window + 1 : 0;
+        const int low_min = A.window > 0 ? max(first_pos, 0) - A.window + 1 : 0;  // a row before position 0 sees nothing
+        const int lim_min = first_pos, low_max = A.window > 0 ? max(lim_max, 0) - A.window + 1 : 0;
         auto any = [&](int j) { return j <= lim_max && (j >= low_min || j < A.n_sink); };
 
         // ---- k and v of a step: page ids of 32 steps at a time, one per lane, the next 32 fetched ahead
@@ -537,7 +537,7 @@ __global__ void __launch_bounds__(PA_NT, STEP_BLOCKS) k_paged_attn(PagedAttnArgs
         for (int i = 0; i < NR; i++) {
             const int r = g + 8 * i;
             lim[i] = r < n_rows ? p_first + (r0 + r) / a.grp : -1;
-            low[i] = A.window > 0 ? lim[i] - A.window + 1 : 0;
+            low[i] = A.window > 0 ? max(lim[i], 0) - A.window + 1 : 0;
             const bool ok = r < n_rows;
             const float* qr = ok ? q_row(r) : nullptr;
             float x[KS * (H16 ? 4 : 2)];  // the thread's elements of the row, in k-step order

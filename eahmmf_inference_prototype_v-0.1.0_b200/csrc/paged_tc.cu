@@ -209,7 +209,7 @@ __device__ __forceinline__ Pair pair_of(const PagedAttnArgs& A, const Seq& sq, i
     p.t1 = min(sq.q, p.t0 + tok);
     const int first = sq.kv - sq.q + p.t0;
     p.lim_max = sq.kv - sq.q + p.t1 - 1;
-    p.low_min = A.window > 0 ? first - A.window + 1 : 0;
+    p.low_min = A.window > 0 ? max(first, 0) - A.window + 1 : 0;  // a row before position 0 sees nothing
     p.ue = (max(p.lim_max, -1) + UNIT) / UNIT;
     p.uw = min(max(0, p.low_min) / UNIT, p.ue);
     p.us = A.window > 0 ? min((min(A.n_sink, max(p.lim_max, -1) + 1) + UNIT - 1) / UNIT, p.uw) : 0;
@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
             const bool row_ok = r < tpt * a.grp && tok < w.pr.t1;
             const int head = w.kvh * a.grp + r % a.grp;
             const int lim = row_ok ? w.sq.kv - w.sq.q + tok : -1;
-            const int low = A.window > 0 ? max(0, lim - A.window + 1) : 0;
+            const int low = A.window > 0 ? max(0, max(lim, 0) - A.window + 1) : 0;
             // ---- q: a warp's rows scaled by the power of two that brings their largest to [2^14, 2^15), then split. The low
             // parts are exact to 2^-25 of that, 2^-39 of the largest row: in a score an absolute error of 2^-39 of the
             // warp's largest, far below that of 32 bits. Rows come one (hd 128) or two (hd 64) to a load instruction.

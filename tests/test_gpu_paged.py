@@ -166,6 +166,13 @@ def test_windows_and_sinks(torch, type, hd, grp, page, window, sinks, lens):
     c.check(window=window, n_sink=sinks)
 
 
+@pytest.mark.parametrize("type,hd,grp", [("f16", 128, 8), ("f32", 64, 2), ("f16", 64, 1)])
+@pytest.mark.parametrize("window", [1, 7, (1 << 31) - 9, (1 << 31) - 1])
+@pytest.mark.parametrize("lens", [((12, 5, 1), (3, 1, 0)), ((40, 3, 150), (20, 1, 140)), ((300,), (270,))])
+def test_more_rows_than_positions_in_a_window(torch, type, hd, grp, window, lens):
+    Call(torch, type, hd, 2, grp, 16, *lens, seed=19).check(window=window, n_sink=2)
+
+
 @pytest.mark.parametrize("type", ["f16", "f32"])
 def test_long_sequences_are_split_and_joined(torch, type):
     c = Call(torch, type, 128, 2, 8, 64, (1, 1), (9001, 37), seed=5)
