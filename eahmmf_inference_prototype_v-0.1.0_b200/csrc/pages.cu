@@ -4,6 +4,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <memory>
 #include <new>
 #include <vector>
 
@@ -227,7 +228,7 @@ extern "C" EahmmfPages* eahmmf_pages_create(int n_pages, int page, int n_seq, in
         (long long)max_pages * page > 0x7fffffffLL)
         return nullptr;
     try {
-        EahmmfPages* p = new EahmmfPages();
+        std::unique_ptr<EahmmfPages> p(new EahmmfPages());
         std::vector<std::vector<int>> ids(n_seq);
         p->n_pages = p->n_free = n_pages;
         p->page = page;
@@ -240,7 +241,7 @@ extern "C" EahmmfPages* eahmmf_pages_create(int n_pages, int page, int n_seq, in
         p->len.assign(n_seq, 0);
         for (auto& v : ids) v.reserve(std::min(max_pages, 64));
         p->ids.swap(ids);
-        return p;
+        return p.release();
     } catch (const std::bad_alloc&) {
         return nullptr;
     }

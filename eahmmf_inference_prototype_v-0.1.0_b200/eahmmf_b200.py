@@ -566,7 +566,7 @@ class Rope:
 
     def __init__(self, inv_freq, style: str = "half", mscale: float = 1.0):
         _dev_tensor(inv_freq, "inv_freq", "float32")
-        self._keep = inv_freq
+        self._keep, self.index = inv_freq, inv_freq.device.index
         self.desc = EahmmfRope(ROPE_STYLES[style], 2 * inv_freq.numel(), mscale, inv_freq.data_ptr())
         self._ref = C.addressof(self.desc)
 
@@ -616,7 +616,7 @@ class PagedCache:
         self._lib = lib()
         # what a call of a few microseconds looks up, once
         self._append, self._attention = self._lib.eahmmf_cuda_rope_append, self._lib.eahmmf_cuda_paged_attention
-        self._f32, self._idx = torch.float32, k.device.index
+        self._f32, self._i32, self._idx = torch.float32, torch.int32, k.device.index
         self._device_now, self._stream_now = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
     def _go(self, batch, stream):
@@ -634,6 +634,13 @@ class PagedCache:
             raise ValueError(f"{name}: float32 rows [{batch.n_tok} x {width}] on {self.device} are needed")
         return x.data_ptr(), stride[0] if shape[0] > 1 else width
 
+    def _status(self, t):
+        if t is None:
+            return None
+        if t.get_device() != self._idx or t.dtype is not self._i32 or t.numel() < 1:
+            raise ValueError(f"d_status: an int32 tensor on {self.device} is needed")
+        return t.data_ptr()
+
     def _norm(self, w, name: str):
         if w is None:
             return None
@@ -646,10 +653,12 @@ class PagedCache:
         """eahmmf_cuda_rope_append: rows qkv [n_tok x (n_head + 2 n_kv) hd] normalised (where weights are given) and
         rotated; q into q_out [n_tok x n_head hd], k and v into the pages of their positions."""
         st = self._go(batch, stream)
+        if rope.index != self._idx:
+            raise ValueError(f"the frequency table lives on cuda:{rope.index}, the cache on {self.device}")
         x, ld = self._rows(qkv, "qkv", batch, (n_head + 2 * self.n_kv) * self.hd)
         q, ldq = self._rows(q_out, "q_out", batch, n_head * self.hd)
         rc = self._append(self._ref, layer, batch._ref, rope._ref, n_head, x, ld, self._norm(q_norm, "q_norm"),
-                          self._norm(k_norm, "k_norm"), eps, q, ldq, st, None if d_status is None else d_status.data_ptr())
+                          self._norm(k_norm, "k_norm"), eps, q, ldq, st, self._status(d_status))
         if rc:
             raise RuntimeError(f"eahmmf_cuda_rope_append returned {rc}")
 
@@ -668,11 +677,10 @@ class PagedCache:
             if stream is not None:
                 raise ValueError("ws: a workspace is needed with a stream of the caller's")
             ws = self.attention_workspace(batch, n_head)
-        elif ws.get_device() != self._idx:
-            raise ValueError(f"ws: a workspace on {self.device} is needed")
+        elif ws.get_device() != self._idx or not ws.is_contiguous():
+            raise ValueError(f"ws: a contiguous workspace on {self.device} is needed")
         rc = self._attention(self._ref, layer, batch._ref, n_head, x, ldq, self.hd ** -0.5 if scale is None else scale, window,
-                             n_sink, y, ldo, ws.data_ptr(), ws.numel() * ws.element_size(), st,
-                             None if d_status is None else d_status.data_ptr())
+                             n_sink, y, ldo, ws.data_ptr(), ws.numel() * ws.element_size(), st, self._status(d_status))
         if rc:
             raise RuntimeError(f"eahmmf_cuda_paged_attention returned {rc}")
 
@@ -680,7 +688,7 @@ class PagedCache:
         """eahmmf_cuda_pages_copy: pairs (from, to) [n x 2] on the host, every layer, k and v."""
         st = self._go(None, stream)
         p = np.asarray(pairs)
-        if p.size % 2:
+        if p.size and (p.ndim != 2 or p.shape[1] != 2):
             raise ValueError("pairs: [n x 2] page ids are needed")
         if p.dtype != np.int32 and p.size:  # what another type holds has to survive the conversion
             if p.dtype.kind not in "iu" or p.min() < 0 or p.max() >= self.desc.n_pages:

@@ -281,7 +281,9 @@ int eahmmf_cuda_rope_append(const EahmmfPagedKv* kv, int layer, const EahmmfPage
  * of those j > p - window or j < n_sink. A row that sees nothing is zero. Positions that no row of a sequence's call
  * sees may hold anything; a NaN or an infinity in v at a position that a later row of the same call sees can reach
  * earlier rows of that sequence. n_head a multiple of n_kv, at most 64 q heads per kv head; row strides multiples of 4,
- * buffers 16-byte aligned. The workspace (256-byte aligned) is written and read within the call: calls that may run at
+ * buffers 16-byte aligned, d_out not overlapping d_q. Over 32-bit pages the products of more than 16 rows (tokens x q heads of
+ * a kv head) hold an element of k and v to 2^-22 of itself or 2^-39 of the largest among its 128 positions, whichever is more.
+ * Elements of q, k and v stay below 2^100. The workspace (256-byte aligned) is written and read within the call: calls that may run at
  * the same time need one each. Asynchronous; results do not depend on what else runs. */
 size_t eahmmf_cuda_paged_attention_workspace_bytes(const EahmmfPagedKv* kv, const EahmmfPagedSeqs* seqs, int n_head);
 int eahmmf_cuda_paged_attention(const EahmmfPagedKv* kv, int layer, const EahmmfPagedSeqs* seqs, int n_head,
@@ -301,7 +303,8 @@ int eahmmf_cuda_pages_copy(const EahmmfPagedKv* kv, const int* pairs, int n, voi
  *  - extend: positions up to len (not below the present length) get pages, the lowest free ones; a part-filled last
  *    page that another sequence shares is replaced by a copy of it (recorded). EAHMMF_ST_CAPACITY: not enough free
  *    pages, or more than max_pages;
- *  - fork: the empty sequence dst takes src's length and shares its pages;
+ *  - fork: the empty sequence dst takes src's length and shares its pages (rows of src that a step is still to append are
+ *    not in a copy that dst needs in the same step: append them first);
  *  - truncate: the sequence is cut to len positions (0 empties it), pages behind them are given back; not into the
  *    middle of a page that slide gave back (EAHMMF_ST_BAD_ARG);
  *  - slide: pages wholly before first_pos and wholly behind the first n_sink positions are given back (a window has

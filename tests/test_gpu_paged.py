@@ -311,6 +311,29 @@ for q in ((1,), (40,)):
     assert r.returncode == 0, r.stderr[-2000:]
 
 
+def test_calls_check_status_workspace_and_table(torch):
+    c = Call(torch, "f16", 64, 2, 2, 16, (2,), (20,), seed=17)
+    x, rope = torch.randn(2, 8 * 64, device="cuda"), eb.Rope(torch.ones(32, device="cuda"))
+    for status in (torch.zeros(1, dtype=torch.int32), c.status.long(), c.status[:0]):
+        with pytest.raises(ValueError):
+            c.cache.attention(0, c.batch, c.q, c.n_head, c.out, d_status=status)
+        with pytest.raises(ValueError):
+            c.cache.append(0, c.batch, x, c.n_head, rope, c.out, d_status=status)
+    ws = c.cache.attention_workspace(c.batch, c.n_head)
+    for bad in (ws.cpu(), torch.cat([ws, ws])[::2]):
+        with pytest.raises(ValueError):
+            c.cache.attention(0, c.batch, c.q, c.n_head, c.out, ws=bad)
+    with pytest.raises(RuntimeError):
+        c.cache.attention(0, c.batch, c.q, c.n_head, c.out, ws=ws[:-256])
+    rope.index += 1  # as of a table on another device
+    with pytest.raises(ValueError):
+        c.cache.append(0, c.batch, x, c.n_head, rope, c.out)
+    for pairs in ([0, 1], [[[0, 1]]], [[0], [1]]):
+        with pytest.raises(ValueError):
+            c.cache.copy_pages(pairs)
+    c.cache.copy_pages([])
+
+
 def test_calls_check_their_tensors(torch):
     c = Call(torch, "f16", 64, 2, 2, 16, (2,), (20,), seed=17)
     for bad in (c.q.double(), c.q[:1], c.q[:, :-4], c.q.cpu(), c.q.t()):
