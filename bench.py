@@ -985,6 +985,13 @@ def main():
     rank, world = int(os.environ.get("RANK", 0)), int(os.environ.get("WORLD_SIZE", 1))
     local = int(os.environ.get("LOCAL_RANK", 0))
 
+    if not os.path.exists(os.path.join(ORACLE, "_ref", "libeahmmf_ref.so")):  # built where the reference's sources are
+        if args.impl == "reference":
+            if rank == 0:
+                print(json.dumps({"impl": "reference", "unavailable": "the reference is not built here (oracle/_ref)"}), flush=True)
+            return 0
+        args.no_cpu = True
+
     if args.impl == "reference" and decode:
         if rank != 0:
             return 0
