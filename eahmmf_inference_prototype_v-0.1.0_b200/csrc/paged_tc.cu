@@ -14,7 +14,7 @@
 // Bound: 4 hd flops per row and position, twice because of the two parts: 2 * 2 * 2 * 128 * 128 * hd per tile and unit. Two
 // tiles share every k and v tile and take turns: while one tile's scores are in the softmax the other's products run.
 // 4,096 tokens over 12,289 positions, 32 q heads of 128 on 4 kv heads, 16-bit pages: 985 us in a burst (1,397 TFLOP/s of both parts),
-// 1,157 back to back, where the power cap holds the clock at 1.55 GHz. 64 tokens over 2,111 positions of 32-bit pages: 36 us,
+// 1,158 back to back, where the power cap holds the clock at 1.55 GHz. 64 tokens over 2,111 positions of 32-bit pages: 35 us,
 // two units a block, most of it start, q and joining.
 //
 // Warps: 0-3 softmax of tile 0, 4-7 of tile 1 (thread = row = tensor-memory lane), 8 loads k, 11 loads v, 9 issues q k, 10 issues
