@@ -60,6 +60,31 @@ struct Tc {
     static constexpr int REGS = F32 ? 128 : 168, REGS_SOFTMAX = 208, REGS_LOAD = F32 ? 104 : 88, REGS_ISSUE = F32 ? 96 : 88;
 };
 static_assert(128 * (2 * 208 + 88) == 384 * 168 && 128 * (208 + 2 * 104 + 96) == 512 * 128, "register shares");
+
+// Bytes of a row tile's q (q_lo, then q_hi: 2 HALVES column blocks of 128 rows of 128 bytes) that a softmax warp writes. Its next q
+// is in q_at's layout; before that its 32 rows of the output pass through the same bytes, in stage_at's. Nothing but the warp's own
+// order keeps the two apart, so they have to lie within the rows of the warp: no other warp of the tile writes or reads there.
+__host__ __device__ constexpr int q_at(int row, int ch) {  // 16-byte chunk ch (8 f16) of a row of q_lo or q_hi
+    return (ch >> 3) * 128 * 128 + row * 128 + (((ch & 7) ^ (row & 7)) << 4);
+}
+__host__ __device__ constexpr int stage_at(int row, int c) {  // 16-byte chunk c (4 floats) of a row of the output
+    return (c >> 3) * 128 * 128 + row * 128 + (((c & 7) ^ (row & 7)) << 4);
+}
+template <int HD, bool F32>
+constexpr bool stage_stays_in_the_rows_of_its_warp() {
+    for (int row = 0; row < MROWS; row++)
+        for (int c = 0; c < HD / 4; c++) {
+            const int at = stage_at(row, c), block = at / Tc<HD, F32>::BLK, in = at % Tc<HD, F32>::BLK;
+            if (block >= 2 * Tc<HD, F32>::HALVES || in / 128 / 32 != row / 32) return false;
+        }
+    for (int row = 0; row < MROWS; row++)
+        for (int ch = 0; ch < HD / 8; ch++)
+            if (q_at(row, ch) % Tc<HD, F32>::BLK / 128 / 32 != row / 32) return false;
+    return true;
+}
+static_assert(stage_stays_in_the_rows_of_its_warp<64, false>() && stage_stays_in_the_rows_of_its_warp<128, false>() &&
+                  stage_stays_in_the_rows_of_its_warp<64, true>() && stage_stays_in_the_rows_of_its_warp<128, true>(),
+              "a warp's output passes through its own rows");
 struct Bars {
     uint64_t kv_full[8], kv_empty[8], q_full[2], s_full[2][2], p_full[2], pv_done[2], s_free[3], o_free;
     uint32_t valid[VALID_RING];                     // by unit: which boxes lie in pages of the pool
@@ -426,7 +451,7 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
                     const __half2 l0 = __floats2half2_rn(fmaf(f[i].x, sc, -b0.x), fmaf(f[i].y, sc, -b0.y)),
                                   l1 = __floats2half2_rn(fmaf(f[i].z, sc, -b1.x), fmaf(f[i].w, sc, -b1.y));
                     const int ch = el >> 1;  // 16-byte chunk
-                    const int at = (ch >> 3) * C::BLK + row * 128 + (((ch & 7) ^ (row & 7)) << 4) + (el & 1) * 8;
+                    const int at = q_at(row, ch) + (el & 1) * 8;
                     *reinterpret_cast<uint2*>(q_hi + at) =
                         make_uint2(*reinterpret_cast<const uint32_t*>(&h0), *reinterpret_cast<const uint32_t*>(&h1));
                     *reinterpret_cast<uint2*>(q_lo + at) =
@@ -546,8 +571,8 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
                 A.meta[blockIdx.x] = make_int4(((int)div64(tile_end - 1, share) - blockIdx.x) | (w.pr.t1 - w.pr.t0) * a.grp << 16, w.sq.q0, w.kvh,
                                                 w.pr.t0 * a.grp);
             }
-            // ---- the warp's rows through shared memory (their q is read), so that a row leaves as one run: to the output, or to
-            // this block's record (rows in (token, head) order: the two tiles' rows follow each other)
+            // ---- the warp's rows through the bytes of their own q (which is read), so that a row leaves as one run: to the output, or
+            // to this block's record (rows in (token, head) order: the two tiles' rows follow each other)
             const int rr = mt * tpt * a.grp + r;
             float* rec = A.part + ((size_t)blockIdx.x * 2 + (w.u0 == 0 ? 1 : 0)) * (256 * (HD + 2));
             float* dst = whole ? A.out + (size_t)(w.sq.q0 + (row_ok ? tok : w.pr.t0)) * A.ldo + (size_t)head * HD : rec + (size_t)rr * HD;
@@ -557,13 +582,13 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
             }
             const float f = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
             const uint64_t ff = f2(f, f);
-            float4* st = reinterpret_cast<float4*>(q_lo) + (size_t)32 * (warp & 3) * (HD / 4);  // [32 rows][hd / 4], chunks exchanged
+            uint8_t* st = q_lo + (r & ~31) * 128;  // row 0 of the warp's in every column block
 #pragma unroll
             for (int c = 0; c < HD / 4; c++) {
                 float4 v;
                 un2(fma2(acc[2 * c], ff, 0), v.x, v.y);
                 un2(fma2(acc[2 * c + 1], ff, 0), v.z, v.w);
-                st[lane * (HD / 4) + (c ^ (lane & 7))] = v;
+                *reinterpret_cast<float4*>(st + stage_at(lane, c)) = v;
             }
             __syncwarp();
             {
@@ -581,7 +606,7 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
                     for (int j = 0; j < AHEAD; j++) {
                         const int row = i + j * RPP + sub;
                         d[j] = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), row));
-                        v[j] = st[row * (HD / 4) + (el ^ (row & 7))];
+                        v[j] = *reinterpret_cast<const float4*>(st + stage_at(row, el));
                     }
 #pragma unroll
                     for (int j = 0; j < AHEAD; j++)
