@@ -34,6 +34,7 @@
 #include "common.cuh"
 #include "decode.cuh"
 #include "kernels.cuh"
+#include "paged.cuh"
 #include "sample.cuh"
 
 namespace eb {
@@ -1224,12 +1225,17 @@ struct EahmmfEngine {
         paged = std::move(made);
         return ST_OK;
     }
+    // The recorded copies of pages, which also frees the pages given back since the first of them.
+    int paged_copies() {
+        Paged& P = *paged;
+        const int n = eahmmf_pages_take_copies(P.pages, P.pairs.data(), (int)P.pairs.size() / 2);
+        return eahmmf_cuda_pages_copy(&P.kv, P.pairs.data(), n, st);
+    }
     // The sequences of a pass: n slots with rows q[i] (their last positions) on the device, after the copies that their pages
     // need. The staging is free: the caller has waited for the stream.
     int paged_begin(const int* slots, const int* rows, int n) {
         Paged& P = *paged;
-        const int n_copy = eahmmf_pages_take_copies(P.pages, P.pairs.data(), (int)P.pairs.size() / 2);
-        const int rc = eahmmf_cuda_pages_copy(&P.kv, P.pairs.data(), n_copy, st);
+        const int rc = paged_copies();
         if (rc != ST_OK) return rc;
         if (eahmmf_pages_table(P.pages, P.table.data(), P.max_pages, nullptr) != ST_OK) return ST_CAPACITY;
         int ld = 1, max_q = 0, max_kv = 0;
@@ -1285,6 +1291,7 @@ struct EahmmfEngine {
         if (rc != ST_OK) {
             P.len[slot] = p0;
             eahmmf_pages_truncate(P.pages, slot, p0);
+            paged_copies();  // none may stay recorded: pages given back would wait for the next pass
         }
         return rc;
     }
@@ -1664,21 +1671,20 @@ extern "C" int eahmmf_engine_step_slots(EahmmfEngine* e, int n, const int* slots
     int rc = ST_OK;
     if (e->paged) {
         auto& P = *e->paged;
-        int got = 0;
-        while (got < n && (rc = eahmmf_pages_extend(P.pages, slots[got], pos[got] + 1)) == ST_OK) got++;
-        if (got == n) {
-            int ones[MAXB];
-            for (int i = 0; i < n; i++) {
-                P.len[slots[i]] = pos[i] + 1;
-                ones[i] = 1;
-            }
-            rc = e->paged_begin(slots, ones, n);
+        rc = pages_grow(P.pages, slots, n);  // all of them, or none
+        if (rc != ST_OK) return rc;
+        int ones[MAXB];
+        for (int i = 0; i < n; i++) {
+            P.len[slots[i]] = pos[i] + 1;
+            ones[i] = 1;
         }
+        rc = e->paged_begin(slots, ones, n);
         if (rc != ST_OK) {  // no row is taken: the slots keep their lengths
-            for (int i = 0; i < got; i++) {
+            for (int i = 0; i < n; i++) {
                 P.len[slots[i]] = pos[i];
                 eahmmf_pages_truncate(P.pages, slots[i], pos[i]);
             }
+            e->paged_copies();
             return rc;
         }
     }

@@ -91,6 +91,10 @@ cudaError_t smem_limit(Kern k, size_t bytes) {
     return e;
 }
 
+// Every sequence of the list (each named once) grows by one position; where there are not enough pages for all of them
+// (ST_CAPACITY) none does, and no copy is recorded.
+int pages_grow(EahmmfPages* p, const int* seqs, int n);
+
 cudaError_t launch_pages_copy(const EahmmfPagedKv& kv, const int* pairs, int n, cudaStream_t st);
 
 }  // namespace eb

@@ -275,6 +275,34 @@ extern "C" int eahmmf_pages_extend(EahmmfPages* p, int seq, int len) {
     return ST_OK;
 }
 
+int eb::pages_grow(EahmmfPages* p, const int* seqs, int n) {
+    int want = 0;
+    for (int i = 0; i < n; i++) {
+        if (!seq_ok(p, seqs[i])) return ST_BAD_ARG;
+        const std::vector<int>& v = p->ids[seqs[i]];
+        const int at = p->len[seqs[i]] / p->page;
+        if (p->len[seqs[i]] % p->page == 0) {
+            if (at + 1 > p->max_pages) return ST_CAPACITY;
+            want++;
+        } else if (v[at] >= 0) {  // a copy, unless the rows before left this one the last holder
+            int holders = p->refs[v[at]];
+            for (int j = 0; j < i; j++) {
+                const int other = p->len[seqs[j]];
+                if (other % p->page && p->ids[seqs[j]][other / p->page] == v[at]) holders--;
+            }
+            want += holders > 1;
+        }
+    }
+    if (want > p->n_free) return ST_CAPACITY;
+    try {
+        for (int i = 0; i < n; i++) p->ids[seqs[i]].reserve(p->len[seqs[i]] / p->page + 1);
+    } catch (const std::bad_alloc&) {
+        return ST_CAPACITY;
+    }
+    for (int i = 0; i < n; i++) eahmmf_pages_extend(p, seqs[i], p->len[seqs[i]] + 1);  // which finds its pages and its room
+    return ST_OK;
+}
+
 extern "C" int eahmmf_pages_fork(EahmmfPages* p, int src, int dst) {
     if (!seq_ok(p, src) || !seq_ok(p, dst) || src == dst || !p->ids[dst].empty() || p->len[dst]) return ST_BAD_ARG;
     try {

@@ -1,0 +1,64 @@
+"""The pages of the engine's paged slots when a step is refused or fails: no row is taken, no page is lost, and what the slots give
+back can be taken again."""
+import os
+
+import numpy as np
+import pytest
+
+import eahmmf_b200 as eb
+import synth
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def kquant_path(tmp_path_factory):
+    import torch
+    if not torch.cuda.is_available():
+        pytest.fail("CUDA device required")
+    return synth.write_gguf(str(tmp_path_factory.mktemp("kp") / "ks.gguf"), synth.config_kquant_small())
+
+
+def test_a_refused_step_with_a_shared_page_loses_nothing(kquant_path):
+    e = eb.Engine(kquant_path, 100)
+    try:
+        assert e.set_paged(4, 4, 16, "f16") == 0
+        rc, a = e.prefill_slot(0, np.arange(20))
+        assert rc == 0 and e.fork_slot(0, 1, 20) == 0
+        rc, c = e.prefill_slot(2, np.arange(16))
+        assert rc == 0 and e.free_pages() == 1
+        for _ in range(2):  # slot 1 would copy the shared page, slot 2 needs another one: there is one
+            assert e.step_slots([1, 2], [20, 16], [a, c])[0] == eb.ST_CAPACITY
+            assert e.step_slots([2, 1], [16, 20], [c, a])[0] == eb.ST_CAPACITY
+            assert [e.slot_len(s) for s in range(3)] == [20, 20, 16] and e.free_pages() == 1
+        # the page is there for whoever steps alone
+        assert e.step_slots([2], [16], [c])[0] == 0 and e.free_pages() == 0
+        assert e.step_slots([0], [20], [a])[0] == eb.ST_CAPACITY
+        assert e.free_slot(2) == 0 and e.free_pages() == 2
+        # both holders of the shared page in one step: the first takes a copy, the second keeps it
+        rc, two = e.step_slots([0, 1], [20, 20], [a, a])
+        assert rc == 0 and e.free_pages() == 1 and two[0] == two[1]
+        for s in range(4):
+            assert e.free_slot(s) == 0
+        assert e.free_pages() == 4
+        rc, again = e.prefill_slot(3, np.arange(20))
+        assert rc == 0 and again == a
+    finally:
+        e.close()
+
+
+def test_slots_emptied_after_a_refused_step_give_every_page_back(kquant_path):
+    e = eb.Engine(kquant_path, 100)
+    try:
+        assert e.set_paged(3, 4, 16, "f16") == 0
+        rc, a = e.prefill_slot(0, np.arange(20))
+        assert rc == 0 and e.fork_slot(0, 1, 20) == 0
+        rc, c = e.prefill_slot(2, np.arange(16))
+        assert e.step_slots([1, 2], [20, 16], [a, c])[0] == eb.ST_CAPACITY
+        for s in range(3):
+            assert e.free_slot(s) == 0
+        assert e.free_pages() == 4
+        rc, b = e.prefill_slot(0, np.arange(60))
+        assert rc == 0 and e.free_pages() == 0
+    finally:
+        e.close()
