@@ -413,9 +413,10 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
             const int head = w.kvh * a.grp + r % a.grp;
             const int lim = row_ok ? w.sq.kv - w.sq.q + tok : -1;
             const int low = A.window > 0 ? max(0, max(lim, 0) - A.window + 1) : 0;
-            // ---- q: a warp's rows scaled by the power of two that brings their largest to [2^14, 2^15), then split. The low
-            // parts are exact to 2^-25 of that, 2^-39 of the largest row: in a score an absolute error of 2^-39 of the
-            // warp's largest, far below that of 32 bits. Rows come one (hd 128) or two (hd 64) to a load instruction.
+            // ---- q: every row scaled by the power of two that brings its largest element to [2^14, 2^15), then split. The low
+            // parts are exact to 2^-25 of that: an element is held to 2^-22 of itself or 2^-39 of its row's largest. (One scale for a
+            // warp's rows would let a large row take the bits of the small ones beside it.) Rows come one (hd 128) or two (hd 64)
+            // to a load instruction.
             float cs;
             {
                 constexpr int LPR = HD / 4, RPP = 32 / LPR;
@@ -427,24 +428,28 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
                         reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(mine), row + sub));
                     asm volatile("ld.global.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "l"(src + 4 * el));
                 };
-                float mx = 0.f;
-                float4 f[32 / RPP];  // all of the warp's rows in flight at once (the sums are not live yet)
+                // of a row whose largest finite element has these bits; elements that are not finite make a NaN of the row alone
+                auto scale_of = [](uint32_t mx) { return mx > 0 ? pow2f(min(max(14 - ((int)(mx >> 23) - 127), -100), 100)) : 1.f; };
+                uint32_t mx_mine = 0;  // of the row of this thread
+                float4 f[32 / RPP];    // all of the warp's rows in flight at once (the sums are not live yet)
 #pragma unroll
                 for (int i = 0; i < 32 / RPP; i++) load(i * RPP, f[i]);
 #pragma unroll
                 for (int i = 0; i < 32 / RPP; i++) {
-                    const float v = fmaxf(fmaxf(fabsf(f[i].x), fabsf(f[i].y)), fmaxf(fabsf(f[i].z), fabsf(f[i].w)));
-                    if (v < INFINITY) mx = fmaxf(mx, v);  // a row that is not finite does not disturb the others
-                }
-#pragma unroll
-                for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                const int ex = (int)((__float_as_uint(mx) >> 23) & 255) - 127;
-                float sc = mx > 0.f ? pow2f(min(max(14 - ex, -100), 100)) : 1.f;
-                cs = fmaxf(fabsf(A.scale) * 1.4426950408889634f / sc, 1e-37f);  // never zero: c times -infinity
-                if (A.scale <= 0.f) sc = A.scale < 0.f ? -sc : 0.f;             // the running maximum is that of +c S
-#pragma unroll
-                for (int i = 0; i < 32 / RPP; i++) {
                     const int ro = i * RPP + sub, row = 32 * (warp & 3) + ro;
+                    const float v = fmaxf(fmaxf(fabsf(f[i].x), fabsf(f[i].y)), fmaxf(fabsf(f[i].z), fabsf(f[i].w)));
+                    uint32_t mx = v < INFINITY ? __float_as_uint(v) : 0u;  // bits of values >= 0 have their order
+                    if constexpr (LPR == 32) {
+                        mx = __reduce_max_sync(0xffffffffu, mx);
+                        if (lane == i) mx_mine = mx;
+                    } else {
+#pragma unroll
+                        for (int o = LPR / 2; o; o >>= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                        const uint32_t other = __shfl_sync(0xffffffffu, mx, (lane % RPP) * LPR);
+                        if (lane / RPP == i) mx_mine = other;
+                    }
+                    float sc = scale_of(mx);
+                    if (A.scale <= 0.f) sc = A.scale < 0.f ? -sc : 0.f;  // the running maximum is that of +c S
                     if (!((rows_ok >> ro) & 1)) f[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                     const __half2 h0 = __floats2half2_rn(f[i].x * sc, f[i].y * sc), h1 = __floats2half2_rn(f[i].z * sc, f[i].w * sc);
                     const float2 b0 = __half22float2(h0), b1 = __half22float2(h1);
@@ -457,6 +462,7 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
                     *reinterpret_cast<uint2*>(q_lo + at) =
                         make_uint2(*reinterpret_cast<const uint32_t*>(&l0), *reinterpret_cast<const uint32_t*>(&l1));
                 }
+                cs = fmaxf(fabsf(A.scale) * 1.4426950408889634f / scale_of(mx_mine), 1e-37f);  // never zero: c times -infinity
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(&B.q_full[mt]);
             }

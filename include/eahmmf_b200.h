@@ -283,6 +283,7 @@ int eahmmf_cuda_rope_append(const EahmmfPagedKv* kv, int layer, const EahmmfPage
  * earlier rows of that sequence. n_head a multiple of n_kv, at most 64 q heads per kv head; row strides multiples of 4,
  * buffers 16-byte aligned, d_out not overlapping d_q. Over 32-bit pages the products of more than 16 rows (tokens x q heads of
  * a kv head) hold an element of k and v to 2^-22 of itself or 2^-39 of the largest among its 128 positions, whichever is more.
+ * An element of q is held to 2^-22 of itself or 2^-33 of the largest of its row (a token's head), whichever is more.
  * Elements of q, k and v stay below 2^100. The workspace (256-byte aligned) is written and read within the call: calls that may run at
  * the same time need one each. Asynchronous; results do not depend on what else runs. */
 size_t eahmmf_cuda_paged_attention_workspace_bytes(const EahmmfPagedKv* kv, const EahmmfPagedSeqs* seqs, int n_head);

@@ -109,3 +109,99 @@ def test_several_row_tiles_a_block_are_the_same_every_time(torch, type, hd, n_kv
             load @ load  # another state of the clocks and the caches
         assert torch.equal(c.attention(), first), i
     c.check(window=200, n_sink=3)
+
+
+LENS = [([40, 3, 17], [300, 50, 17]), ([130], [1000])]
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("hd,grp", [(128, 8), (64, 8), (128, 5)])
+@pytest.mark.parametrize("lens", LENS)
+def test_rows_of_very_different_size_do_not_disturb_each_other(torch, type, hd, grp, lens):
+    """A third of the tokens and one head have a q 2^45 as large: the others' outputs are as without them."""
+    c = Chunks(torch, type, hd, 2, grp, 16, *lens, seed=2)
+    large = torch.zeros(c.q.shape, dtype=torch.bool, device="cuda")
+    large[1::3] = True
+    large[:, 3 * hd:4 * hd] = True
+    for o in (dict(), dict(scale=-0.05, window=100, n_sink=2)):
+        want, tol = c.want(**o)
+        c.q[large] *= 2.0 ** 45
+        got = c.attention(**o).double()
+        c.q[large] *= 2.0 ** -45
+        far = ((got - want).abs() - tol)[~large]
+        assert bool((far <= 0).all()), (int((far > 0).sum()), float(far.max()))
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("q_scale", [0.0, 1e-30, 1e-6, 40.0, 1e5])
+@pytest.mark.parametrize("lens", LENS)
+def test_chunk_scores_of_every_size(torch, type, q_scale, lens):
+    g = torch.Generator("cuda")
+    g.manual_seed(4)
+    c = Chunks(torch, type, 128, 2, 8, 16, *lens, seed=4,
+               make=lambda what, shape: torch.randn(shape, generator=g, device="cuda") * (q_scale if what == "q" else 1.0))
+    for scale in (None, -0.3 if q_scale < 1e4 else -1e-6, 0.0, 1e-36):
+        c.check(scale=scale)
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("lens", LENS)
+def test_a_row_that_is_not_finite_is_alone(torch, type, lens):
+    c = Chunks(torch, type, 128, 2, 8, 16, *lens, seed=5)
+    want, tol = c.want()
+    rows = {1: float("nan"), 7: float("inf"), 30: float("-inf")}
+    for r, x in rows.items():
+        c.q[r, 5 * 128 + 17] = x  # head 5 of the row
+    got = c.attention().double()
+    for r in rows:
+        assert not bool(torch.isfinite(got[r, 5 * 128:6 * 128]).any())
+        got[r, 5 * 128:6 * 128] = want[r, 5 * 128:6 * 128]
+    assert bool(((got - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("lens", LENS + [([1, 1], [300, 40]), ([2], [500])])
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("x", [float("nan"), float("inf"), float("-inf")])
+def test_a_cached_element_that_is_not_finite_reaches_the_rows_that_see_it(torch, type, lens, what, x):
+    c = Chunks(torch, type, 128, 2, 8, 16, *lens, seed=6)
+    want, tol = c.want()
+    n, m = c.q_len[0], c.kv_len[0]
+    at = m - (n + 1) // 2  # a position in the middle of the first sequence's new ones
+    (c.k if what == "k" else c.v)[0, c.table[0, at // 16], 1, at % 16, 9] = x
+    got = c.attention().double()
+    first, half = n - (m - at), 8 * 128  # the rows from `first` on see it, in the heads of kv head 1
+    seen = got[first:n, half:]
+    if what == "v":
+        assert not bool(torch.isfinite(seen.view(-1, 8, 128)[..., 9]).any())
+    elif x != x:
+        assert not bool(torch.isfinite(seen).any())
+    ok = (got - want).abs() <= tol
+    ok[first:n, half:] = True
+    if what == "v":
+        ok[:first, half:] = True  # an earlier row of the sequence: a weight of zero does not hide it
+    assert bool(ok.all())
+
+
+@pytest.mark.parametrize("lens", LENS)
+@pytest.mark.parametrize("hd", [64, 128])
+def test_wide_ranges_over_32_bit_pages(torch, hd, lens):
+    """k and v of 2^-30 to 2^10 beside each other: an element is held to 2^-22 of itself or 2^-39 of the largest of its unit, so a
+    score is off by 2^-39 max|k| sum|q| and an output by 2^-39 max|v| more."""
+    g = torch.Generator("cuda")
+    g.manual_seed(7)
+
+    def make(what, shape):
+        x = torch.randn(shape, generator=g, device="cuda")
+        return x * 2.0 ** -8 if what == "q" else x * 2.0 ** torch.randint(-30, 11, shape, generator=g, device="cuda").float()
+    c = Chunks(torch, "f32", hd, 2, 8, 16, *lens, seed=7, make=make)
+    got = c.attention().double()
+    want, tol = c.want()
+    row = 0
+    for (k, v), n, m in zip(c.hist, c.q_len, c.kv_len):
+        s = slice(row, row + n)
+        extra = c.q[s].double().abs().view(n, -1, hd).sum(-1) * hd ** -0.5 * float(k.abs().max()) * 2.0 ** -39
+        tol[s] += (2 * extra[..., None] * float(v.abs().max()) + float(v.abs().max()) * 2.0 ** -39).expand(n, -1, hd).reshape(n, -1)
+        row += n
+    assert bool(((got - want).abs() <= tol).all())
+    assert int(c.status.item()) == 0
