@@ -538,8 +538,27 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
                 const float mn = mx == -INFINITY ? m : fmaxf(m, mx * csu);
                 alpha = mn == -INFINITY ? 1.f : ex2(m - mn);
                 m = mn;
-                const float mo = mn == -INFINITY ? 0.f : mn - 15.f;
-                const uint64_t cs2 = f2(csu, csu), mo2 = f2(-mo, -mo);
+                // c S - (m - 15) in one rounding, of which c S loses none: where m itself is rounded by more than a little (from
+                // 2^22 an eighth), the largest weight would miss 2^15 and overflow. Such scores are rounded first, as m was.
+                float c1 = csu, mo = mn == -INFINITY ? 0.f : mn - 15.f;
+                const bool far = mn != -INFINITY && fabsf(mn) >= 4194304.f;
+                if (__any_sync(0xffffffffu, far)) {
+#pragma unroll 1
+                    for (int c = 0; c < UNIT; c += 32) {
+                        uint32_t s[32];
+                        tm_ld32(s_tm + c, s);
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if (far) s[j] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(s[j]), csu), mn));
+                        tm_st32(s_tm + c, s);
+                    }
+                    tm_wait_st();
+                    if (far) {
+                        c1 = 1.f;
+                        mo = -15.f;
+                    }
+                }
+                const uint64_t cs2 = f2(c1, c1), mo2 = f2(-mo, -mo);
                 uint64_t ls2 = 0;
 #pragma unroll 1
                 for (int c = 0; c < UNIT; c += 32) {

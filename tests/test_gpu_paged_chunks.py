@@ -205,3 +205,30 @@ def test_wide_ranges_over_32_bit_pages(torch, hd, lens):
         row += n
     assert bool(((got - want).abs() <= tol).all())
     assert int(c.status.item()) == 0
+
+
+def far_scores(torch, type, hd, grp, lens, e):
+    """Small whole numbers in q and k, q times 2^e: the scores are exact, and a row's largest ones outweigh the rest by 2^256 at
+    least, so that it has the mean of their v. The weights of the largest are equal; their sum and the products with v round n
+    times in 32 bits and once to 22."""
+    g = torch.Generator("cuda")
+    g.manual_seed(8)
+
+    def make(what, shape):
+        x = torch.randint(-3, 4, shape, generator=g, device="cuda").float()
+        return torch.randn(shape, generator=g, device="cuda") if what == "v" else x * 2.0 ** e if what == "q" else x
+    c = Chunks(torch, type, hd, 2, grp, 16, *lens, seed=8, make=make)
+    for scale in (1.0, -1.0):
+        want, _ = c.want(scale=scale)
+        got = c.attention(scale=scale).double()
+        assert bool(torch.isfinite(got).all())
+        vmax = max(float(v.abs().max()) for _, v in c.hist)
+        assert float((got - want).abs().max()) <= vmax * (2.0 ** -21 + max(c.kv_len) * U)
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("hd,grp", [(128, 8), (64, 6)])
+@pytest.mark.parametrize("lens", LENS + [([24], [24])])
+@pytest.mark.parametrize("e", [8, 14, 15, 16, 17, 18, 20, 23, 26, 40, 80])
+def test_chunk_scores_past_24_bits(torch, type, hd, grp, lens, e):
+    far_scores(torch, type, hd, grp, lens, e)
