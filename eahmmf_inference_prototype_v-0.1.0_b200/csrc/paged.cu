@@ -703,7 +703,7 @@ __global__ void __launch_bounds__(PA_NT, STEP_BLOCKS) k_paged_attn(PagedAttnArgs
             uint32_t ph[4], pl[4];
 #pragma unroll
             for (int i = 0; i < NR; i++) {
-                const float mo = m[i] == -INFINITY ? 0.f : m[i] - P_SHIFT;
+                const float mo = m[i] == -INFINITY ? 0.f : __fadd_ru(m[i], -P_SHIFT);  // up: no weight passes 2^15, which halves hold
 #pragma unroll
                 for (int j = 0; j < PT; j++) {
                     sv[i][j] = ex2(sv[i][j] - mo);

@@ -232,3 +232,11 @@ def far_scores(torch, type, hd, grp, lens, e):
 @pytest.mark.parametrize("e", [8, 14, 15, 16, 17, 18, 20, 23, 26, 40, 80])
 def test_chunk_scores_past_24_bits(torch, type, hd, grp, lens, e):
     far_scores(torch, type, hd, grp, lens, e)
+
+
+@pytest.mark.parametrize("type", ["f16", "f32"])
+@pytest.mark.parametrize("hd,grp", [(128, 8), (64, 5), (128, 16)])  # tiles of 8 and of 16 rows
+@pytest.mark.parametrize("lens", [([1, 1], [300, 40]), ([1], [3000]), ([1] * 40, [41] * 40)])
+@pytest.mark.parametrize("e", [8, 14, 15, 16, 17, 18, 20, 23, 26, 40, 80])
+def test_step_scores_past_24_bits(torch, type, hd, grp, lens, e):
+    far_scores(torch, type, hd, grp, lens, e)
