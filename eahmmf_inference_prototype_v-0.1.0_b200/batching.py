@@ -44,8 +44,9 @@ class ContinuousBatcher:
         self.rows = 0  # sequence-tokens decoded by steps (throughput accounting)
 
     def _need(self, r: Request) -> int:
-        """Pages of a request's positions: its prompt and every token but the last, which is not fed."""
-        return -(-(len(r.prompt) + r.n_gen - 1) // self.page)
+        """Pages of a request's positions: its prompt, which is always prefilled, and every token but the last, which is
+        not fed."""
+        return -(-(len(r.prompt) + max(r.n_gen, 1) - 1) // self.page)
 
     def submit(self, prompt, n_gen: int) -> Request:
         r = Request(list(map(int, prompt)), int(n_gen))
