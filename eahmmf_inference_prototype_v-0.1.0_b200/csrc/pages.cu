@@ -166,7 +166,7 @@ extern "C" int eahmmf_rope_inv_freq(int scaling, int n_rot, double base, double 
     if (scaling == EAHMMF_ROPE_YARN) {
         lo = std::max(0.0, floor(pair_of(beta_fast)));
         hi = std::min(n_rot - 1.0, ceil(pair_of(beta_slow)));
-        if (hi <= lo) hi = lo + 0.001;
+        if (hi <= lo) lo = hi - 0.001;  // every pair past hi (a short ctx_orig), or none of them up to lo
     }
     for (int i = 0; i < n_rot / 2; i++) {
         double f = pow(base, -2.0 * i / n_rot);
