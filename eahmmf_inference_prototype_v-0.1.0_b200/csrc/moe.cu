@@ -336,10 +336,17 @@ __device__ void route_token(const float* __restrict__ lg, int E, int K, int lane
 #pragma unroll
     for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     uint32_t key[PER];
+    bool isnan_e = false;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         d[i] = d[i] - mx;  // the CPU's fp32 difference
+        isnan_e |= (lane + 32 * i) < E && d[i] != d[i];
         key[i] = (lane + 32 * i) < E ? fkey(d[i]) : 0u;
+    }
+    if (__any_sync(0xffffffffu, isnan_e)) {  // a NaN has no rank: no expert
+        out_e = -1;
+        out_w = __int_as_float(0x7fffffff);
+        return;
     }
     // (d desc, index asc) top k; lane j keeps the j-th (d, e)
     float cd = 0.f, dk = 0.f;
@@ -552,7 +559,7 @@ __device__ void route_one(const MoeArgs& a, RouteSm r, bool global) {
             if (lane < K) {
                 if (my_e < 0 || my_e >= E) {  // only reachable with NaN logits
                     if (global) set_flag(a.status, ST_BAD_INDEX);
-                    my_e = 0;
+                    my_e = lane;  // see route_block
                 }
                 r.s_ids[lane] = my_e;
                 r.s_w[lane] = my_w;
@@ -621,6 +628,8 @@ __device__ void route_one(const MoeArgs& a, RouteSm r, bool global) {
 }
 
 // GIVEN: the experts of every slot come from a.given (weight 1, entries < 0 absent) instead of a top-k.
+// A token whose logits hold a NaN (or two infinities) has no top k: it is flagged and takes experts 0 .. k - 1, each once as every
+// token's experts are. Slots, groups and the slot map count on that: an expert twice would leave entries of theirs unwritten.
 template <bool TEAMS, int GS = MU, bool GIVEN = false>
 __device__ void route_block(const MoeArgs& a, RouteSm r, bool global) {
     static_assert(GS >= MU && GS <= 32, "group size");
@@ -662,7 +671,7 @@ __device__ void route_block(const MoeArgs& a, RouteSm r, bool global) {
             } else if (lane < K) {
                 if (my_e < 0 || my_e >= E) {  // NaN logits or a given id out of range
                     if (global) set_flag(a.status, ST_BAD_INDEX);
-                    my_e = 0;
+                    my_e = GIVEN ? 0 : lane;
                 }
                 r.s_ids[t * K + lane] = my_e;
                 r.s_w[t * K + lane] = my_w;
@@ -711,7 +720,7 @@ __device__ void route_block(const MoeArgs& a, RouteSm r, bool global) {
                     const float my_w = __fdiv_rn(rk, tot);
                     if (my_e < 0 || my_e >= E) {  // only reachable with NaN logits
                         if (global) set_flag(a.status, ST_BAD_INDEX);
-                        my_e = 0;
+                        my_e = lane;
                     }
                     r.s_ids[t * K + lane] = my_e;
                     r.s_w[t * K + lane] = my_w;
@@ -825,7 +834,7 @@ __device__ void route_block(const MoeArgs& a, RouteSm r, bool global) {
                     const float my_w = __fdiv_rn(sel_r[tt], tot);
                     if (my_e < 0 || my_e >= E) {  // only reachable with NaN logits
                         if (global) set_flag(a.status, ST_BAD_INDEX);
-                        my_e = 0;
+                        my_e = tt;
                     }
                     r.s_ids[t * K + tt] = my_e;
                     r.s_w[t * K + tt] = my_w;
@@ -1652,7 +1661,7 @@ __global__ void __launch_bounds__(BIG_NT) k_route_big(MoeArgs a, int* __restrict
             } else {
                 if (my_e < 0 || my_e >= E) {  // NaN logits or a given id out of range
                     set_flag(a.status, ST_BAD_INDEX);
-                    my_e = 0;
+                    my_e = GIVEN ? 0 : lane;
                 }
                 a.rw.ids[(size_t)t * K + lane] = my_e;
                 a.rw.wts[(size_t)t * K + lane] = my_w;
