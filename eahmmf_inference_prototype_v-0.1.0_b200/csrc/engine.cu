@@ -1267,6 +1267,11 @@ struct EahmmfEngine {
         if (rc == ST_OK && launch_prep_x(att, QD, nb, QD, xf_o, st) != cudaSuccess) rc = ST_CUDA;
         return rc;
     }
+    // A slot back at the length it had before a call that failed. What was appended since lies behind its positions.
+    void paged_back(int slot, int len) {
+        paged->len[slot] = len;
+        eahmmf_pages_truncate(paged->pages, slot, len);
+    }
     // n tokens behind those of `slot`, in passes of n_batch; the last token's logits in `logits`. A failure takes the slot back
     // to its length of before.
     int paged_extend(int slot, const int* htoks, int n, int n_batch) {
@@ -1289,8 +1294,7 @@ struct EahmmfEngine {
             pass.n_seq = 0;
         }
         if (rc != ST_OK) {
-            P.len[slot] = p0;
-            eahmmf_pages_truncate(P.pages, slot, p0);
+            paged_back(slot, p0);
             paged_copies();  // none may stay recorded: pages given back would wait for the next pass
         }
         return rc;
@@ -1592,14 +1596,19 @@ bool tokens_ok(const EahmmfEngine* e, const int* toks, int n) {
 int extend_slot(EahmmfEngine* e, int slot, const int* toks, int n, int n_batch, int* next) {
     if (!tokens_ok(e, toks, n)) return ST_BAD_ARG;
     if ((long long)e->paged->len[slot] + n > e->n_ctx) return ST_BAD_ARG;
+    const int p0 = e->paged->len[slot];
     int rc = e->paged_extend(slot, toks, n, n_batch);
     if (rc != ST_OK) return rc;
     if (launch_argmax_rows(e->logits, e->n_vocab, e->n_vocab, 1, e->d_btok, e->st) != cudaSuccess ||
         cudaMemcpyAsync(e->h_b, e->d_btok, 4, cudaMemcpyDeviceToHost, e->st) != cudaSuccess)
-        return ST_CUDA;
-    rc = e->read_status();
+        rc = ST_CUDA;
+    if (rc == ST_OK) rc = e->read_status();
+    if (rc != ST_OK) {
+        e->paged_back(slot, p0);
+        return rc;
+    }
     *next = e->h_b[0];
-    return rc;
+    return ST_OK;
 }
 }  // namespace
 
@@ -1679,23 +1688,18 @@ extern "C" int eahmmf_engine_step_slots(EahmmfEngine* e, int n, const int* slots
             ones[i] = 1;
         }
         rc = e->paged_begin(slots, ones, n);
-        if (rc != ST_OK) {  // no row is taken: the slots keep their lengths
-            for (int i = 0; i < n; i++) {
-                P.len[slots[i]] = pos[i];
-                eahmmf_pages_truncate(P.pages, slots[i], pos[i]);
-            }
-            e->paged_copies();
-            return rc;
-        }
+        if (rc != ST_OK) e->paged_copies();
     }
-    rc = e->forward(e->d_btok, n, true, true);
+    if (rc == ST_OK) rc = e->forward(e->d_btok, n, true, true);
     e->pass.n_seq = 0;
-    if (rc != ST_OK) return rc;
-    if (launch_argmax_rows(e->logits_b, e->n_vocab, e->n_vocab, n, e->d_btok, e->st) != cudaSuccess ||
-        cudaMemcpyAsync(h, e->d_btok, (size_t)n * 4, cudaMemcpyDeviceToHost, e->st) != cudaSuccess)
-        return ST_CUDA;
-    rc = e->read_status();
-    memcpy(next, h, (size_t)n * 4);
+    if (rc == ST_OK && (launch_argmax_rows(e->logits_b, e->n_vocab, e->n_vocab, n, e->d_btok, e->st) != cudaSuccess ||
+                        cudaMemcpyAsync(h, e->d_btok, (size_t)n * 4, cudaMemcpyDeviceToHost, e->st) != cudaSuccess))
+        rc = ST_CUDA;
+    const bool ran = rc == ST_OK;
+    if (ran) rc = e->read_status();
+    if (rc != ST_OK && e->paged)  // no row is taken: the slots keep their lengths
+        for (int i = 0; i < n; i++) e->paged_back(slots[i], pos[i]);
+    if (ran) memcpy(next, h, (size_t)n * 4);
     return rc;
 }
 

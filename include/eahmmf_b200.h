@@ -426,9 +426,10 @@ int eahmmf_engine_step_slots(EahmmfEngine* e, int n, const int* slots, const int
  * they grow, up to n_ctx positions each; the single-sequence calls keep the contiguous cache. EAHMMF_ST_CAPACITY: not enough
  * memory, nothing changed. eahmmf_engine_set_slots goes back to contiguous slots.
  *  - prefill_slot then frees the slot's pages first; step_slots wants each row at its slot's length, and returns
- *    EAHMMF_ST_CAPACITY without taking any row when there are not enough pages;
+ *    EAHMMF_ST_CAPACITY without taking any row when there are not enough pages; a step that fails in another way
+ *    takes none either;
  *  - extend_slot: n tokens behind those of the slot (a further turn, or the rest of a prompt behind a shared start), the first
- *    maximum of the last one's logits into *next; EAHMMF_ST_CAPACITY leaves the slot as it was;
+ *    maximum of the last one's logits into *next; EAHMMF_ST_CAPACITY, or another failure, leaves the slot as it was;
  *  - fork_slot: the empty slot dst takes the first len positions of src and shares their pages; the one that grows into a
  *    shared part-filled page gets a copy of it in its next step;
  *  - free_slot: the slot's pages are given back; slot_len: its positions (-1: no such paged slot); free_pages: pages that

@@ -62,3 +62,49 @@ def test_slots_emptied_after_a_refused_step_give_every_page_back(kquant_path):
         assert rc == 0 and e.free_pages() == 0
     finally:
         e.close()
+
+
+BAD_TOKEN = 777
+
+
+@pytest.fixture(scope="module")
+def nan_path(tmp_path_factory):
+    """The same model with NaN in one token's embedding: its routing is no expert's, which raises EAHMMF_ST_BAD_INDEX."""
+    cfg = synth.config_kquant_small()
+    path = synth.write_gguf(str(tmp_path_factory.mktemp("kn") / "kn.gguf"), cfg)
+    header, specs, offsets, _ = synth._layout(cfg)
+    assert specs[0].name == "token_embd.weight" and cfg.embd_type == synth.Q4_K
+    row = synth.row_bytes(cfg.embd_type, cfg.D)
+    with open(path, "r+b") as f:
+        for block in range(cfg.D // 256):
+            f.seek(len(header) + offsets[0] + BAD_TOKEN * row + 144 * block)
+            f.write(np.float16("nan").tobytes())  # the scale of a block
+    return path
+
+
+@pytest.mark.parametrize("n_batch", [2, 64])
+def test_a_failed_call_takes_no_position(nan_path, n_batch):
+    e = eb.Engine(nan_path, 100)
+    try:
+        assert e.set_paged(4, 12, 16, "f16") == 0
+        rc, a = e.prefill_slot(0, np.arange(20))
+        assert rc == 0 and e.fork_slot(0, 1, 20) == 0
+        rc, b = e.prefill_slot(2, np.arange(7))
+        assert rc == 0 and e.free_pages() == 9
+        assert e.extend_slot(0, [5, 6, BAD_TOKEN, 7], n_batch)[0] == eb.ST_BAD_INDEX
+        assert e.slot_len(0) == 20
+        assert e.step_slots([2, 1], [7, 20], [b, BAD_TOKEN])[0] == eb.ST_BAD_INDEX
+        assert [e.slot_len(s) for s in range(3)] == [20, 20, 7]
+        assert e.prefill_slot(3, [1, BAD_TOKEN], n_batch)[0] == eb.ST_BAD_INDEX and e.slot_len(3) == 0
+        # each goes on as if nothing had been: the NaN lie behind its positions
+        rc, nxt = e.step_slots([0, 1, 2], [20, 20, 7], [a, a, b])
+        assert rc == 0 and nxt[0] == nxt[1]
+        rc, same = e.prefill_slot(3, np.arange(7))
+        assert rc == 0 and same == b
+        rc, step = e.step_slots([3], [7], [b])
+        assert rc == 0 and step[0] == nxt[2]
+        for s in range(4):
+            assert e.free_slot(s) == 0
+        assert e.free_pages() == 12
+    finally:
+        e.close()
