@@ -1180,7 +1180,8 @@ struct EahmmfEngine {
         p.reset();
     }
     void drop_paged() { release(paged); }
-    // A new paged cache in the place of the present one, which stays where there is not enough memory.
+    // A new paged cache in the place of the present one and of the contiguous slots but one, which the single-sequence calls keep.
+    // All of them stay where there is not enough memory.
     int set_paged(int n_slots_, int n_pages, int page, int type) {
         if (cudaStreamSynchronize(st) != cudaSuccess) return ST_CUDA;
         std::unique_ptr<Paged> made;
@@ -1216,6 +1217,7 @@ struct EahmmfEngine {
         } catch (const std::bad_alloc&) {
             ok = false;
         }
+        if (ok && n_slots > 1) ok = set_slots(1);  // which frees nothing before it has its own
         if (!ok) {
             cudaGetLastError();
             release(made);
@@ -1579,10 +1581,7 @@ extern "C" int eahmmf_engine_set_slots(EahmmfEngine* e, int n_slots) {
 extern "C" int eahmmf_engine_set_paged(EahmmfEngine* e, int n_slots, int n_pages, int page, int type) {
     if (!e || n_slots < 1 || n_slots > 4096 || n_pages < 1 || page < 16 || page > 1024 || page % 16) return ST_BAD_ARG;
     if (type != T_F32 && type != T_F16) return ST_BAD_TYPE;
-    const int rc = e->set_paged(n_slots, n_pages, page, type);
-    if (rc != ST_OK) return rc;
-    if (e->n_slots > 1 && !e->set_slots(1)) return ST_CUDA;  // the contiguous cache keeps the single-sequence calls' slot
-    return ST_OK;
+    return e->set_paged(n_slots, n_pages, page, type);
 }
 
 namespace {

@@ -2,6 +2,8 @@
 back can be taken again."""
 import os
 
+import dataclasses
+
 import numpy as np
 import pytest
 
@@ -107,4 +109,34 @@ def test_a_failed_call_takes_no_position(nan_path, n_batch):
             assert e.free_slot(s) == 0
         assert e.free_pages() == 12
     finally:
+        e.close()
+
+
+def test_a_paged_cache_without_room_leaves_the_slots(tmp_path_factory):
+    """Memory for the pages, but not for the one contiguous slot that takes the place of two: nothing changes."""
+    import torch
+    if not torch.cuda.is_available():
+        pytest.fail("CUDA device required")
+    cfg = dataclasses.replace(synth.config_kquant_small(), ctx_train=1 << 16)
+    path = synth.write_gguf(str(tmp_path_factory.mktemp("kc") / "kc.gguf"), cfg)
+    e = eb.Engine(path, 1 << 16)  # a slot: 100 MB of k and as much of v
+    hog = None
+    try:
+        assert e.set_slots(2) == 0
+        nxt = [e.prefill_slot(s, np.arange(10 + s)) for s in range(2)]
+        assert [rc for rc, _ in nxt] == [0, 0]
+        rc, want = e.step_slots([0, 1], [10, 11], [t for _, t in nxt])
+        assert rc == 0
+        torch.cuda.empty_cache()
+        hog = torch.empty(torch.cuda.mem_get_info()[0] - (150 << 20), dtype=torch.uint8, device="cuda")
+        assert e.set_paged(2, 64, 16, "f16") == eb.ST_CAPACITY
+        hog = None
+        torch.cuda.empty_cache()
+        assert e.free_pages() == -1 and e.slot_len(0) == -1
+        rc, again = e.step_slots([0, 1], [10, 11], [t for _, t in nxt])
+        assert rc == 0 and list(again) == list(want)
+        assert e.set_paged(2, 64, 16, "f16") == 0 and e.free_pages() == 64
+    finally:
+        hog = None
+        torch.cuda.empty_cache()
         e.close()
