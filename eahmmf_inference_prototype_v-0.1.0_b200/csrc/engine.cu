@@ -270,13 +270,13 @@ struct EahmmfEngine {
     };
     std::vector<Slice> slices;
     std::string path;
-    // Oversubscribed mode (expert_budget > 0): the experts stay in the mapped file (pinned for DMA) and a
+    // Oversubscribed mode (expert_budget > 0): the experts stay in host memory (a pinned copy of the file) and a
     // device cache of `slots` expert footprints holds the resident ones (see ExpertCache).
     struct ExpertCache {
         std::unique_ptr<Gguf> file;     // the mapping the host copies come from
-        bool pinned = false;            // fills are DMA copies: from the registered mapping or a pinned copy
+        bool pinned = false;            // fills are DMA copies from the pinned copy
         const uint8_t* host = nullptr;  // the bytes fills copy from (file offsets)
-        uint8_t* host_copy = nullptr;   // pinned copy of the file when the mapping cannot be registered
+        uint8_t* host_copy = nullptr;   // pinned copy of the file
         size_t comp[3] = {0, 0, 0};     // bytes of one expert's gate, up, down
         size_t off[3] = {0, 0, 0};      // their offsets inside a slot
         size_t foot = 0;                // slot bytes
@@ -386,7 +386,6 @@ struct EahmmfEngine {
             if (C.h_tab) cudaFreeHost(C.h_tab);
             if (C.h_ids) cudaFreeHost(C.h_ids);
             if (C.host_copy) cudaFreeHost(C.host_copy);
-            else if (C.pinned && C.file) cudaHostUnregister(const_cast<uint8_t*>(C.file->map));
             cache.reset();  // unmaps the file
         }
         drop_paged();
@@ -637,10 +636,20 @@ struct EahmmfEngine {
     }
 
     // ---- oversubscribed mode ------------------------------------------------------------------------
+    // Whether the host has n bytes to give away: pinned pages cannot be taken back from a machine that runs short.
+    static bool host_room(size_t n) {
+        unsigned long long kb = 0;
+        bool known = false;
+        if (FILE* f = fopen("/proc/meminfo", "r")) {
+            char line[256];
+            while (!known && fgets(line, sizeof line, f)) known = sscanf(line, "MemAvailable: %llu", &kb) == 1;
+            fclose(f);
+        }
+        return !known || kb * 1024 > n + n / 16 + (1ull << 30);
+    }
     // The cache: slots of one expert footprint each (gate, up, down at 256-byte aligned offsets), at
-    // least one layer's worth; the file mapping registered with the driver so that fills are DMA copies
-    // from it (pageable copies otherwise); every layer's pointer table aimed at slot 0 until its experts
-    // are made resident.
+    // least one layer's worth; a pinned copy of the file so that fills are DMA copies (pageable copies from the
+    // mapping otherwise); every layer's pointer table aimed at slot 0 until its experts are made resident.
     bool init_cache(std::unique_ptr<Gguf> file, size_t budget) {
         ExpertCache& C = *cache;
         C.file = std::move(file);
@@ -652,29 +661,25 @@ struct EahmmfEngine {
         C.slots = (int)std::min<size_t>(budget / C.foot, (size_t)n_layer * n_expert);
         if (C.slots < n_expert) return fail("expert budget below one layer's experts");
         if (!dalloc(C.dev, (size_t)C.slots * C.foot)) return fail("cannot allocate the expert cache");
-        // DMA source: the mapping registered read-only, else a pinned copy of the file, else the pageable
-        // mapping (the driver then stages every fill)
+        // DMA source: a pinned copy of the file, else the pageable mapping (the driver then stages every fill). The mapping itself
+        // is not registered: some machines refuse that for a file, on others it took minutes without an end (4 MB of a
+        // file's pages: more than 100 s; the copy of a 19 GB file: 9 to 13 s).
         C.host = C.file->map;
-        if (cudaHostRegister(const_cast<uint8_t*>(C.file->map), C.file->size, cudaHostRegisterReadOnly) == cudaSuccess) {
+        if (host_room(C.file->size) && cudaHostAlloc((void**)&C.host_copy, C.file->size, cudaHostAllocDefault) == cudaSuccess) {
+            const unsigned nt = std::max(1u, std::min(32u, std::thread::hardware_concurrency()));
+            std::vector<std::thread> pool;
+            const size_t per = (C.file->size + nt - 1) / nt;
+            for (unsigned t = 0; t < nt; t++)
+                pool.emplace_back([&, t]() {
+                    const size_t b = std::min(C.file->size, (size_t)t * per), n = std::min(C.file->size - b, per);
+                    memcpy(C.host_copy + b, C.file->map + b, n);
+                });
+            for (auto& th : pool) th.join();
+            C.host = C.host_copy;
             C.pinned = true;
         } else {
             cudaGetLastError();
-            if (cudaHostAlloc((void**)&C.host_copy, C.file->size, cudaHostAllocDefault) == cudaSuccess) {
-                const unsigned nt = std::max(1u, std::min(32u, std::thread::hardware_concurrency()));
-                std::vector<std::thread> pool;
-                const size_t per = (C.file->size + nt - 1) / nt;
-                for (unsigned t = 0; t < nt; t++)
-                    pool.emplace_back([&, t]() {
-                        const size_t b = std::min(C.file->size, (size_t)t * per), n = std::min(C.file->size - b, per);
-                        memcpy(C.host_copy + b, C.file->map + b, n);
-                    });
-                for (auto& th : pool) th.join();
-                C.host = C.host_copy;
-                C.pinned = true;
-            } else {
-                cudaGetLastError();
-                C.host_copy = nullptr;
-            }
+            C.host_copy = nullptr;
         }
         const size_t nk = (size_t)n_layer * n_expert;
         for (int c = 0; c < 3; c++)

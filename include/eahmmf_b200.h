@@ -364,8 +364,8 @@ EahmmfEngine* eahmmf_engine_load(const char* gguf_path, int n_ctx, char* err, si
 void eahmmf_engine_free(EahmmfEngine* e);
 /* Expert residency beyond HBM (the reference's reason to exist: eahmmf.h's RAM/VRAM tiers, with the
  * asynchronous prefetch its README lists as not implemented): the model loads with only the non-expert
- * tensors in HBM; expert bytes stay in the mapped GGUF (registered with the driver for DMA) and a device
- * cache of expert_vram_bytes holds whole experts (at least one layer's worth). Each MoE pass reads back
+ * tensors in HBM; expert bytes stay in host memory (a pinned copy of the GGUF, where the host has room for one beside its
+ * page cache, else the mapped file) and a device cache of expert_vram_bytes holds whole experts (at least one layer's worth). Each MoE pass reads back
  * its routing, makes every routed expert resident (a hit waits for a fill in flight; a miss evicts the
  * least recently used expert the pass does not need), uploads the layer's pointer table and starts, on a
  * second stream, the fills of the experts the next layer routed at its last pass, which overlap this
@@ -374,8 +374,8 @@ void eahmmf_engine_free(EahmmfEngine* e);
 EahmmfEngine* eahmmf_engine_load_budget(const char* gguf_path, int n_ctx, size_t expert_vram_bytes, char* err,
                                         size_t err_cap);
 /* Cache counters: [0] slots (experts), [1] hits, [2] misses, [3] prefetch fills, [4] hits on prefetched
- * experts, [5] evictions, [6] bytes copied host -> device, [7] 1 when fills are DMA from the registered
- * mapping. All zero for a fully resident engine. */
+ * experts, [5] evictions, [6] bytes copied host -> device, [7] 1 when fills are DMA from the pinned
+ * copy. All zero for a fully resident engine. */
 #define EAHMMF_CACHE_STATS 8
 int eahmmf_engine_cache_stats(EahmmfEngine* e, uint64_t* v, int cap);
 /* dims[0..10] = n_layer, D, n_head, n_kv, hd, n_expert, n_used, FF, n_vocab, n_ctx, embedding rows */
