@@ -393,10 +393,14 @@ class Engine:
 
     def set_paged(self, n_slots: int, n_pages: int, page: int = 64, dtype: str = "f16") -> int:
         """eahmmf_engine_set_paged: the slots share a cache of n_pages pages ("f16" or "f32")."""
+        if not _fit(n_slots, n_pages, page):
+            return ST_BAD_ARG
         return lib().eahmmf_engine_set_paged(self._h, n_slots, n_pages, page, {"f32": 0, "f16": 1}[dtype])
 
     def extend_slot(self, slot: int, toks, n_batch: int = 64):
         """Tokens behind those of a paged slot: (rc, next token)."""
+        if not _fit(slot, n_batch):
+            return ST_BAD_ARG, 0
         t = np.ascontiguousarray(toks, np.int32)
         nxt = C.c_int(0)
         rc = lib().eahmmf_engine_extend_slot(self._h, slot, t.ctypes.data, len(t), n_batch, C.byref(nxt))
@@ -404,13 +408,15 @@ class Engine:
 
     def fork_slot(self, src: int, dst: int, length: int) -> int:
         """eahmmf_engine_fork_slot: dst shares the first `length` positions of src."""
+        if not _fit(src, dst, length):
+            return ST_BAD_ARG
         return lib().eahmmf_engine_fork_slot(self._h, src, dst, length)
 
     def free_slot(self, slot: int) -> int:
-        return lib().eahmmf_engine_free_slot(self._h, slot)
+        return lib().eahmmf_engine_free_slot(self._h, slot) if _fit(slot) else ST_BAD_ARG
 
     def slot_len(self, slot: int) -> int:
-        return lib().eahmmf_engine_slot_len(self._h, slot)
+        return lib().eahmmf_engine_slot_len(self._h, slot) if _fit(slot) else -1
 
     def free_pages(self) -> int:
         return lib().eahmmf_engine_free_pages(self._h)
@@ -576,6 +582,17 @@ def _dev_tensor(t, name: str, dtype: str, device=None):
         raise ValueError(f"{name}: a contiguous {dtype} tensor on {device or 'a CUDA device'} is needed")
 
 
+def _fit(*values) -> bool:
+    """Whether numbers are what a C int holds: ctypes would take others modulo 2^32."""
+    return all(-(1 << 31) <= x < 1 << 31 for x in values)
+
+
+def _ints(**values) -> None:
+    for name, x in values.items():
+        if not _fit(x):
+            raise ValueError(f"{name}: {x} does not fit in 32 bits")
+
+
 class PagedBatch:
     """The sequences of one call (EahmmfPagedSeqs): int32 device tensors table [n_seq x ld], cu_q [n_seq + 1] and
     kv_len [n_seq]; rows of activations and the bounds max_q, max_kv of their lengths (they choose kernels, results do
@@ -587,6 +604,7 @@ class PagedBatch:
         n_seq = kv_len.numel()
         if cu_q.numel() != n_seq + 1 or table.dim() != 2 or table.shape[0] != n_seq or (n_seq and table.shape[1] < 1):
             raise ValueError("table [n_seq x ld], cu_q [n_seq + 1] and kv_len [n_seq] are needed")
+        _ints(n_tok=n_tok, max_q=max_q, max_kv=max_kv)
         self._keep = (table, cu_q, kv_len)
         self.n_tok, self.device = n_tok, kv_len.device
         self.desc = EahmmfPagedSeqs(n_seq, n_tok, max_q, max_kv, cu_q.data_ptr(), kv_len.data_ptr(), table.data_ptr(),
@@ -655,6 +673,8 @@ class PagedCache:
         st = self._go(batch, stream)
         if rope.index != self._idx:
             raise ValueError(f"the frequency table lives on cuda:{rope.index}, the cache on {self.device}")
+        if (layer | n_head) >> 31:
+            _ints(layer=layer, n_head=n_head)
         x, ld = self._rows(qkv, "qkv", batch, (n_head + 2 * self.n_kv) * self.hd)
         q, ldq = self._rows(q_out, "q_out", batch, n_head * self.hd)
         rc = self._append(self._ref, layer, batch._ref, rope._ref, n_head, x, ld, self._norm(q_norm, "q_norm"),
@@ -671,6 +691,8 @@ class PagedCache:
                   n_sink: int = 0, ws=None, stream=None, d_status=None) -> None:
         """eahmmf_cuda_paged_attention: out [n_tok x n_head hd] from the rows q (scale: 1 / sqrt(hd))."""
         st = self._go(batch, stream)
+        if (layer | n_head | window | n_sink) >> 31:
+            _ints(layer=layer, n_head=n_head, window=window, n_sink=n_sink)
         x, ldq = self._rows(q, "q", batch, n_head * self.hd)
         y, ldo = self._rows(out, "out", batch, n_head * self.hd)
         if ws is None:
@@ -705,7 +727,8 @@ class Pages:
 
     def __init__(self, n_pages: int, page: int, n_seq: int, max_pages: int):
         self._lib = lib()
-        self._free = self._lib.eahmmf_pages_destroy
+        self._free, self._h = self._lib.eahmmf_pages_destroy, None
+        _ints(n_pages=n_pages, page=page, n_seq=n_seq, max_pages=max_pages)
         self._h = self._lib.eahmmf_pages_create(n_pages, page, n_seq, max_pages)
         if not self._h:
             raise RuntimeError("eahmmf_pages_create failed")
@@ -725,15 +748,19 @@ class Pages:
             raise RuntimeError(f"eahmmf_pages_{name} returned {rc}")
 
     def extend(self, seq: int, length: int) -> None:
+        _ints(seq=seq, length=length)
         self._call("extend", seq, length)
 
     def fork(self, src: int, dst: int) -> None:
+        _ints(src=src, dst=dst)
         self._call("fork", src, dst)
 
     def truncate(self, seq: int, length: int = 0) -> None:
+        _ints(seq=seq, length=length)
         self._call("truncate", seq, length)
 
     def slide(self, seq: int, first_pos: int, n_sink: int = 0) -> None:
+        _ints(seq=seq, first_pos=first_pos, n_sink=n_sink)
         self._call("slide", seq, first_pos, n_sink)
 
     def compact(self) -> None:
@@ -759,7 +786,7 @@ class Pages:
         return self._lib.eahmmf_pages_free_count(self._h)
 
     def refs(self, page_id: int) -> int:
-        return self._lib.eahmmf_pages_refs(self._h, page_id)
+        return self._lib.eahmmf_pages_refs(self._h, page_id) if _fit(page_id) else -1
 
 
 def hash64(data) -> int:

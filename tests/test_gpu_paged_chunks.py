@@ -240,3 +240,21 @@ def test_chunk_scores_past_24_bits(torch, type, hd, grp, lens, e):
 @pytest.mark.parametrize("e", [8, 14, 15, 16, 17, 18, 20, 23, 26, 40, 80])
 def test_step_scores_past_24_bits(torch, type, hd, grp, lens, e):
     far_scores(torch, type, hd, grp, lens, e)
+
+
+def test_calls_refuse_numbers_past_32_bits(torch):
+    c = Chunks(torch, "f16", 64, 1, 2, 16, [20], [30], seed=9)
+    first = c.check(window=7)
+    far = 1 << 32
+    for o in (dict(window=far), dict(window=far + 7), dict(window=7, n_sink=far)):
+        with pytest.raises(ValueError):
+            c.attention(**o)
+    with pytest.raises(ValueError):
+        c.cache.attention(far, c.batch, c.q, c.n_head, c.out, ws=c.ws)
+    rope = eb.Rope(torch.ones(32, device="cuda"))
+    with pytest.raises(ValueError):
+        c.cache.append(far, c.batch, torch.zeros(20, 4 * 64, device="cuda"), c.n_head, rope, c.out)
+    for o in ((far + 20, 20, 30), (20, far + 20, 30), (20, 20, far)):
+        with pytest.raises(ValueError):
+            eb.PagedBatch(c.table, c.batch._keep[1], c.batch._keep[2], *o)
+    assert torch.equal(c.attention(window=7).double(), first)
