@@ -60,11 +60,12 @@ class ContinuousBatcher:
         while free and self.queue and len(self.active) < self.max_rows:
             if self.pages and sum(map(self._need, self.active.values())) + self._need(self.queue[0]) > self.pages:
                 break
-            r = self.queue.popleft()
-            r.slot = free.pop(0)
-            rc, first = self.e.prefill_slot(r.slot, r.prompt, self.n_batch)
-            if rc:
+            r = self.queue[0]
+            rc, first = self.e.prefill_slot(free[0], r.prompt, self.n_batch)
+            if rc:  # the request stays at the head of the queue
                 raise RuntimeError(f"eahmmf_engine_prefill_slot returned {rc}")
+            self.queue.popleft()
+            r.slot = free.pop(0)
             r.tokens.append(first)
             r.pos = len(r.prompt)
             if len(r.tokens) < r.n_gen:

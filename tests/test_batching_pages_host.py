@@ -27,3 +27,26 @@ def test_the_whole_prompt_is_counted(page, n_gen):
     later = b.submit([1] * (page + 1), n_gen)  # two: not beside it
     b.run()
     assert first.tokens == [1, 1] and len(later.tokens) == max(n_gen, 1) and not b.queue
+
+
+@pytest.mark.parametrize("pages", [0, 4])
+def test_a_refused_prefill_leaves_the_request_in_the_queue(pages):
+    class Refusing(Strict):
+        refuse = True
+
+        def set_slots(self, n):
+            return self.set_paged(n, 1 << 20, 16, "f16")
+
+        def prefill_slot(self, slot, prompt, n_batch):
+            return (eb.ST_CAPACITY, 0) if self.refuse else super().prefill_slot(slot, prompt, n_batch)
+
+    e = Refusing()
+    b = batching.ContinuousBatcher(e, n_slots=2, pages=pages, page=16)
+    rs = [b.submit([1] * n, 3) for n in (5, 9)]
+    for _ in range(2):
+        with pytest.raises(RuntimeError):
+            b.step()
+        assert list(b.queue) == rs and not b.active and all(not r.tokens for r in rs)
+    e.refuse = False
+    b.run()
+    assert [len(r.tokens) for r in rs] == [3, 3]
