@@ -648,8 +648,9 @@ class PagedCache:
     def _rows(self, x, name: str, batch, width: int):
         shape, stride = x.shape, x.stride()
         if (x.dtype is not self._f32 or x.get_device() != self._idx or len(shape) != 2 or shape[0] < batch.n_tok
-                or shape[1] != width or stride[1] != 1):
-            raise ValueError(f"{name}: float32 rows [{batch.n_tok} x {width}] on {self.device} are needed")
+                or shape[1] != width or stride[1] != 1 or stride[0] >> 31):
+            raise ValueError(f"{name}: float32 rows [{batch.n_tok} x {width}] on {self.device} are needed, less than 2^31 elements "
+                             "apart")
         return x.data_ptr(), stride[0] if shape[0] > 1 else width
 
     def _status(self, t):

@@ -258,3 +258,12 @@ def test_calls_refuse_numbers_past_32_bits(torch):
         with pytest.raises(ValueError):
             eb.PagedBatch(c.table, c.batch._keep[1], c.batch._keep[2], *o)
     assert torch.equal(c.attention(window=7).double(), first)
+
+
+def test_rows_too_far_apart_are_refused(torch):
+    c = Chunks(torch, "f16", 64, 1, 2, 16, [2], [30], seed=9)
+    w = c.q.shape[1]
+    far = torch.empty((1 << 32) + 2 * w, device="cuda").as_strided((2, w), ((1 << 32) + w, 1))  # w apart, modulo 2^32
+    for q, out in ((far, c.out), (c.q, far)):
+        with pytest.raises(ValueError):
+            c.cache.attention(0, c.batch, q, c.n_head, out, ws=c.ws)
