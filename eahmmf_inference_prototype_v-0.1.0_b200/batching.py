@@ -9,7 +9,9 @@ the next request at once. Greedy selection; per-sequence tokens equal that seque
 
 With `pages` the slots share a paged cache (eahmmf_engine_set_paged): a request is admitted when the pages
 for its prompt and all of its tokens are free beside those that the running ones will still take, and its
-pages go back when it leaves.
+pages go back when it leaves. Keys and values are then held in 16 bits unless dtype is "f32" (contiguous slots
+hold 32), and attention sums over a batch's pages in an order that depends on the batch: tokens equal those of
+the sequence alone in the same kind of cache up to the rounding of a logit.
 """
 from __future__ import annotations
 

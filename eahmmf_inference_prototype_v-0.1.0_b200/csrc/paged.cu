@@ -210,7 +210,8 @@ __global__ void __launch_bounds__(CP_NT) k_pages_copy(uint4* __restrict__ k, uin
 // Up to 8 rows (STACK) the two parts of a row lie in rows g and g + 8 of one instruction: no extra work, and the
 // thread that holds row g holds row g + 8 too. 16 rows take an instruction for each part.
 constexpr int PA_NW = 4, PA_NT = 32 * PA_NW;
-constexpr int STEP_BLOCKS = 3;  // blocks an SM holds, by registers and by the rings' shared memory: all run at once
+constexpr int STEP_BLOCKS = 3;  // blocks an SM holds, by registers and by the rings' shared memory: all run at once (but for 9 to 16
+                                // rows over 32-bit pages with heads of 128, whose 82 KB let two run and the rest follow)
 constexpr float P_SHIFT = 15.f;
 
 template <typename T>
@@ -308,7 +309,6 @@ struct AttnSmem {
     uint8_t ring[PA_NW][NS][2][TILE];                             // at a tile's end the warp's sums [RT][HD + 4]
     uint4 qf[STACK ? 1 : KS * 32 * 2];                            // 16 rows: q in fragment order, hi then lo
     float m[PA_NW][RT], l[PA_NW][RT];
-    float cs[RT];  // score scale of each row
 };
 
 // A partial record: o [16][hd], m [16], sum [16].

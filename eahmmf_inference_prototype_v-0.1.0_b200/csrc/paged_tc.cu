@@ -13,9 +13,9 @@
 //
 // Bound: 4 hd flops per row and position, twice because of the two parts: 2 * 2 * 2 * 128 * 128 * hd per tile and unit. Two
 // tiles share every k and v tile and take turns: while one tile's scores are in the softmax the other's products run.
-// 4,096 tokens over 12,289 positions, 32 q heads of 128 on 4 kv heads, 16-bit pages: 985 us in a burst (1,397 TFLOP/s of both parts),
-// 1,158 back to back, where the power cap holds the clock at 1.55 GHz. 64 tokens over 2,111 positions of 32-bit pages: 35 us,
-// two units a block, most of it start, q and joining.
+// 4,096 tokens over 12,289 positions, 32 q heads of 128 on 4 kv heads, 16-bit pages: 1,037 us in a burst (1,327 TFLOP/s of both
+// parts), 1,200 back to back, where the power cap holds the clock at 1.52 to 1.64 GHz. 64 tokens over 2,111 positions of 32-bit
+// pages: 36 us, two units a block, most of it start, q and joining.
 //
 // Warps: 0-3 softmax of tile 0, 4-7 of tile 1 (thread = row = tensor-memory lane), 8 loads k, 11 loads v, 9 issues q k, 10 issues
 // p v (one warp for both products left the tensor cores idle a third of the time: each wait costs it some 150 cycles). 32-bit
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
             const int low = A.window > 0 ? max(0, max(lim, 0) - A.window + 1) : 0;
             // ---- q: every row scaled by the power of two that brings its largest element to [2^14, 2^15), then split. The low
             // parts are exact to 2^-25 of that: an element is held to 2^-22 of itself or 2^-39 of its row's largest. (One scale for a
-            // warp's rows would let a large row take the bits of the small ones beside it.) Rows come one (hd 128) or two (hd 64)
+            // warp's rows, which let a large row take the bits of the small ones beside it, was 0.7 % faster over a long prompt.) Rows come one (hd 128) or two (hd 64)
             // to a load instruction.
             float cs;
             {
@@ -539,7 +539,8 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
                 alpha = mn == -INFINITY ? 1.f : ex2(m - mn);
                 m = mn;
                 // c S - (m - 15) in one rounding, of which c S loses none: where m itself is rounded by more than a little (from
-                // 2^22 an eighth), the largest weight would miss 2^15 and overflow. Such scores are rounded first, as m was.
+                // 2^22 an eighth), the largest weight would miss 2^15 and overflow. Such scores are rounded first, as m was. To
+                // look for them costs 0.8 % of a long prompt.
                 float c1 = csu, mo = mn == -INFINITY ? 0.f : mn - 15.f;
                 const bool far = mn != -INFINITY && fabsf(mn) >= 4194304.f;
                 if (__any_sync(0xffffffffu, far)) {
@@ -644,9 +645,9 @@ __global__ void __launch_bounds__(Tc<HD, F32>::NT, 1) k_paged_attn_tc(PagedAttnA
         regs_less<C::REGS_LOAD>();
         // ---------------------------------------------------------------- k and v tiles of 32-bit pools
         // Eight warps, 16 positions each (of one page): read, scaled by the power of two that brings the tile's largest element to
-        // [2^14, 2^15), split in two 11-bit parts. What the parts leave out is 2^-39 of the tile's largest element, or 2^-22 of the
-        // element itself, whichever is more: an absolute error of a score or an output far below that of 32 bits. Positions that
-        // no row sees are not read: their rows are zero.
+        // [2^14, 2^15), split in two 11-bit parts. What the parts leave out of an element is 2^-39 of the tile's largest, or 2^-22 of
+        // the element itself, whichever is more: below the rounding of 32 bits for a score of elements of one size, and for the
+        // columns of v that are not 2^-16 of the tile's largest or less. Positions that no row sees are not read: their rows are zero.
         constexpr int LPR = HD / 4, RPP = 32 / LPR, N = 16 / RPP;
         const int cw = warp - C::W_LOAD, el = lane % LPR, sub = lane / LPR;
         uint32_t n = 0, n_valid = 0;

@@ -392,7 +392,8 @@ class Engine:
         return lib().eahmmf_engine_set_slots(self._h, n)
 
     def set_paged(self, n_slots: int, n_pages: int, page: int = 64, dtype: str = "f16") -> int:
-        """eahmmf_engine_set_paged: the slots share a cache of n_pages pages ("f16" or "f32")."""
+        """eahmmf_engine_set_paged: the slots share a cache of n_pages pages, in 16 bits ("f16") or in the contiguous
+        cache's 32 ("f32")."""
         if not _fit(n_slots, n_pages, page):
             return ST_BAD_ARG
         return lib().eahmmf_engine_set_paged(self._h, n_slots, n_pages, page, {"f32": 0, "f16": 1}[dtype])
@@ -595,8 +596,8 @@ def _ints(**values) -> None:
 
 class PagedBatch:
     """The sequences of one call (EahmmfPagedSeqs): int32 device tensors table [n_seq x ld], cu_q [n_seq + 1] and
-    kv_len [n_seq]; rows of activations and the bounds max_q, max_kv of their lengths (they choose kernels, results do
-    not depend on them). The tensors may be rewritten between calls; the object keeps their addresses."""
+    kv_len [n_seq]; rows of activations and the bounds max_q, max_kv of their lengths (they choose kernels, and with them
+    the order of sums, nothing else). The tensors may be rewritten between calls; the object keeps their addresses."""
 
     def __init__(self, table, cu_q, kv_len, n_tok: int, max_q: int, max_kv: int):
         for t, n in ((table, "table"), (cu_q, "cu_q"), (kv_len, "kv_len")):

@@ -280,12 +280,15 @@ int eahmmf_cuda_rope_append(const EahmmfPagedKv* kv, int layer, const EahmmfPage
  * h / (n_head / n_kv), out = softmax(scale q k^T) v over the positions j <= p of the row at p, and, where window > 0,
  * of those j > p - window or j < n_sink. A row that sees nothing is zero. Positions that no row of a sequence's call
  * sees may hold anything; a NaN or an infinity in v at a position that a later row of the same call sees can reach
- * earlier rows of that sequence. n_head a multiple of n_kv, at most 64 q heads per kv head; row strides multiples of 4,
- * buffers 16-byte aligned, d_out not overlapping d_q. Over 32-bit pages the products of more than 16 rows (tokens x q heads of
- * a kv head) hold an element of k and v to 2^-22 of itself or 2^-39 of the largest among its 128 positions, whichever is more.
- * An element of q is held to 2^-22 of itself or 2^-33 of the largest of its row (a token's head), whichever is more.
- * Elements of q, k and v stay below 2^100. The workspace (256-byte aligned) is written and read within the call: calls that may run at
- * the same time need one each. Asynchronous; results do not depend on what else runs. */
+ * earlier rows of that sequence. A NaN in q or in a k that a row sees makes the row NaN, and an infinity there may.
+ * n_head a multiple of n_kv, at most 64 q heads per kv head; row strides multiples of 4, buffers 16-byte aligned, d_out
+ * not overlapping d_q.
+ * Precision: sums are 32-bit; an element of q is held to 2^-22 of itself or 2^-33 of the largest of its row (a token's
+ * head), whichever is more; over 32-bit pages an element of k and v to 2^-21 of itself, and in sequences of more than 16 rows
+ * (tokens x q heads of a kv head) to 2^-22 of itself or 2^-39 of the largest among its 128 positions, whichever is more.
+ * Elements of q and k stay below 2^100, of v below 2^80, scores below 2^126.
+ * The workspace (256-byte aligned) is written and read within the call: calls that may run at the same time need one
+ * each. Asynchronous; results do not depend on what else runs. */
 size_t eahmmf_cuda_paged_attention_workspace_bytes(const EahmmfPagedKv* kv, const EahmmfPagedSeqs* seqs, int n_head);
 int eahmmf_cuda_paged_attention(const EahmmfPagedKv* kv, int layer, const EahmmfPagedSeqs* seqs, int n_head,
                                 const float* d_q, int ldq, float scale, int window, int n_sink, float* d_out, int ldo,
